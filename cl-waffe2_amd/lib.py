@@ -29,6 +29,8 @@ EQ, LT, LE, GT, GE = 0, 1, 2, 3, 4  # enum wf2hip_compare_op
 COMPARE_NAMES = ("eq", "lt", "le", "gt", "ge")
 MAXVALUE, MINVALUE, ARGMAX, ARGMIN = 48, 49, 50, 51  # enum wf2hip_select_op
 
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2  # enum wf2hip_reduction
+
 EINVAL = -1
 EOVERLAP = -3
 EUNSUPPORTED = -4
@@ -195,6 +197,8 @@ _SIGNATURES = {
     "wf2hip_sgd_step_f32": ([_L, _P, _P, _F], C.c_int),
     "wf2hip_adam_step_f32": ([_L, _P, _P, _P, _P, _F, _F, _F, _F], C.c_int),
     "wf2hip_embedding_add_f32": ([_L, _L, _L, _P, _P, _L, _P, _L, _P], C.c_int),
+    "wf2hip_linear_cross_entropy_f32": ([_L] * 3 + [_P] * 3 + [C.c_int] + [_P] * 2, C.c_int),
+    "wf2hip_linear_cross_entropy_backward_f32": ([_L] * 3 + [_P] * 4 + [C.c_int, _P, _F] + [_P] * 2, C.c_int),
     "wf2hip_attention_f32": ([C.POINTER(AttentionDesc), _P, _P, _P, _P], C.c_int),
     "wf2hip_attention_forward_f32": ([C.POINTER(AttentionDesc), _P, _P, _P, _P, _P], C.c_int),
     "wf2hip_attention_backward_f32": ([C.POINTER(AttentionDesc)] + [_P] * 9, C.c_int),

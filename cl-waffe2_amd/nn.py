@@ -173,3 +173,48 @@ def softmax_cross_entropy_backward_fused(dy, z: HIPTensor, labels: HIPTensor, in
     full = list(dy.shape) == list(z.shape)
     dx = dy if (in_place and full) else HIPTensor(list(z.shape), initial_element=None)
     return nodes.forward("HIP-Softmax-Cross-Entropy-Node-backward", dy, z, labels, dx)
+
+
+def linear_cross_entropy(x: HIPTensor, w: HIPTensor, labels: HIPTensor, reduction: str | None = "mean",
+                         loss: HIPTensor | None = None, lse: HIPTensor | None = None):
+    """Softmax cross entropy of the logits ``(!matmul x (!t w))`` against token ids as ONE node
+    (HIP-Linear-Cross-Entropy-Node), without the logits: the lm-head of a language model
+    (``examples/gpt-2/model.lisp:137-196``) and its criterion, ``loss = logsumexp(x . w^T) - x . w[label]``.
+    ``x[~ dim]`` are hidden states, ``w[vocab dim]`` the token table, ``labels[~]`` :int32 token ids; a negative
+    id leaves its position out (loss 0, no gradient).  ``reduction``: None (one loss per position), 'sum' or
+    'mean' (over the positions that count).  Returns ``(loss, lse)``; ``lse``, one number per position, is what
+    :func:`linear_cross_entropy_backward` needs.  Given ``loss`` / ``lse`` tensors are written."""
+    x2, labels1 = F.reshape(x, -1, x.shape[-1]), F.reshape(labels, -1)
+    rows = x2.shape[0]
+    if lse is None:
+        lse = HIPTensor([rows], initial_element=None)
+    if loss is None:
+        loss = HIPTensor(list(labels.shape) if reduction is None else [1], initial_element=None)
+    nodes.forward("HIP-Linear-Cross-Entropy-Node", x2, F.to_contiguous(w), labels1, _as_rows(loss, "loss"),
+                  _as_rows(lse, "lse"), reduction)
+    return loss, lse
+
+
+def linear_cross_entropy_backward(dy, x: HIPTensor, w: HIPTensor, labels: HIPTensor, lse: HIPTensor,
+                                  reduction: str | None = "mean", dx: HIPTensor | None = None,
+                                  dw: HIPTensor | None = None):
+    """``(dx, dw)`` of :func:`linear_cross_entropy` from its inputs and its ``lse``.  ``dy``: the gradient of the
+    loss, a tensor of the loss's shape or a number.  Given ``dx`` / ``dw`` tensors are overwritten."""
+    x2, labels1 = F.reshape(x, -1, x.shape[-1]), F.reshape(labels, -1)
+    if dx is None:
+        dx = HIPTensor(list(x.shape), initial_element=None)
+    if dw is None:
+        dw = HIPTensor(list(w.shape), initial_element=None)
+    if not dx.is_contiguous() or list(dx.shape) != list(x.shape):
+        raise ValueError(f"linear_cross_entropy_backward: dx must be a contiguous tensor of shape {x.shape}")
+    dout = F.reshape(dy, -1) if isinstance(dy, HIPTensor) else None
+    nodes.forward("HIP-Linear-Cross-Entropy-Node-backward", x2, F.to_contiguous(w), labels1, _as_rows(lse, "lse"), dout,
+                  HIPTensor(list(x2.shape), vec=dx.vec), dw, reduction, 1.0 if dout is not None else float(dy))
+    return dx, dw
+
+
+def _as_rows(t: HIPTensor, what: str) -> HIPTensor:
+    """An output (or saved) tensor as one axis, without a copy."""
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous tensor that owns its storage")
+    return t if t.ndim == 1 else HIPTensor([t.size], vec=t.vec, dtype=t.dtype)

@@ -38,10 +38,11 @@ NODE_NAMES = (
     # the define-op nodes of lisp/fusion.lisp (one kernel each)
     "HIP-Sum-Node", "HIP-Activation-Node", "HIP-Softmax-Node", "HIP-LayerNorm-Node", "HIP-Linear-Node",
     "HIP-Linear-Residual-Node", "HIP-Causal-Softmax-Node", "HIP-Attention-Node", "HIP-Softmax-Cross-Entropy-Node",
-    "HIP-Unfold-Node",
+    "HIP-Unfold-Node", "HIP-Linear-Cross-Entropy-Node",
     # the -backward nodes define-op generates for them, where the backward is one kernel too
     "HIP-Activation-Node-backward", "HIP-Softmax-Node-backward", "HIP-Causal-Softmax-Node-backward",
     "HIP-LayerNorm-Node-backward", "HIP-Attention-Node-backward", "HIP-Softmax-Cross-Entropy-Node-backward",
+    "HIP-Linear-Cross-Entropy-Node-backward",
     # the node of the reference's GPT-2 example (examples/gpt-2/utils.lisp:68-72)
     "GPT2PositionalEmbedding",
 )
@@ -615,6 +616,60 @@ def _softmax_cross_entropy_backward_node(dout: HIPTensor, z: HIPTensor, labels: 
                                                                    C.c_void_p(z.ptr), C.c_void_p(labels.ptr), batch,
                                                                    C.c_void_p(dx.ptr)))
     return dx
+
+
+_REDUCTIONS = {None: _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
+
+
+def _require_labels(name: str, x: HIPTensor, w: HIPTensor, labels: HIPTensor, lse: HIPTensor, reduction) -> int:
+    """Checks what both directions of HIP-Linear-Cross-Entropy-Node read; returns the number of rows."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{name}: reduction must be None, 'sum' or 'mean', got {reduction!r}")
+    if len(x.shape) != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"{name}: x[rows dim] and w[vocab dim] expected, got {x.shape} and {w.shape}")
+    rows = x.shape[0]
+    _require_rows(f"{name}: x", x)
+    _require_rows(f"{name}: w", w)
+    _require_rows(f"{name}: lse", lse, [rows])
+    if labels.dtype != "int32":
+        raise ValueError(f"{name}: labels must be :int32 token ids, got :{labels.dtype}")
+    if not labels.is_contiguous() or list(labels.shape) != [rows]:
+        raise ValueError(f"{name}: labels must be {rows} contiguous token ids, got shape {labels.shape}")
+    return rows
+
+
+@define_impl("HIP-Linear-Cross-Entropy-Node", HIPTensor, _only_float)
+def _linear_cross_entropy_node(x: HIPTensor, w: HIPTensor, labels: HIPTensor, loss: HIPTensor, lse: HIPTensor,
+                               reduction: str | None = "mean") -> HIPTensor:
+    """``X[rows dim] W[vocab dim] Labels[rows] LOSS LSE[rows] -> LOSS``: softmax cross entropy of the logits
+    x . w^T against token ids, without the logits.  LOSS has one element per row (reduction None) or one."""
+    name = "HIP-Linear-Cross-Entropy-Node"
+    rows = _require_labels(name, x, w, labels, lse, reduction)
+    _require_rows(f"{name}: loss", loss, [rows] if reduction is None else [1])
+    _lib.check(_lib.get().wf2hip_linear_cross_entropy_f32(rows, x.shape[1], w.shape[0], C.c_void_p(x.ptr),
+                                                         C.c_void_p(w.ptr), C.c_void_p(labels.ptr),
+                                                         _REDUCTIONS[reduction], C.c_void_p(loss.ptr),
+                                                         C.c_void_p(lse.ptr)))
+    return loss
+
+
+@define_impl("HIP-Linear-Cross-Entropy-Node-backward", HIPTensor, _only_float)
+def _linear_cross_entropy_backward_node(x: HIPTensor, w: HIPTensor, labels: HIPTensor, lse: HIPTensor,
+                                        dout: HIPTensor | None, dx: HIPTensor, dw: HIPTensor,
+                                        reduction: str | None = "mean", scale: float = 1.0):
+    """``X W Labels LSE DOUT DX[rows dim] DW[vocab dim] -> DX DW``.  DOUT: the gradient of the loss, of its shape,
+    or None for ones; both times ``scale``."""
+    name = "HIP-Linear-Cross-Entropy-Node-backward"
+    rows = _require_labels(name, x, w, labels, lse, reduction)
+    _require_rows(f"{name}: dx", dx, x.shape)
+    _require_rows(f"{name}: dw", dw, w.shape)
+    if dout is not None:
+        _require_rows(f"{name}: dout", dout, [rows] if reduction is None else [1])
+    _lib.check(_lib.get().wf2hip_linear_cross_entropy_backward_f32(
+        rows, x.shape[1], w.shape[0], C.c_void_p(x.ptr), C.c_void_p(w.ptr), C.c_void_p(labels.ptr),
+        C.c_void_p(lse.ptr), _REDUCTIONS[reduction], None if dout is None else C.c_void_p(dout.ptr), float(scale),
+        C.c_void_p(dx.ptr), C.c_void_p(dw.ptr)))
+    return dx, dw
 
 
 @define_impl("HIP-LayerNorm-Node", HIPTensor, _only_float)

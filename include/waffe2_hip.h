@@ -829,6 +829,31 @@ int wf2hip_attention_backward_f32(const wf2hip_attention_desc* desc, const float
                                   const float* v, const float* o, const float* dout,
                                   const float* lse, float* dq, float* dk, float* dv);
 
+/* ---- a language model's loss ------------------------------------------------- */
+/* Softmax cross entropy over a vocabulary from the hidden states x(rows, dim) and the token
+ * table w(vocab, dim), without the (rows, vocab) logits: with s = x . w^T,
+ *   lse[n] = log sum_v exp s[n, v],   loss[n] = lse[n] - s[n, labels[n]].
+ * It stands for the lm-head product (examples/gpt-2/model.lisp:137-196) followed by
+ * Softmax-Cross-Entropy-Node (source/nn/criterion.lisp:82-196), whose labels are one-hot
+ * matrices there and token ids here (delta = 0).  A label below 0 leaves its row out: loss 0, gradient 0,
+ * whatever the row of x holds (lse is still that of the row).  A label of vocab or more has no
+ * logit: its loss is NaN, and so are the gradients.  reduction: the losses one by one
+ * (loss has `rows` elements), their sum, or their mean over the rows that have a label (loss has
+ * one element; the mean of no rows is NaN).  lse(rows) is what the backward needs.  All arrays contiguous; the
+ * outputs overlap nothing else.  dim, vocab >= 1; every extent below 2^31.  Scratch comes from the
+ * library's pool. */
+enum wf2hip_reduction { WF2HIP_REDUCE_NONE = 0, WF2HIP_REDUCE_SUM = 1, WF2HIP_REDUCE_MEAN = 2 };
+int wf2hip_linear_cross_entropy_f32(long rows, long dim, long vocab, const float* x, const float* w,
+                                    const int32_t* labels, int reduction, float* loss, float* lse);
+/* Its gradients from the same inputs and the forward's lse: with
+ *   ds[n, v] = g[n] (exp(s[n, v] - lse[n]) - [v = labels[n]]),   dx = ds . w,   dw = ds^T . x
+ * (both overwritten), g[n] = scale * dloss[n] (reduction none), scale * dloss[0] (sum), the same over the number
+ * of rows with a label (mean); dloss NULL stands for ones. */
+int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long vocab, const float* x,
+                                             const float* w, const int32_t* labels, const float* lse,
+                                             int reduction, const float* dloss, float scale, float* dx,
+                                             float* dw);
+
 /* ---- GPT-2 example: token + position embedding ------------------------------ */
 /* out[r, :] <- wte[round(ctx[r]), :] + wpe[r % seq, :] for r < rows (rows = sentences x seq):
  * the GPT2PositionalEmbedding node of examples/gpt-2/utils.lisp:19-110, which the example

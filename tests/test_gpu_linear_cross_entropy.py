@@ -1,0 +1,323 @@
+"""The language model's loss (HIP-Linear-Cross-Entropy-Node) and its gradients against float64.
+
+Tolerances.  An element of a product of K terms may be off by (K + 14) U sum |a||b|, U = 2^-24: K + 2 for binary32
+additions in any order and the last roundings; 12 for operands that go through the matrix cores as two numbers of 11 significant bits each
+(each operand is then within 2^-22 = 4 U of itself, the product of the two low parts, at most 2^-22, is left out).
+Those parts are kept relative to the largest number of the whole operand, in steps of 2^-24 where that is 2^14 or more: half
+a step is 2^-39 of the largest.  The row statistic adds 4 ulp of its own (exponential, sum, logarithm), log-sum-exp
+passes the logits' error on with weights that add up to one.  A probability carries the relative error of its
+exponent, err(s) + err(lse), plus 4 ulp."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+f32 = np.float32
+U = 2.0 ** -24
+
+
+def truth(x, w, labels, reduction, dy=None):
+    """loss, lse, dx, dw in float64 and the magnitudes their bounds go by."""
+    keep = labels >= 0
+    x = np.where(keep[:, None], x, 0).astype(np.float64)
+    w = w.astype(np.float64)
+    s = x @ w.T
+    mag = np.abs(x) @ np.abs(w).T
+    top = s.max(axis=1, keepdims=True)
+    e = np.exp(s - top)
+    lse = (top + np.log(e.sum(axis=1, keepdims=True)))[:, 0]
+    p = e / e.sum(axis=1, keepdims=True)
+    at = np.maximum(labels, 0)
+    rows = np.arange(len(x))
+    loss = np.where(keep, lse - s[rows, at], 0.0)
+    count = keep.sum()
+    if reduction is None:
+        g = (np.ones(len(x)) if dy is None else dy.astype(np.float64)) * keep
+    else:
+        one = 1.0 if dy is None else float(dy)
+        g = keep * (one / max(count, 1) if reduction == "mean" else one)
+    p[rows, at] -= 1.0
+    ds = p * g[:, None]
+    total = {None: loss, "sum": loss.sum(), "mean": loss.sum() / count if count else np.nan}[reduction]
+    return dict(loss=total, lse=lse, dx=ds @ w, dw=ds.T @ x, s=s, mag=mag, ds=ds, each=loss, g=g, keep=keep, x=x, w=w,
+                count=count)
+
+
+def bounds(t):
+    """Elementwise bounds for (each loss, lse, dx, dw)."""
+    dim, vocab, rows = t["x"].shape[1], t["w"].shape[0], t["x"].shape[0]
+    small = lambda a, b: 2.0 ** -39 * (np.abs(a).max(initial=0) * np.abs(b).sum(axis=0) +  # noqa: E731
+                                       np.abs(b).max(initial=0) * np.abs(a).sum(axis=1)[:, None])
+    err_s = (dim + 14) * U * t["mag"] + small(t["x"], t["w"].T)
+    err_lse = err_s.max(axis=1) + 4 * U * (np.abs(t["lse"]) + 1) + 4 * U + np.abs(t["s"] - t["lse"][:, None]).max(axis=1) * U
+    err_loss = err_lse + err_s.max(axis=1) + 2 * U * np.abs(t["s"]).max(axis=1)
+    onehot = t["ds"] + 0.0
+    p_err = (err_s + err_lse[:, None] + (4 + np.abs(t["s"] - t["lse"][:, None])) * U)
+    prob = np.exp(t["s"] - t["lse"][:, None])
+    err_ds = np.abs(t["g"])[:, None] * (prob * p_err + 4 * U * (prob + (np.abs(onehot) > 0) * U))
+    err_ds += 4 * U * np.abs(t["ds"])
+    err_dx = err_ds @ np.abs(t["w"]) + (vocab + 14) * U * (np.abs(t["ds"]) @ np.abs(t["w"])) + small(t["ds"], t["w"])
+    err_dw = err_ds.T @ np.abs(t["x"]) + (rows + 14) * U * (np.abs(t["ds"]).T @ np.abs(t["x"])) + small(t["ds"].T, t["x"])
+    return err_loss, err_lse, err_dx + 1e-37, err_dw + 1e-37
+
+
+def inputs(rows, dim, vocab, left_out=0.0, seed=0, sharp=1.0):
+    rng = np.random.default_rng(rows * 31 + dim * 7 + vocab + seed)
+    w = (rng.standard_normal((vocab, dim)) * 0.3).astype(f32)
+    labels = rng.integers(0, vocab, rows).astype(np.int32)
+    x = rng.standard_normal((rows, dim)) * sharp
+    if rows:
+        x += 3.0 * rng.random((rows, 1)) * w[labels] / np.maximum(np.linalg.norm(w[labels], axis=1, keepdims=True), 1e-3)
+    labels[rng.random(rows) < left_out] = -1
+    return x.astype(f32), w, labels
+
+
+def check(W, x, w, labels, reduction, dy=None):
+    F, nn = W.functional, W.nn
+    dx_, dw_ = F.from_numpy(x), F.from_numpy(w)
+    dl = F.from_numpy(labels, dtype="int32")
+    loss, lse = nn.linear_cross_entropy(dx_, dw_, dl, reduction=reduction)
+    up = 1.0 if dy is None else (F.from_numpy(dy) if isinstance(dy, np.ndarray) else dy)
+    gx, gw = nn.linear_cross_entropy_backward(up, dx_, dw_, dl, lse, reduction=reduction)
+    t = truth(x, w, labels, reduction, dy)
+    e_loss, e_lse, e_dx, e_dw = bounds(t)
+    assert np.all(np.abs(lse.numpy() - t["lse"])[t["keep"]] <= e_lse[t["keep"]])
+    if reduction is None:
+        assert np.all(np.abs(loss.numpy() - t["each"]) <= e_loss * t["keep"])
+    else:
+        share = 1.0 / max(t["count"], 1) if reduction == "mean" else 1.0
+        got = float(loss.numpy()[0])
+        if t["count"] == 0 and reduction == "mean":
+            assert np.isnan(got)
+        else:
+            assert abs(got - t["loss"]) <= share * (e_loss * t["keep"]).sum() + 2 * U * abs(t["loss"])
+    assert np.all(np.abs(gx.numpy() - t["dx"]) <= e_dx), np.max(np.abs(gx.numpy() - t["dx"]) / e_dx)
+    assert np.all(np.abs(gw.numpy() - t["dw"]) <= e_dw), np.max(np.abs(gw.numpy() - t["dw"]) / e_dw)
+    assert not gx.numpy()[~t["keep"]].any()
+    return loss, lse, gx, gw
+
+
+# one row, one word, one element; sizes around the tiles (16, 32, 64, 128, 256) on every axis; odd ones
+SHAPES = [(1, 1, 1), (1, 64, 300), (2, 3, 5), (24, 64, 300), (31, 33, 129), (33, 31, 127), (63, 65, 257), (64, 64, 256),
+          (65, 100, 1000), (128, 96, 512), (129, 130, 131), (255, 768, 1003), (257, 70, 2049), (513, 256, 640),
+          (1000, 770, 301), (3, 1600, 5003), (17, 8, 50257), (300, 17, 9001)]
+
+
+def test_truth_gradients_by_differences():
+    """The closed form that the kernels are held against: its gradients by central differences."""
+    x, w, labels = inputs(7, 5, 11, left_out=0.3)
+    labels[0] = 4
+    for reduction, dy in (("mean", 1.5), ("sum", None), (None, np.linspace(0.5, 2.0, 7).astype(f32))):
+        t = truth(x, w, labels, reduction, dy)
+
+        def value(xx, ww):
+            r = truth(xx, ww, labels, reduction, dy)
+            each = r["each"]
+            if reduction is None:
+                return float((each * dy).sum())
+            return float(r["loss"]) * (1.0 if dy is None else dy)
+
+        h = 1e-3
+        x8, w8 = x.astype(np.float64), w.astype(np.float64)
+        for grad, which in ((t["dx"], 0), (t["dw"], 1)):
+            for i, j in ((0, 0), (3, 2), (6, 4)):
+                hi, lo = [x8.copy(), w8.copy()], [x8.copy(), w8.copy()]
+                hi[which][i, j] += h
+                lo[which][i, j] -= h
+                numeric = (value(*hi) - value(*lo)) / (2 * h)
+                assert abs(numeric - grad[i, j]) <= 1e-5 * max(1.0, abs(grad[i, j]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,vocab", SHAPES)
+@pytest.mark.parametrize("reduction", ["mean", None])
+def test_against_float64(gpu, rows, dim, vocab, reduction):
+    x, w, labels = inputs(rows, dim, vocab, left_out=0.2 if rows > 2 else 0.0)
+    dy = np.random.default_rng(rows).uniform(0.1, 2.0, rows).astype(f32) if reduction is None else None
+    check(gpu, x, w, labels, reduction, dy)
+
+
+@pytest.mark.gpu
+def test_sum_and_upstream_number(gpu):
+    x, w, labels = inputs(70, 48, 777, left_out=0.1)
+    check(gpu, x, w, labels, "sum", 0.25)
+    check(gpu, x, w, labels, "mean", -3.0)
+    # the upstream gradient as one number on the device
+    F, nn = gpu.functional, gpu.nn
+    d = [F.from_numpy(x), F.from_numpy(w), F.from_numpy(labels, dtype="int32")]
+    _, lse = nn.linear_cross_entropy(*d, reduction="mean")
+    a = nn.linear_cross_entropy_backward(-3.0, *d, lse)
+    b = nn.linear_cross_entropy_backward(F.from_numpy(np.array([-3.0], f32)), *d, lse)
+    for p, q in zip(a, b):
+        assert np.array_equal(p.numpy(), q.numpy())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,vocab", [(40, 64, 300), (300, 130, 1111)])
+def test_rows_left_out_hold_anything(gpu, rows, dim, vocab):
+    """NaN, infinities and the largest numbers in rows without a label change nothing elsewhere."""
+    W = gpu
+    x, w, labels = inputs(rows, dim, vocab, left_out=0.3)
+    clean = check(W, x, w, labels, "mean")
+    dirty = x.copy()
+    out = np.flatnonzero(labels < 0)
+    dirty[out[0]] = np.nan
+    dirty[out[1]] = np.inf
+    dirty[out[2]] = 3e38
+    dirty[out[3], 0] = -np.inf
+    labels2 = labels.copy()
+    labels2[out] = [-1, -100, -2 ** 31, -7] + [-1] * (len(out) - 4)
+    got = check(W, dirty, w, labels2, "mean")
+    for a, b in ((clean[0], got[0]), (clean[2], got[2]), (clean[3], got[3])):
+        assert np.array_equal(a.numpy(), b.numpy())
+
+
+@pytest.mark.gpu
+def test_all_rows_left_out_and_no_rows(gpu):
+    W = gpu
+    F, nn = W.functional, W.nn
+    x, w, _ = inputs(9, 20, 50)
+    labels = np.full(9, -1, np.int32)
+    check(W, x, w, labels, "mean")
+    check(W, x, w, labels, "sum")
+    check(W, x, w, labels, None, np.ones(9, f32))
+    for reduction, want in (("sum", 0.0), ("mean", np.nan)):
+        e = W.HIPTensor([0, 20])
+        l = W.HIPTensor([0], dtype="int32")
+        loss, lse = nn.linear_cross_entropy(e, F.from_numpy(w), l, reduction=reduction)
+        assert np.array_equal(loss.numpy(), np.array([want], f32), equal_nan=True) and lse.shape == [0]
+        dw = F.from_numpy(np.ones_like(w))
+        dx, dw = nn.linear_cross_entropy_backward(1.0, e, F.from_numpy(w), l, lse, reduction=reduction, dw=dw)
+        assert not dw.numpy().any() and dx.shape == [0, 20]
+
+
+@pytest.mark.gpu
+def test_label_behind_the_vocabulary_is_nan(gpu):
+    W = gpu
+    F, nn = W.functional, W.nn
+    x, w, labels = inputs(40, 24, 100)
+    labels[7] = 100
+    labels[11] = 2 ** 31 - 1
+    d = [F.from_numpy(x), F.from_numpy(w), F.from_numpy(labels, dtype="int32")]
+    each, lse = nn.linear_cross_entropy(*d, reduction=None)
+    bad = np.isnan(each.numpy())
+    assert list(np.flatnonzero(bad)) == [7, 11]
+    dx, dw = nn.linear_cross_entropy_backward(1.0, *d, lse, reduction=None)
+    assert np.isnan(dx.numpy()[[7, 11]]).all() and not np.isnan(np.delete(dx.numpy(), [7, 11], axis=0)).any()
+    assert np.isnan(dw.numpy()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale_x,scale_w", [(1e-3, 1e3), (1e4, 1e-5), (1e-18, 1e17), (2e-30, 1.0), (0.0, 1.0), (1e20, 1e-20)])
+def test_sizes_of_numbers(gpu, scale_x, scale_w):
+    """Hidden states and tables of any size whose logits are ordinary."""
+    x, w, labels = inputs(50, 40, 333)
+    check(gpu, (x * scale_x).astype(f32), (w * scale_w).astype(f32), labels, "mean")
+
+
+@pytest.mark.gpu
+def test_confident_and_spread_rows(gpu):
+    """Logits far apart: probabilities that underflow, losses near zero and very large ones."""
+    x, w, labels = inputs(60, 32, 400, sharp=1.0)
+    x[:20] *= 30
+    x[20:30] = 0
+    x[30:40] = 50 * w[labels[30:40]]
+    check(gpu, x, w, labels, None, np.ones(60, f32))
+
+
+@pytest.mark.gpu
+def test_shapes_of_a_batch_and_views(gpu):
+    """(batch, seq, dim) hidden states; windows of wider tensors are materialised by the wrapper."""
+    W = gpu
+    F, nn = W.functional, W.nn
+    x, w, labels = inputs(60, 24, 90, left_out=0.1)
+    loss, lse = nn.linear_cross_entropy(F.from_numpy(x.reshape(5, 12, 24)), F.from_numpy(w),
+                                        F.from_numpy(labels.reshape(5, 12), dtype="int32"), reduction=None)
+    want = nn.linear_cross_entropy(F.from_numpy(x), F.from_numpy(w), F.from_numpy(labels, dtype="int32"), reduction=None)
+    assert loss.shape == [5, 12]
+    assert np.array_equal(loss.numpy().ravel(), want[0].numpy())
+    wide = np.zeros((60, 30), f32)
+    wide[:, 3:27] = x
+    tall = np.zeros((24, 90), f32)
+    tall[:] = w.T
+    got = nn.linear_cross_entropy(F.from_numpy(wide).view(True, (3, 27)), F.from_numpy(tall).permute(1, 0),
+                                  F.from_numpy(labels, dtype="int32"), reduction=None)
+    assert np.array_equal(got[0].numpy(), want[0].numpy())
+    dx, dw = nn.linear_cross_entropy_backward(1.0, F.from_numpy(x.reshape(5, 12, 24)), F.from_numpy(w),
+                                              F.from_numpy(labels.reshape(5, 12), dtype="int32"), lse, reduction=None)
+    assert dx.shape == [5, 12, 24] and dw.shape == [90, 24]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,vocab", [(48, 64, 300), (700, 96, 2100)])
+def test_replayed_graph_equals_eager(gpu, rows, dim, vocab):
+    W = gpu
+    F, nn = W.functional, W.nn
+    x, w, labels = inputs(rows, dim, vocab, left_out=0.1)
+    dx_, dw_, dl = F.from_numpy(x), F.from_numpy(w), F.from_numpy(labels, dtype="int32")
+    outs = [W.HIPTensor([1]), W.HIPTensor([rows]), W.HIPTensor([rows, dim]), W.HIPTensor([vocab, dim])]
+
+    def step():
+        nn.linear_cross_entropy(dx_, dw_, dl, loss=outs[0], lse=outs[1])
+        nn.linear_cross_entropy_backward(1.0, dx_, dw_, dl, outs[1], dx=outs[2], dw=outs[3])
+
+    step()
+    eager = [t.numpy() for t in outs]
+    with W.lib.Graph() as g:
+        step()
+    for i in range(3):
+        for t in outs:
+            F.mul_(t, 0.0)
+        g.launch()
+        for a, t in zip(eager, outs):
+            assert np.array_equal(a, t.numpy()), f"replay {i}"
+        junk = F.exp(F.from_numpy(np.full((rows, dim), 0.5, f32)))
+        assert junk.numpy()[0, 0] == f32(np.exp(np.float64(0.5)))
+    x2, _, labels2 = inputs(rows, dim, vocab, left_out=0.2, seed=5)
+    F.move_(dx_, F.from_numpy(x2))
+    W.lib.check(W.lib.get().wf2hip_memcpy_d2d(C.c_void_p(dl.ptr), C.c_void_p(F.from_numpy(labels2, dtype="int32").ptr), 4 * rows))
+    g.launch()
+    replayed = [t.numpy() for t in outs]
+    step()
+    for a, t in zip(replayed, outs):
+        assert np.array_equal(a, t.numpy())
+    g.destroy()
+
+
+@pytest.mark.gpu
+def test_argument_checks(gpu):
+    W = gpu
+    F, nn = W.functional, W.nn
+    lib = W.lib.get()
+    x, w, dx, dw = (W.HIPTensor(s) for s in ([8, 16], [20, 16], [8, 16], [20, 16]))
+    labels, loss, lse = W.HIPTensor([8], dtype="int32"), W.HIPTensor([8]), W.HIPTensor([8])
+    p = lambda t: C.c_void_p(t.ptr)  # noqa: E731
+    fw, bw = lib.wf2hip_linear_cross_entropy_f32, lib.wf2hip_linear_cross_entropy_backward_f32
+    assert fw(8, 16, 20, p(x), p(w), p(labels), 0, p(loss), p(lse)) == 0
+    assert fw(-1, 16, 20, p(x), p(w), p(labels), 0, p(loss), p(lse)) == W.lib.EINVAL
+    assert fw(8, 0, 20, p(x), p(w), p(labels), 0, p(loss), p(lse)) == W.lib.EINVAL
+    assert fw(8, 16, 0, p(x), p(w), p(labels), 0, p(loss), p(lse)) == W.lib.EINVAL
+    assert fw(8, 16, 20, p(x), p(w), p(labels), 3, p(loss), p(lse)) == W.lib.EINVAL
+    assert fw(8, 16, 20, None, p(w), p(labels), 0, p(loss), p(lse)) == W.lib.EINVAL
+    assert fw(8, 16, 20, p(x), p(w), p(labels), 0, None, p(lse)) == W.lib.EINVAL
+    assert fw(2 ** 31, 16, 20, p(x), p(w), p(labels), 0, p(loss), p(lse)) == W.lib.EUNSUPPORTED
+    assert fw(8, 16, 20, p(x), p(w), p(labels), 0, p(x), p(lse)) == W.lib.EOVERLAP
+    assert fw(8, 16, 20, p(x), p(w), p(labels), 0, p(loss), p(loss)) == W.lib.EOVERLAP
+    assert bw(8, 16, 20, p(x), p(w), p(labels), p(lse), 2, None, 1.0, p(dx), p(dw)) == 0
+    assert bw(8, 16, 20, p(x), p(w), p(labels), p(lse), 2, None, 1.0, p(x), p(dw)) == W.lib.EOVERLAP
+    assert bw(8, 16, 20, p(x), p(w), p(labels), p(lse), 2, None, 1.0, p(dx), p(w)) == W.lib.EOVERLAP
+    assert bw(8, 16, 20, p(x), p(w), p(labels), p(lse), 2, None, 1.0, p(dx), p(dx)) == W.lib.EOVERLAP
+    assert bw(8, 16, 20, p(x), p(w), p(labels), p(lse), 0, p(dx), 1.0, p(dx), p(dw)) == W.lib.EOVERLAP
+    assert bw(8, 16, 20, p(x), p(w), p(labels), p(lse), 2, None, 1.0, None, p(dw)) == W.lib.EINVAL
+    for bad in (lambda: nn.linear_cross_entropy(x, W.HIPTensor([20, 15]), labels),
+                lambda: nn.linear_cross_entropy(x, w, W.HIPTensor([7], dtype="int32")),
+                lambda: nn.linear_cross_entropy(x, w, W.HIPTensor([8])),
+                lambda: nn.linear_cross_entropy(x, w, labels, reduction="max"),
+                lambda: nn.linear_cross_entropy(x, w, labels, reduction="mean", loss=loss),
+                lambda: nn.linear_cross_entropy(x, w, labels, lse=W.HIPTensor([9])),
+                lambda: nn.linear_cross_entropy_backward(1.0, x, w, labels, lse, dx=W.HIPTensor([8, 15])),
+                lambda: nn.linear_cross_entropy_backward(W.HIPTensor([3]), x, w, labels, lse, reduction=None)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(W.nodes.NodeNotFound):
+        nn.linear_cross_entropy(W.HIPTensor([8, 16], dtype="double"), w, labels)
