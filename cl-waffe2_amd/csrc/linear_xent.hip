@@ -6,77 +6,325 @@
 //
 // What the reference composes from !matmul, !softmax and cross-entropy-loss on one-hot labels
 // (source/nn/criterion.lisp:82-196, the lm-head of examples/gpt-2/model.lisp:137-196) holds the (rows, vocab)
-// logits, the softmax, the one-hot labels and their gradients.  Here the vocabulary is walked in pieces:
-// a piece's logits live in a workspace, every row keeps a running maximum and sum, and the gradient forms
-// a piece's logits anew.
+// logits, the softmax, the one-hot labels and their gradients.  Here
+//   forward   a tile of logits never leaves the registers: it leaves one maximum and one sum of exponentials per
+//             row behind, which a second kernel folds over the tiles of the vocabulary;
+//   backward  the vocabulary is walked in pieces: a piece's logits are formed anew and leave as ds, from which the
+//             piece's rows of dw and its share of dx are formed.
+// All products run on the 16-bit matrix cores on pairs of binary16 numbers (wf2_pairs.h): they are what bounds the
+// operator beyond a few hundred rows.
 #include <utility>
 
+#include "wf2_pairs.h"
 #include "wf2_rows.h"
 
 namespace wf2 {
 
 constexpr float kLog2eF = 1.44269504088896340736f;
-constexpr float kLn2F = 0.693147180559945309417f;
 
-// A row's running state over the pieces: maximum, sum of exp(s - maximum), the label's logit.
-struct XentRow {
-  float top, sum, at;
+// What the kernels of one backward call hand each other.
+struct XentHead {
+  int ex, ew;      // x and w are held times 2^ex, 2^ew
+  int eg;          // the rows' gradients are held over 2^eg
+  float weight;    // 1 / number of rows with a label (mean), 1 otherwise
+  float alpha;     // what the rows' gradients have in common
 };
 
-// One workgroup per row of a piece: fold the piece's maximum and sum into the row's state.
-__global__ __launch_bounds__(kBlock) void xent_fold_piece(const float* __restrict__ s, long cols, long first,
-                                                          const int32_t* __restrict__ labels,
-                                                          XentRow* __restrict__ state) {
+constexpr int kLargestW = 1024, kLargestX = 256;   // workgroups (and partial maxima) of xent_largest
+
+__device__ __forceinline__ float block_max(float v, float* lds) {
+  v = wave_max(v);
+  if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  v = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+  __syncthreads();
+  return v;
+}
+
+__device__ __forceinline__ float finite_size(float v) {
+  v = __builtin_fabsf(v);
+  return v < INFINITY ? v : 0.0f;   // NaN and infinities set no scale
+}
+
+// ---- operands as pairs --------------------------------------------------------------------------------------
+
+// Largest finite |w|, |x| over the rows with a label (partial maxima), the number of such rows, the largest |g|.
+__global__ __launch_bounds__(kBlock) void xent_largest(long rows, long dim, long vocab, const float* __restrict__ x,
+                                                       const float* __restrict__ w, const int32_t* __restrict__ labels,
+                                                       const float* __restrict__ dloss, bool per_row, bool mean,
+                                                       float* __restrict__ largest, XentHead* __restrict__ head) {
   __shared__ float part[kWavesPerBlock];
-  const int64_t row = blockIdx.x;
-  const float* r = s + row * cols;
-  float top = -INFINITY;
-  bool bad = false;
-  for (long c = threadIdx.x; c < cols; c += kBlock) {
-    top = fmaxf(top, r[c]);
-    bad |= r[c] != r[c];
-  }
-  if (bad) top = NAN;
-  // a maximum that lets a NaN through, as the sums below do
-  const int w = threadIdx.x / kWave;
+  __shared__ double dpart[kWavesPerBlock];
+  const uint32_t b = blockIdx.x;
+  float m = 0.0f;
+  if (b < kLargestW) {
+    const int64_t n = (int64_t)vocab * dim, stride = (int64_t)kLargestW * kBlock;
+    int64_t i = (int64_t)b * kBlock + threadIdx.x;
+    if ((uintptr_t)w % 16 == 0) {
+      const f4* w4 = reinterpret_cast<const f4*>(w);
+      const int64_t n4 = n / 4;
+      int64_t j = i;
+      for (; j + 3 * stride < n4; j += 4 * stride) {
+        const f4 a = w4[j], c = w4[j + stride], d = w4[j + 2 * stride], e = w4[j + 3 * stride];
 #pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1) {
-    const float other = __shfl_xor(top, o);
-    top = (top != top || other != other) ? NAN : fmaxf(top, other);
-  }
-  if ((threadIdx.x & (kWave - 1)) == 0) part[w] = top;
-  __syncthreads();
-  const XentRow old = state[row];
-  top = first ? old.top : -INFINITY;
+        for (int k = 0; k < 4; k++)
+          m = fmaxf(m, fmaxf(fmaxf(finite_size(a[k]), finite_size(c[k])), fmaxf(finite_size(d[k]), finite_size(e[k]))));
+      }
+      for (; j < n4; j += stride) {
+        const f4 a = w4[j];
 #pragma unroll
-  for (int i = 0; i < kWavesPerBlock; i++) top = (top != top || part[i] != part[i]) ? NAN : fmaxf(top, part[i]);
-  __syncthreads();
-  const float base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
-  for (long c = threadIdx.x; c < cols; c += kBlock) sum += __builtin_amdgcn_exp2f((r[c] - base) * kLog2eF);
-  sum = wave_sum32(sum);
-  if ((threadIdx.x & (kWave - 1)) == 0) part[w] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float total = first ? old.sum * __builtin_amdgcn_exp2f((old.top - base) * kLog2eF) : 0.0f;
-    for (int i = 0; i < kWavesPerBlock; i++) total += part[i];
-    const long label = labels[row];
-    float at = first ? old.at : NAN;   // a label behind the vocabulary finds no logit: its loss is NaN
-    if (label >= first && label < first + cols) at = r[label - first];
-    state[row] = XentRow{top, total, at};
+        for (int k = 0; k < 4; k++) m = fmaxf(m, finite_size(a[k]));
+      }
+      i += n4 * 4;
+    }
+    for (; i < n; i += stride) m = fmaxf(m, finite_size(w[i]));
+    m = block_max(m, part);
+    if (threadIdx.x == 0) largest[b] = m;
+  } else if (b < kLargestW + kLargestX) {
+    for (int64_t r = b - kLargestW; r < rows; r += kLargestX) {
+      if (labels[r] < 0) continue;
+      for (long c = threadIdx.x; c < dim; c += kBlock) m = fmaxf(m, finite_size(x[r * dim + c]));
+    }
+    m = block_max(m, part);
+    if (threadIdx.x == 0) largest[b] = m;
+  } else {
+    double count = 0.0;
+    for (long r = threadIdx.x; r < rows; r += kBlock) {
+      if (labels[r] < 0) continue;
+      count += 1.0;
+      if (per_row && dloss) m = fmaxf(m, finite_size(dloss[r]));
+    }
+    m = block_max(m, part);
+    count = block_sum(count, dpart);
+    if (threadIdx.x == 0) {
+      head->eg = m > 0.0f ? __builtin_amdgcn_frexp_expf(m) : 0;
+      head->weight = mean ? (count > 0.0 ? (float)(1.0 / count) : 0.0f) : 1.0f;
+    }
   }
 }
 
-// loss and row statistic from the rows' states
-__global__ __launch_bounds__(kBlock) void xent_rows(long rows, const XentRow* __restrict__ state,
-                                                    const int32_t* __restrict__ labels, float* __restrict__ loss,
-                                                    float* __restrict__ lse) {
-  const long row = (long)blockIdx.x * kBlock + threadIdx.x;
-  if (row >= rows) return;
-  const XentRow r = state[row];
-  const float l = r.top + logf(r.sum);
-  lse[row] = l;
-  loss[row] = labels[row] < 0 ? 0.0f : l - r.at;
+// A block of 32 rows of x or w to pairs.  PER_ROW: every row under a power of two of its own (`exponent`, the rows of x
+// behind those of w), so that no row depends on another; otherwise one power of two for the whole matrix, from the
+// partial maxima of xent_largest, and rows of x without a label become zero; the first workgroup then also
+// finishes `head`, and the workgroups of x write the rows' gradients `g` (0 without a label, NaN for a label
+// behind the vocabulary).
+struct XentSplit {
+  const float *x, *w;
+  const int32_t* labels;
+  long rows, dim, vocab;
+  char *px, *pw;        // pair layout
+  int col_blocks;       // of 16
+  uint32_t wblocks;     // workgroups of w; those of x follow
+  int* exponent;        // PER_ROW: wblocks * 32 of w, then those of x
+  const float* largest;
+  const float* dloss;
+  bool per_row_gradient;
+  float scale;
+  float* g;
+  XentHead* head;
+};
+
+template <bool PER_ROW, bool VEC>
+__global__ __launch_bounds__(kBlock) void xent_split(XentSplit p) {
+  __shared__ float part[kWavesPerBlock];
+  const bool of_x = blockIdx.x >= p.wblocks;
+  const int64_t block = of_x ? blockIdx.x - p.wblocks : blockIdx.x;
+  const float* src = of_x ? p.x : p.w;
+  const int64_t nrows = of_x ? p.rows : p.vocab;
+  const int rr = threadIdx.x >> 3, c8 = (threadIdx.x & 7);   // eight threads to a row
+  const int64_t row = block * 32 + rr;
+  const float* r = src + row * p.dim;
+  const bool inside = row < nrows;
+  bool live = inside;
+  int e;
+  if (PER_ROW) {
+    float m = 0.0f;
+    if (inside) {
+      if (VEC) {
+        for (long c = c8 * 4; c < p.dim; c += 32) {
+          const f4 a = *reinterpret_cast<const f4*>(r + c);
+#pragma unroll
+          for (int k = 0; k < 4; k++) m = fmaxf(m, finite_size(a[k]));
+        }
+      } else {
+        for (long c = c8; c < p.dim; c += 8) m = fmaxf(m, finite_size(r[c]));
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    e = pair_exponent(m);
+    if (c8 == 0) p.exponent[((int64_t)(of_x ? p.wblocks : 0) + block) * 32 + rr] = e;
+  } else {
+    float m = 0.0f;
+    const float* q = p.largest + (of_x ? kLargestW : 0);
+    for (int i = threadIdx.x; i < (of_x ? kLargestX : kLargestW); i += kBlock) m = fmaxf(m, q[i]);
+    e = pair_exponent(block_max(m, part));
+    if (blockIdx.x == 0) {
+      m = block_max(p.largest[kLargestW + threadIdx.x], part);   // kLargestX == kBlock
+      if (threadIdx.x == 0) {
+        p.head->ew = e;
+        p.head->ex = pair_exponent(m);
+        p.head->alpha = p.scale * p.head->weight * (p.dloss && !p.per_row_gradient ? p.dloss[0] : 1.0f);
+      }
+    }
+    if (of_x && inside) {
+      const int32_t label = p.labels[row];
+      live = label >= 0;
+      if (c8 == 0)
+        p.g[row] = label < 0 ? 0.0f
+                   : label >= p.vocab ? NAN
+                   : p.dloss && p.per_row_gradient ? __builtin_ldexpf(p.dloss[row], -p.head->eg) : 1.0f;
+    }
+  }
+  char* out = (of_x ? p.px : p.pw) + block * p.col_blocks * (int64_t)kPiece + rr * 16;
+  const float up = __builtin_ldexpf(1.0f, e);
+  for (int c = c8; c < p.col_blocks * 2; c += 8) {   // eight columns each
+    float a[8];
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+      const long col = (long)c * 8 + k;
+      if (VEC) {
+        const f4 t = live && col < p.dim ? *reinterpret_cast<const f4*>(r + col) : f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 4; i++) a[k + i] = t[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) a[k + i] = live && col + i < p.dim ? r[col + i] : 0.0f;
+      }
+    }
+    h8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      _Float16 h, l;
+      split_pair(a[k] * up, &h, &l);
+      hi[k] = h;
+      lo[k] = l;
+    }
+    char* q = out + (int64_t)(c >> 1) * kPiece + (c & 1) * 512;
+    *reinterpret_cast<h8*>(q) = hi;
+    *reinterpret_cast<h8*>(q + kPiece / 2) = lo;
+  }
+}
+
+// ---- forward --------------------------------------------------------------------------------------------------
+
+struct XentLoss {
+  PairMatrix w, x;
+  const int* exponent;     // of w's rows, then (wblocks * 32 behind) of x's
+  int64_t x_exponents;
+  const int32_t* labels;
+  long rows, vocab;
+  uint32_t tiles_m, tiles_n;
+  float2* part;            // [tile of the vocabulary][row]: maximum, sum of exp(s - maximum)
+  float* at;               // [row] the label's logit
+};
+
+// A tile of 128 words x 256 rows of x: a lane of the accumulators holds 32 words of one row of x, so that maxima and sums
+// run along registers.
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_loss(XentLoss p) {
+  __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
+  uint32_t tm, tn;
+  pair_tile(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
+  f16v acc[2][4];
+  pair_product<false, false, false>(p.w, p.x, m0, n0, 0, p.w.col_blocks, smem, acc);
+  __syncthreads();   // the stages are free
+  float2* fold = reinterpret_cast<float2*>(smem);            // [wave / 2][256 rows]
+  int* ew = reinterpret_cast<int*>(smem + 2 * kTileN * sizeof(float2));
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
+  if (threadIdx.x < kTileM) {
+    const int64_t v = m0 + threadIdx.x;
+    ew[threadIdx.x] = v < p.vocab ? p.exponent[v] : 0;
+  }
+  __syncthreads();
+  const int wm = (wave >> 1) * 64;
+  const bool ragged = m0 + kTileM > p.vocab;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int64_t n = n0 + (wave & 1) * 128 + j * 32 + (lane & 31);
+    const bool inside = n < p.rows;
+    const int ex = inside ? p.exponent[p.x_exponents + n] : 0;
+    const int64_t label = inside ? p.labels[n] : -1;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const int v = wm + i * 32 + q * 8 + h * 4;
+        const int4 e = *reinterpret_cast<const int4*>(ew + v);
+        const int ee[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          float s = __builtin_ldexpf(acc[i][j][q * 4 + r], -(ex + ee[r]));
+          if (ragged && m0 + v + r >= p.vocab) s = -INFINITY;
+          acc[i][j][q * 4 + r] = s;
+          top = fmaxf(top, s);
+        }
+      }
+    const int64_t local = label - m0 - wm;
+    if (local >= 0 && local < 64 && label < p.vocab && ((local >> 2) & 1) == h) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if (local == i * 32 + (r >> 2) * 8 + h * 4 + (r & 3)) p.at[n] = acc[i][j][r];
+    }
+    const float base = (top == -INFINITY ? 0.0f : top) * kLog2eF;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2eF, -base));
+    const float top2 = __shfl_xor(top, 32), sum2 = __shfl_xor(sum, 32);
+    const float both = fmaxf(top, top2);
+    const float safe = both == -INFINITY ? 0.0f : both;
+    sum = sum * __builtin_amdgcn_exp2f((top - safe) * kLog2eF) + sum2 * __builtin_amdgcn_exp2f((top2 - safe) * kLog2eF);
+    if (h == 0) fold[(wave >> 1) * kTileN + (wave & 1) * 128 + j * 32 + lane] = float2{both, sum};
+  }
+  __syncthreads();
+  const int64_t n = n0 + threadIdx.x;
+  if (n < p.rows) {
+    const float2 a = fold[threadIdx.x], b = fold[kTileN + threadIdx.x];
+    const float both = fmaxf(a.x, b.x);
+    const float safe = both == -INFINITY ? 0.0f : both;
+    const float sum = a.y * __builtin_amdgcn_exp2f((a.x - safe) * kLog2eF) + b.y * __builtin_amdgcn_exp2f((b.x - safe) * kLog2eF);
+    p.part[(int64_t)tm * p.rows + n] = float2{both, sum};
+  }
+}
+
+// The tiles' maxima and sums of 64 rows of x: sixteen wavefronts take every sixteenth tile each and meet in LDS.
+constexpr int kFoldBlock = 1024;
+__global__ __launch_bounds__(kFoldBlock) void xent_fold(long rows, long vocab, uint32_t tiles, const float2* __restrict__ part,
+                                                        const float* __restrict__ at, const int32_t* __restrict__ labels,
+                                                        float* __restrict__ loss, float* __restrict__ lse) {
+  __shared__ float2 meet[kFoldBlock];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int64_t n = (int64_t)blockIdx.x * kWave + lane;
+  float top = -INFINITY, sum = 0.0f;
+  if (n < rows) {
+    for (uint32_t t = wave; t < tiles; t += kFoldBlock / kWave) {
+      const float2 a = part[(int64_t)t * rows + n];
+      const float both = fmaxf(top, a.x);
+      const float safe = both == -INFINITY ? 0.0f : both;
+      sum = sum * __builtin_amdgcn_exp2f((top - safe) * kLog2eF) + a.y * __builtin_amdgcn_exp2f((a.x - safe) * kLog2eF);
+      top = both;
+    }
+  }
+  meet[threadIdx.x] = float2{top, sum};
+  __syncthreads();
+  if (wave != 0 || n >= rows) return;
+  for (int i = 1; i < kFoldBlock / kWave; i++) {
+    const float2 a = meet[i * kWave + lane];
+    const float both = fmaxf(top, a.x);
+    const float safe = both == -INFINITY ? 0.0f : both;
+    sum = sum * __builtin_amdgcn_exp2f((top - safe) * kLog2eF) + a.y * __builtin_amdgcn_exp2f((a.x - safe) * kLog2eF);
+    top = both;
+  }
+  const float l = top + logf(sum);
+  const int32_t label = labels[n];
+  lse[n] = l;
+  loss[n] = label < 0 ? 0.0f : label >= vocab ? NAN : l - at[n];   // a label behind the vocabulary has no logit
 }
 
 // out[0] = sum of the losses (over the number of rows with a label)
@@ -95,41 +343,134 @@ __global__ __launch_bounds__(kBlock) void xent_reduce(long rows, const float* __
   if (threadIdx.x == 0) out[0] = (float)(mean ? sum / count : sum);
 }
 
-// 1 / the number of rows with a label
-__global__ __launch_bounds__(kBlock) void xent_weight(long rows, const int32_t* __restrict__ labels, float* __restrict__ out) {
-  __shared__ double part[kWavesPerBlock];
-  double count = 0.0;
-  for (long i = threadIdx.x; i < rows; i += kBlock) count += labels[i] >= 0;
-  count = block_sum(count, part);
-  if (threadIdx.x == 0) out[0] = (float)(1.0 / count);
-}
+// ---- backward -------------------------------------------------------------------------------------------------
 
-// s <- g (exp(s - lse) - [label]); rows without a label are zero whatever they hold
-__global__ __launch_bounds__(kBlock) void xent_gradient(float* __restrict__ s, long cols, long first,
-                                                        const int32_t* __restrict__ labels, const float* __restrict__ lse,
-                                                        const float* __restrict__ weight, const float* __restrict__ dloss,
-                                                        bool per_row, float scale, long vocab) {
-  const int64_t row = blockIdx.x;
-  float* r = s + row * cols;
-  const long label = labels[row];
-  float g = scale;
-  if (weight) g *= weight[0];
-  if (dloss) g *= dloss[per_row ? row : 0];
-  if (label >= vocab) g = NAN;
-  const float l = lse[row];
-  for (long c = threadIdx.x; c < cols; c += kBlock) {
-    const float p = __builtin_amdgcn_exp2f((r[c] - l) * kLog2eF) - (c + first == label ? 1.0f : 0.0f);
-    r[c] = label < 0 ? 0.0f : g * p;
+struct XentGradient {
+  PairMatrix w, x, ds;     // w: the piece's rows; ds: rows of x by the piece's words, lo parts 2^11 times too large
+  const XentHead* head;
+  const int32_t* labels;
+  const float *lse, *g;
+  long rows, dim;
+  long first, words;       // the piece
+  uint32_t tiles_m, tiles_n;
+  int split, steps;        // dx: K steps per share of the piece, in all
+  float* out;              // dw (the piece's rows) or dx's planes
+};
+
+constexpr float kLoud = 32768.0f;   // ds is held times 2^15: at most 1 before
+
+// ds of a tile of 128 words x 256 rows of x; also of the tiles' rows and words behind the matrix, as zeros.
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_ds(XentGradient p) {
+  __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
+  uint32_t tm, tn;
+  pair_tile(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
+  f16v acc[2][4];
+  pair_product<false, false, false>(p.w, p.x, m0, n0, 0, p.w.col_blocks, smem, acc);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
+  const int wm = (wave >> 1) * 64;
+  const int down = -(p.head->ex + p.head->ew);
+  const bool ragged = m0 + kTileM > p.words;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int64_t n = n0 + (wave & 1) * 128 + j * 32 + (lane & 31);
+    const bool inside = n < p.rows;
+    const float g = inside ? p.g[n] * kLoud : 0.0f;
+    const float base = inside ? p.lse[n] * kLog2eF : 0.0f;
+    const int64_t local = (inside ? (int64_t)p.labels[n] : -1) - p.first - m0 - wm;
+    char* out = const_cast<char*>(p.ds.base) + (n >> 5) * p.ds.pitch() + ((m0 + wm) >> 4) * (int64_t)kPiece +
+                (n & 31) * 16 + h * 8;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        h4 hi, lo;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int v = i * 32 + q * 8 + h * 4 + r;
+          const float s = __builtin_ldexpf(acc[i][j][q * 4 + r], down);
+          float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s, kLog2eF, -base));
+          if (local == v) d -= 1.0f;
+          d = g == 0.0f || (ragged && m0 + wm + v >= p.words) ? 0.0f : d * g;
+          const _Float16 a = (_Float16)d;
+          hi[r] = a;
+          lo[r] = (_Float16)((d - (float)a) * 2048.0f);
+        }
+        char* o = out + (i * 2 + (q >> 1)) * kPiece + (q & 1) * 512;
+        *reinterpret_cast<h4*>(o) = hi;
+        *reinterpret_cast<h4*>(o + kPiece / 2) = lo;
+      }
   }
 }
 
-// rows of x without a label contribute nothing to dw, also where they hold no numbers
-__global__ __launch_bounds__(kBlock) void xent_clean_rows(const float* __restrict__ x, const int32_t* __restrict__ labels,
-                                                          long dim, float* __restrict__ out) {
-  const int64_t row = blockIdx.x;
-  const bool held = labels[row] >= 0;
-  for (long c = threadIdx.x; c < dim; c += kBlock) out[row * dim + c] = held ? x[row * dim + c] : 0.0f;
+// A share of K of dx: plane `share` of p.out, (rows, dim), unscaled.
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_dx(XentGradient p) {
+  __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
+  const uint32_t tiles = p.tiles_m * p.tiles_n, share = blockIdx.x / tiles;
+  uint32_t tm, tn;
+  pair_tile(blockIdx.x - share * tiles, p.tiles_m, p.tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
+  const int64_t s0 = (int64_t)share * p.split;
+  const int steps = p.steps - s0 < p.split ? (int)(p.steps - s0) : p.split;
+  f16v acc[2][4];
+  pair_product<false, true, true>(p.ds, p.w, m0, n0, s0 * 16, steps, smem, acc);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
+  float* out = p.out + (int64_t)share * p.rows * p.dim;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int64_t d = n0 + (wave & 1) * 128 + j * 32 + (lane & 31);
+    if (d < p.dim) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int64_t n = m0 + (wave >> 1) * 64 + i * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
+          if (n < p.rows) out[n * p.dim + d] = acc[i][j][r];
+        }
+    }
+  }
 }
+
+// dx <- the planes' sum, scaled; rows without a label are zero whatever the common factor is
+__global__ __launch_bounds__(kBlock) void xent_fold_dx(long rows, long dim, int planes, const float* __restrict__ part,
+                                                       const float* __restrict__ g, const XentHead* __restrict__ head,
+                                                       float* __restrict__ dx) {
+  const int64_t n = (int64_t)rows * dim, i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (i >= n) return;
+  float sum = part[i];
+  for (int s = 1; s < planes; s++) sum += part[s * n + i];
+  const float v = __builtin_ldexpf(sum, head->eg - 15 - head->ew) * head->alpha;
+  dx[i] = g[i / dim] == 0.0f ? 0.0f : v;
+}
+
+// The piece's rows of dw.
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_dw(XentGradient p) {
+  __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
+  uint32_t tm, tn;
+  pair_tile(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
+  f16v acc[2][4];
+  pair_product<true, true, true>(p.ds, p.x, m0, n0, 0, p.steps, smem, acc);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
+  const int down = p.head->eg - 15 - p.head->ex;
+  const float alpha = p.head->alpha;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int64_t d = n0 + (wave & 1) * 128 + j * 32 + (lane & 31);
+    if (d < p.dim) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int64_t v = m0 + (wave >> 1) * 64 + i * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
+          const float a = __builtin_ldexpf(acc[i][j][r], down);
+          if (v < p.words) p.out[v * p.dim + d] = a == 0.0f ? 0.0f : a * alpha;
+        }
+    }
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------
 
 static bool meets(const void* a, int64_t na, const void* b, int64_t nb) {
   const char *p = (const char*)a, *q = (const char*)b;
@@ -142,17 +483,51 @@ static int xent_check(const char* name, long rows, long dim, long vocab, const v
   if (reduction < WF2HIP_REDUCE_NONE || reduction > WF2HIP_REDUCE_MEAN)
     return fail(WF2HIP_EINVAL, "%s: unknown reduction %d", name, reduction);
   if (dim < 1 || vocab < 1) return fail(WF2HIP_EINVAL, "%s: needs a vocabulary and hidden states of at least one element", name);
-  if (rows > INT32_MAX || dim > INT32_MAX || vocab > INT32_MAX)
-    return fail(WF2HIP_EUNSUPPORTED, "%s: an extent beyond 2^31 - 1", name);
+  if (rows > (1L << 28) || dim > (1L << 20) || vocab > (1L << 28))
+    return fail(WF2HIP_EUNSUPPORTED, "%s: more than 2^28 rows or words, or 2^20 elements of a hidden state", name);
   if (!w || (rows && (!x || !labels || !lse))) return fail(WF2HIP_EINVAL, "%s: null pointer", name);
   return 0;
 }
 
-// columns of the vocabulary that a workspace of at most 256 MiB of logits takes
-static long xent_piece(long rows, long vocab) {
-  const int64_t fit = ((int64_t)64 << 20) / (rows > 0 ? rows : 1);
-  const int64_t cols = fit < 256 ? 256 : fit / 256 * 256;
-  return (long)(cols < vocab ? cols : vocab);
+// Blocks of the pool that are given back when the call returns (its kernels are enqueued by then).
+struct Blocks {
+  void* held[8];
+  int count = 0;
+  int rc = 0;
+  ~Blocks() {
+    for (int i = 0; i < count; i++) (void)wf2hip_free(held[i]);
+  }
+  template <typename T>
+  T* take(int64_t bytes) {
+    void* p = nullptr;
+    if (rc == 0) rc = wf2hip_malloc_uninitialized(&p, (size_t)(bytes > 0 ? bytes : 1));
+    if (p) held[count++] = p;
+    return (T*)p;
+  }
+};
+
+static PairMatrix pair_matrix(const char* base, int64_t rows, int64_t cols) {
+  return PairMatrix{base, (int)ceil_div(rows, 32), (int)ceil_div(cols, 16)};
+}
+static int64_t pair_bytes(const PairMatrix& m) { return m.row_blocks * m.pitch(); }
+
+// Words of a piece of the backward: ds (4 bytes per row of x and word) takes at most 1 GiB, in pieces of equal size.
+static int64_t xent_words(int64_t rows, int64_t vocab) {
+  const int64_t padded = ceil_div(rows, kTileN) * kTileN;
+  int64_t fit = ((int64_t)1 << 28) / padded / kTileM;
+  if (fit < 1) fit = 1;
+  const int64_t tiles = ceil_div(vocab, kTileM), pieces = ceil_div(tiles, fit);
+  return ceil_div(tiles, pieces) * kTileM;
+}
+
+template <bool PER_ROW>
+static int split_operands(const XentSplit& p, hipStream_t st) {
+  const uint32_t blocks = p.wblocks + (uint32_t)ceil_div(p.rows, 32);
+  if (p.dim % 4 == 0 && ((uintptr_t)p.x | (uintptr_t)p.w) % 16 == 0)
+    xent_split<PER_ROW, true><<<blocks, kBlock, 0, st>>>(p);
+  else
+    xent_split<PER_ROW, false><<<blocks, kBlock, 0, st>>>(p);
+  return after_launch("xent_split");
 }
 
 }  // namespace wf2
@@ -164,42 +539,53 @@ WF2_API int wf2hip_linear_cross_entropy_f32(long rows, long dim, long vocab, con
   const char* name = "linear cross entropy";
   WF2_TRY(require_init());
   WF2_TRY(xent_check(name, rows, dim, vocab, x, w, labels, lse, reduction));
-  const int64_t losses = reduction == WF2HIP_REDUCE_NONE ? rows : 1;
+  const bool each = reduction == WF2HIP_REDUCE_NONE;
+  const int64_t losses = each ? rows : 1;
   if (losses && !loss) return fail(WF2HIP_EINVAL, "%s: null pointer", name);
   for (auto [out, n] : {std::pair<const float*, int64_t>(loss, losses), std::pair<const float*, int64_t>(lse, rows)})
     if (meets(out, n, x, (int64_t)rows * dim) || meets(out, n, w, (int64_t)vocab * dim) || meets(out, n, labels, rows))
       return fail(WF2HIP_EOVERLAP, "%s: an output overlaps an input", name);
   if (meets(loss, losses, lse, rows)) return fail(WF2HIP_EOVERLAP, "%s: the loss overlaps the row statistics", name);
   hipStream_t st = rt().stream;
-  const long piece = xent_piece(rows, vocab);
-  void *s = nullptr, *state = nullptr, *each = nullptr;
-  int rc = 0;
+  Blocks blocks;
+  float* per_row = loss;
   if (rows) {
-    if ((rc = wf2hip_malloc_uninitialized(&s, (size_t)rows * piece * 4)) == 0 &&
-        (rc = wf2hip_malloc_uninitialized(&state, (size_t)rows * sizeof(XentRow))) == 0 &&
-        reduction != WF2HIP_REDUCE_NONE)
-      rc = wf2hip_malloc_uninitialized(&each, (size_t)rows * 4);
-    for (long c = 0; rc == 0 && c < vocab; c += piece) {
-      const long cols = piece < vocab - c ? piece : vocab - c;
-      rc = wf2hip_sgemm('T', 'N', cols, rows, dim, 1.0f, w + (int64_t)c * dim, dim, x, dim, 0.0f, (float*)s, cols);
-      if (rc == 0) {
-        xent_fold_piece<<<(uint32_t)rows, kBlock, 0, st>>>((const float*)s, cols, c, labels, (XentRow*)state);
-        rc = after_launch("xent_fold_piece");
-      }
-    }
-    if (rc == 0) {
-      xent_rows<<<(uint32_t)ceil_div(rows, kBlock), kBlock, 0, st>>>(rows, (const XentRow*)state, labels,
-                                                                    each ? (float*)each : loss, lse);
-      rc = after_launch("xent_rows");
-    }
+    XentLoss p{};
+    p.w = pair_matrix(nullptr, vocab, dim);
+    p.x = pair_matrix(nullptr, rows, dim);
+    p.tiles_m = (uint32_t)ceil_div(vocab, kTileM);
+    p.tiles_n = (uint32_t)ceil_div(rows, kTileN);
+    if ((int64_t)p.tiles_m * p.tiles_n >= ((int64_t)1 << 31)) return fail(WF2HIP_EUNSUPPORTED, "%s: too many tiles for one launch", name);
+    p.w.base = blocks.take<char>(pair_bytes(p.w));
+    p.x.base = blocks.take<char>(pair_bytes(p.x));
+    int* exponent = blocks.take<int>((p.w.row_blocks + p.x.row_blocks) * (int64_t)32 * 4);
+    p.part = blocks.take<float2>((int64_t)p.tiles_m * rows * 8);
+    p.at = blocks.take<float>(rows * (int64_t)4);
+    if (!each) per_row = blocks.take<float>(rows * (int64_t)4);
+    WF2_TRY(blocks.rc);
+    XentSplit s{};
+    s.x = x; s.w = w; s.labels = labels;
+    s.rows = rows; s.dim = dim; s.vocab = vocab;
+    s.px = const_cast<char*>(p.x.base); s.pw = const_cast<char*>(p.w.base);
+    s.col_blocks = p.w.col_blocks;
+    s.wblocks = (uint32_t)p.w.row_blocks;
+    s.exponent = exponent;
+    WF2_TRY(split_operands<true>(s, st));
+    p.exponent = exponent;
+    p.x_exponents = (int64_t)p.w.row_blocks * 32;
+    p.labels = labels;
+    p.rows = rows;
+    p.vocab = vocab;
+    xent_tile_loss<<<p.tiles_m * p.tiles_n, kBlock, 0, st>>>(p);
+    WF2_TRY(after_launch("xent_tile_loss"));
+    xent_fold<<<(uint32_t)ceil_div(rows, kWave), kFoldBlock, 0, st>>>(rows, vocab, p.tiles_m, p.part, p.at, labels, per_row, lse);
+    WF2_TRY(after_launch("xent_fold"));
   }
-  if (rc == 0 && reduction != WF2HIP_REDUCE_NONE) {
-    xent_reduce<<<1, kBlock, 0, st>>>(rows, (const float*)each, labels, reduction == WF2HIP_REDUCE_MEAN, loss);
-    rc = after_launch("xent_reduce");
+  if (!each) {
+    xent_reduce<<<1, kBlock, 0, st>>>(rows, per_row, labels, reduction == WF2HIP_REDUCE_MEAN, loss);
+    WF2_TRY(after_launch("xent_reduce"));
   }
-  for (void* block : {s, state, each})
-    if (block) (void)wf2hip_free(block);
-  return rc;
+  return 0;
 }
 
 WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long vocab, const float* x, const float* w,
@@ -209,7 +595,8 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
   WF2_TRY(require_init());
   WF2_TRY(xent_check(name, rows, dim, vocab, x, w, labels, lse, reduction));
   if (!dw || (rows && !dx)) return fail(WF2HIP_EINVAL, "%s: null pointer", name);
-  const int64_t nx = (int64_t)rows * dim, nw = (int64_t)vocab * dim, ng = reduction == WF2HIP_REDUCE_NONE ? rows : 1;
+  const bool each = reduction == WF2HIP_REDUCE_NONE;
+  const int64_t nx = (int64_t)rows * dim, nw = (int64_t)vocab * dim, ng = each ? rows : 1;
   for (auto [out, n] : {std::pair<const float*, int64_t>(dx, nx), std::pair<const float*, int64_t>(dw, nw)})
     if (meets(out, n, x, nx) || meets(out, n, w, nw) || meets(out, n, labels, rows) || meets(out, n, lse, rows) ||
         meets(out, n, dloss, ng))
@@ -217,37 +604,91 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
   if (meets(dx, nx, dw, nw)) return fail(WF2HIP_EOVERLAP, "%s: the gradients overlap", name);
   if (rows == 0) return wf2hip_fill_f32(dw, (size_t)nw, 0.0f);
   hipStream_t st = rt().stream;
-  const long piece = xent_piece(rows, vocab);
-  void *s = nullptr, *clean = nullptr, *weight = nullptr;
-  int rc = wf2hip_malloc_uninitialized(&s, (size_t)rows * piece * 4);
-  if (rc == 0) rc = wf2hip_malloc_uninitialized(&clean, (size_t)nx * 4);
-  if (rc == 0 && reduction == WF2HIP_REDUCE_MEAN) {
-    rc = wf2hip_malloc_uninitialized(&weight, 4);
-    if (rc == 0) {
-      xent_weight<<<1, kBlock, 0, st>>>(rows, labels, (float*)weight);
-      rc = after_launch("xent_weight");
-    }
+  const int64_t words = xent_words(rows, vocab);
+  const int64_t padded = ceil_div(rows, kTileN) * kTileN;
+  const int64_t tiles_d = ceil_div(dim, kTileN);
+  // dx has few tiles and a long K: shares of K that fill the device twice, of at least 16 K steps, in even numbers (a
+  // share starts at a whole row block of w)
+  const int64_t dx_tiles = ceil_div(rows, kTileM) * tiles_d, all_steps = ceil_div(words < vocab ? words : vocab, 16);
+  int64_t shares = ceil_div(4 * rt().num_cus, dx_tiles);
+  if (shares > all_steps / 16) shares = all_steps / 16;
+  if (shares < 1) shares = 1;
+  const int64_t split = ceil_div(ceil_div(all_steps, shares), 2) * 2;
+  int64_t planes = 0;
+  for (int64_t c = 0; c < vocab; c += words) planes += ceil_div(ceil_div(words < vocab - c ? words : vocab - c, 16), split);
+  const int64_t most = ((int64_t)1 << 31) - 1;
+  if (words / kTileM * (padded / kTileN) > most || dx_tiles * shares > most || words / kTileM * tiles_d > most ||
+      ceil_div(nx, kBlock) > most)
+    return fail(WF2HIP_EUNSUPPORTED, "%s: too many tiles for one launch", name);
+
+  Blocks blocks;
+  PairMatrix pw = pair_matrix(nullptr, vocab, dim), px = pair_matrix(nullptr, rows, dim);
+  PairMatrix ds = pair_matrix(nullptr, padded, words);
+  pw.base = blocks.take<char>(pair_bytes(pw));
+  px.base = blocks.take<char>(pair_bytes(px));
+  ds.base = blocks.take<char>(pair_bytes(ds));
+  float* part = blocks.take<float>(planes * nx * 4);
+  float* g = blocks.take<float>(rows * (int64_t)4);
+  float* largest = blocks.take<float>((kLargestW + kLargestX) * 4);
+  XentHead* head = blocks.take<XentHead>(sizeof(XentHead));
+  WF2_TRY(blocks.rc);
+
+  xent_largest<<<kLargestW + kLargestX + 1, kBlock, 0, st>>>(rows, dim, vocab, x, w, labels, dloss, each,
+                                                            reduction == WF2HIP_REDUCE_MEAN, largest, head);
+  WF2_TRY(after_launch("xent_largest"));
+  XentSplit s{};
+  s.x = x; s.w = w; s.labels = labels;
+  s.rows = rows; s.dim = dim; s.vocab = vocab;
+  s.px = const_cast<char*>(px.base); s.pw = const_cast<char*>(pw.base);
+  s.col_blocks = pw.col_blocks;
+  s.wblocks = (uint32_t)pw.row_blocks;
+  s.largest = largest;
+  s.dloss = dloss;
+  s.per_row_gradient = each;
+  s.scale = scale;
+  s.g = g;
+  s.head = head;
+  WF2_TRY(split_operands<false>(s, st));
+
+  int64_t plane = 0;
+  for (int64_t c = 0; c < vocab; c += words) {
+    XentGradient p{};
+    p.words = (long)(words < vocab - c ? words : vocab - c);
+    p.first = (long)c;
+    p.w = pw;
+    p.w.base += c / 32 * pw.pitch();
+    p.w.row_blocks -= (int)(c / 32);
+    p.x = px;
+    p.ds = ds;
+    p.head = head;
+    p.labels = labels;
+    p.lse = lse;
+    p.g = g;
+    p.rows = rows;
+    p.dim = dim;
+    p.tiles_m = (uint32_t)ceil_div(p.words, kTileM);
+    p.tiles_n = (uint32_t)(padded / kTileN);
+    xent_tile_ds<<<p.tiles_m * p.tiles_n, kBlock, 0, st>>>(p);
+    WF2_TRY(after_launch("xent_tile_ds"));
+
+    XentGradient q = p;
+    q.tiles_m = (uint32_t)ceil_div(rows, kTileM);
+    q.tiles_n = (uint32_t)tiles_d;
+    q.steps = (int)ceil_div(p.words, 16);
+    q.split = (int)split;
+    const int64_t here = ceil_div(q.steps, split);
+    q.out = part + plane * nx;
+    xent_tile_dx<<<(uint32_t)(dx_tiles * here), kBlock, 0, st>>>(q);
+    WF2_TRY(after_launch("xent_tile_dx"));
+    plane += here;
+
+    q = p;
+    q.tiles_n = (uint32_t)tiles_d;
+    q.steps = (int)ceil_div(rows, 16);
+    q.out = dw + c * dim;
+    xent_tile_dw<<<(uint32_t)(q.tiles_m * tiles_d), kBlock, 0, st>>>(q);
+    WF2_TRY(after_launch("xent_tile_dw"));
   }
-  if (rc == 0) {
-    xent_clean_rows<<<(uint32_t)rows, kBlock, 0, st>>>(x, labels, dim, (float*)clean);
-    rc = after_launch("xent_clean_rows");
-  }
-  for (long c = 0; rc == 0 && c < vocab; c += piece) {
-    const long cols = piece < vocab - c ? piece : vocab - c;
-    const float* wc = w + (int64_t)c * dim;
-    rc = wf2hip_sgemm('T', 'N', cols, rows, dim, 1.0f, wc, dim, (const float*)clean, dim, 0.0f, (float*)s, cols);
-    if (rc == 0) {
-      xent_gradient<<<(uint32_t)rows, kBlock, 0, st>>>((float*)s, cols, c, labels, lse, (const float*)weight, dloss,
-                                                      reduction == WF2HIP_REDUCE_NONE, scale, vocab);
-      rc = after_launch("xent_gradient");
-    }
-    if (rc == 0)
-      rc = wf2hip_sgemm('N', 'N', dim, rows, cols, 1.0f, wc, dim, (const float*)s, cols, c ? 1.0f : 0.0f, dx, dim);
-    if (rc == 0)
-      rc = wf2hip_sgemm('N', 'T', dim, cols, rows, 1.0f, (const float*)clean, dim, (const float*)s, cols, 0.0f,
-                        dw + (int64_t)c * dim, dim);
-  }
-  for (void* block : {s, clean, weight})
-    if (block) (void)wf2hip_free(block);
-  return rc;
+  xent_fold_dx<<<(uint32_t)ceil_div(nx, kBlock), kBlock, 0, st>>>(rows, dim, (int)planes, part, g, head, dx);
+  return after_launch("xent_fold_dx");
 }

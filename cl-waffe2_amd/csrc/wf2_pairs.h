@@ -1,0 +1,216 @@
+// wf2_pairs.h -- binary32 matrix products on the 16-bit matrix cores.
+//
+// A binary32 number a, scaled by a power of two into the range of binary16, is kept as a pair of binary16
+// numbers: hi = a rounded to 11 significant bits, lo = (a - hi) rounded to 11 bits; a - hi is exact, so
+// |a - hi - lo| <= 2^-22 |a| (numbers more than 2^17 times smaller than the largest of their matrix, whose lo
+// is subnormal, are kept to 2^-39 of that largest one).  A product is then
+//   a b = ah bh + ah bl + al bh   (+ al bl, at most 2^-22 |a b|, left out),
+// three v_mfma_f32_32x32x16_f16 accumulating in binary32: errors of a few 2^-22 per term, the size of those
+// that binary32 additions make over a few dozen terms.  The binary32 matrix cores do 256 flop per cycle and
+// compute unit, the binary16 ones 4096: three passes of the latter are 5.3 times as fast.
+//
+// Storage ("pair layout").  Pieces of 32 rows x 16 columns: 1 KB of hi, 1 KB of lo; piece (rb, cb) at
+// (rb * col_blocks + cb) * 2 KB.  Within a part: [column / 8][row][column % 8].  That is the order in which the
+// lanes of a matrix instruction read an operand whose columns are the product's k (lane l: row l % 32, columns
+// 8 (l / 32) ... + 7), so a part moves from memory into LDS and from there into registers as one linear
+// kilobyte; and four neighbouring rows x 16 columns are the 16-lane groups of the transposing LDS read
+// (ds_read_b64_tr_b16), so the same storage serves products whose k runs along its rows.
+#pragma once
+
+#include "wf2_common.h"
+#include "wf2_dma.h"
+
+namespace wf2 {
+
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __fp16 fp4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+constexpr int kPiece = 2048;   // bytes of a 32 x 16 piece, both parts
+
+struct PairMatrix {
+  const char* base;
+  int row_blocks;   // of 32
+  int col_blocks;   // of 16
+  __host__ __device__ int64_t pitch() const { return (int64_t)col_blocks * kPiece; }
+};
+
+// One workgroup's 128 x 256 tile of C[m][n] = sum_k A(m, k) B(n, k): four wavefronts, each 64 x 128 as 2 x 4
+// blocks of 32 x 32; two workgroups to a compute unit, so that one's prologue and epilogue run under the
+// other's products.  K steps of 16 arrive by DMA in a ring of three stages of 24 KB, two steps ahead.
+// AT / BT: k runs along the rows of that operand's storage instead of its columns.
+// LOUD: the lo parts of A are stored 2^11 times too large (numbers of a wide range: dozens of octaves below the
+// largest still keep 22 bits); their partner is scaled down in registers, exactly unless it is 2^18 times below its
+// largest.
+constexpr int kTileM = 128, kTileN = 256;
+constexpr int kStageA = kTileM / 32 * kPiece, kStageB = kTileN / 32 * kPiece, kStage = kStageA + kStageB;
+constexpr int kRing = 3;
+
+template <bool T>
+struct PairStream {
+  // DMA instruction q moves 1 KB: [k along columns] one part of row block q / 2; [k along rows] the 16 rows of
+  // column block q, both parts.
+  const char* at;
+  int64_t skip;   // to the next pair of K steps (T)
+
+  __device__ __forceinline__ void start(const PairMatrix& p, int64_t first, int q, int64_t k0) {
+    if (T) {
+      int64_t cb = first / 16 + q;
+      cb = cb < p.col_blocks ? cb : p.col_blocks - 1;   // columns behind the matrix feed outputs nobody stores
+      at = p.base + (k0 / 32) * p.pitch() + cb * kPiece;
+      skip = p.pitch() - 256;
+    } else {
+      int64_t rb = first / 32 + q / 2;
+      rb = rb < p.row_blocks ? rb : p.row_blocks - 1;
+      at = p.base + rb * p.pitch() + (k0 / 16) * kPiece + (q & 1) * (kPiece / 2);
+    }
+  }
+  __device__ __forceinline__ void next(bool odd) { at += T ? (odd ? skip : 256) : (int64_t)kPiece; }
+
+  // byte offset of this lane's 16 bytes; `parity`: q & 1
+  __device__ static __forceinline__ uint32_t lane_offset(int lane, int parity) {
+    if (!T) return lane * 16;
+    // rows are turned within the 16 so that the transposing reads of a wavefront meet no LDS bank twice
+    const int part = lane >> 5, chunk = (lane >> 4) & 1, slot = lane & 15;
+    return part * 1024 + chunk * 512 + (slot ^ (chunk * 4) ^ (parity * 8)) * 16;
+  }
+  // byte offset within a stage's operand of this lane's first read of block 0
+  __device__ static __forceinline__ uint32_t read_offset(int lane) {
+    if (!T) return lane * 16;
+    const int g = lane >> 4, i = lane & 15, chunk = (i & 3) >> 1;
+    const int slot = ((g >> 1) * 8 + (i >> 2)) ^ (chunk * 4) ^ ((g & 1) * 8);
+    return (g & 1) * 1024 + chunk * 256 + slot * 16 + (i & 1) * 8;
+  }
+  __device__ static __forceinline__ h8 read(const char* smem, uint32_t offset, int part) {
+    if (!T) return *reinterpret_cast<const h8*>(smem + offset + part * 1024);
+    auto q = [&](uint32_t o) {
+      return __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+          (__attribute__((address_space(3))) fp4*)(__attribute__((address_space(3))) char*)(smem + o));
+    };
+    const h4 lo = __builtin_bit_cast(h4, q(offset + part * 512));
+    const h4 hi = __builtin_bit_cast(h4, q((offset ^ 64) + part * 512));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+template <bool AT, bool BT, bool LOUD>
+__device__ __forceinline__ void pair_product(const PairMatrix& A, const PairMatrix& B, int64_t m0, int64_t n0,
+                                             int64_t k0, int steps, char* smem, f16v (&acc)[2][4]) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+
+  PairStream<AT> sa[2];
+  PairStream<BT> sb[4];
+#pragma unroll
+  for (int j = 0; j < 2; j++) sa[j].start(A, m0, wave * 2 + j, k0);
+#pragma unroll
+  for (int j = 0; j < 4; j++) sb[j].start(B, n0, wave * 4 + j, k0);
+  uint32_t oa[2], ob[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    oa[j] = PairStream<AT>::lane_offset(lane, j);
+    ob[j] = PairStream<BT>::lane_offset(lane, j);
+  }
+  int fetched = 0;
+  uint32_t into = 0;
+  auto fetch = [&]() {
+    const uint32_t to = lds0 + into;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      dma16(to + (wave * 2 + j) * 1024, oa[AT ? j : 0], reinterpret_cast<const float*>(sa[j].at));
+      sa[j].next(fetched & 1);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      dma16(to + kStageA + (wave * 4 + j) * 1024, ob[BT ? (j & 1) : 0], reinterpret_cast<const float*>(sb[j].at));
+      sb[j].next(fetched & 1);
+    }
+    fetched++;
+    into = into == (kRing - 1) * kStage ? 0 : into + kStage;
+  };
+
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+
+  const uint32_t ra = PairStream<AT>::read_offset(lane) + (wave >> 1) * 2 * kPiece;
+  const uint32_t rb = PairStream<BT>::read_offset(lane) + kStageA + (wave & 1) * 4 * kPiece;
+
+  fetch();
+  if (steps > 1) fetch();
+  uint32_t from = 0;
+  for (int s = 0; s < steps; s++) {
+    // this wavefront's part of the stage has landed when at most the next stage's six loads are in flight; its own
+    // reads of the stage before have ended
+    if (s + 1 < steps)
+      asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // everybody is past the products of the step before: its stage is free
+    if (s + 2 < steps) fetch();
+    h8 ah[2], al[2], bh[4], bl[4];
+    const char* st = smem + from;
+#pragma unroll
+    for (int i = 0; i < 2; i++) ah[i] = PairStream<AT>::read(st, ra + i * kPiece, 0);
+#pragma unroll
+    for (int j = 0; j < 4; j++) bh[j] = PairStream<BT>::read(st, rb + j * kPiece, 0);
+#pragma unroll
+    for (int j = 0; j < 4; j++) bl[j] = PairStream<BT>::read(st, rb + j * kPiece, 1);
+#pragma unroll
+    for (int i = 0; i < 2; i++) al[i] = PairStream<AT>::read(st, ra + i * kPiece, 1);
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
+    if (LOUD) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) bh[j] = bh[j] * (_Float16)0.00048828125f;   // 2^-11
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
+    from = from == (kRing - 1) * kStage ? 0 : from + kStage;
+  }
+}
+
+// Tile order: workgroups go to the eight XCDs round robin, so each XCD gets a contiguous range of tiles, walked in
+// groups of 8 tiles along m so that neighbours share operand rows in that XCD's L2.
+__device__ __forceinline__ void pair_tile(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t* tm, uint32_t* tn) {
+  const uint32_t all = tiles_m * tiles_n, per = all / 8;
+  if (id < per * 8) id = (id & 7) * per + (id >> 3);
+  const uint32_t group = 8 * tiles_n, g = id / group, rest = id - g * group;
+  const uint32_t high = tiles_m - g * 8 < 8 ? tiles_m - g * 8 : 8;
+  *tn = rest / high;
+  *tm = g * 8 + rest - *tn * high;
+}
+
+// hi and lo of a scaled number
+__device__ __forceinline__ void split_pair(float a, _Float16* hi, _Float16* lo) {
+  const _Float16 h = (_Float16)a;
+  *hi = h;
+  *lo = (_Float16)(a - (float)h);
+}
+
+// The exponent e whose 2^e brings `largest` into [2^14, 2^15); at most 126, so that 2^e is a binary32 number.
+__device__ __forceinline__ int pair_exponent(float largest) {
+  if (!(largest > 0.0f)) return 0;
+  const int e = 15 - __builtin_amdgcn_frexp_expf(largest);   // largest = f 2^x, f in [1/2, 1)
+  return e < 126 ? e : 126;
+}
+
+}  // namespace wf2

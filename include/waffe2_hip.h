@@ -840,8 +840,10 @@ int wf2hip_attention_backward_f32(const wf2hip_attention_desc* desc, const float
  * logit: its loss is NaN, and so are the gradients.  reduction: the losses one by one
  * (loss has `rows` elements), their sum, or their mean over the rows that have a label (loss has
  * one element; the mean of no rows is NaN).  lse(rows) is what the backward needs.  All arrays contiguous; the
- * outputs overlap nothing else.  dim, vocab >= 1; every extent below 2^31.  Scratch comes from the
- * library's pool. */
+ * outputs overlap nothing else.  w and the rows of x that have a label must hold finite numbers (otherwise the
+ * losses they meet are NaN).  dim, vocab >= 1; at most 2^28 rows and words, 2^20 elements of a hidden state
+ * (WF2HIP_EUNSUPPORTED).  Scratch comes from the library's pool: about the size of x and w, and 8 bytes per row
+ * and 128 words. */
 enum wf2hip_reduction { WF2HIP_REDUCE_NONE = 0, WF2HIP_REDUCE_SUM = 1, WF2HIP_REDUCE_MEAN = 2 };
 int wf2hip_linear_cross_entropy_f32(long rows, long dim, long vocab, const float* x, const float* w,
                                     const int32_t* labels, int reduction, float* loss, float* lse);
