@@ -1,0 +1,388 @@
+// adamw.hip -- one AdamW step over many tensors in one launch, its states in 32 bits or in 8.
+//
+//   m <- m + (g - m) (1 - b1)        v <- v + (1 - b2) (g g - v)             (the reference's Adam,
+//   p <- p - lr wd p - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)     source/optimizers/impls/adam.lisp:45-117,
+//                                                                             with the decay of the weights apart)
+// Bound by HBM: 28 bytes per parameter with 32-bit states, 16 with 8-bit ones.  A model has hundreds of tensors, most of
+// them vectors: one launch per tensor costs more than their work, so the tensors' addresses travel as kernel arguments
+// and a workgroup finds the tensor its 4096 elements belong to by comparing its index with every tensor's first workgroup,
+// a tensor per lane.
+//
+// States in 8 bits: blocks of 256 consecutive elements of a tensor share a scale, largest / 448, and an element is an e4m3
+// number times that scale: half a step is 2^-4 of the element, down to 2^-6 / 448 of the block's largest, 2^-10 / 448
+// absolute below.  The scale follows the block's largest exactly, so a block whose elements shrink together keeps its
+// codes and loses nothing.  The second moment is held as r = sqrt(v): the root halves the range of exponents that a
+// block has to span (2^17 down to the smallest code, 2^35 of v) and is what the step divides by.  The parameters take
+// the step of the unrounded moments.  A wavefront holds a block, four elements per lane.
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "wf2_common.h"
+
+namespace wf2 {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+constexpr int kAdamwBlock = 256;                         // elements that share a scale
+constexpr int kAdamwUnroll = 4;                          // vectors of four elements per lane
+constexpr int kAdamwChunk = kBlock * 4 * kAdamwUnroll;   // elements of a workgroup
+
+template <int BITS>
+struct AdamwArgs {
+  // tensors per launch: as many as 4 KB of arguments take, 44 or 60 bytes each
+  static constexpr int kTensors = BITS == 32 ? 91 : 67;
+  float* p[kTensors];
+  const float* g[kTensors];
+  void* m[kTensors];
+  void* v[kTensors];
+  float* m_scale[BITS == 8 ? kTensors : 1];
+  float* r_scale[BITS == 8 ? kTensors : 1];
+  uint32_t n[kTensors];
+  uint32_t first[kTensors];    // first workgroup
+  float decay[kTensors];
+  double* steps;                    // b1^(t-1), b2^(t-1), t - 1, arrivals
+  const float* lr_at;               // learning rate on the device, or null
+  float lr, beta1, beta2, eps;
+  int32_t count;
+  int32_t last;                     // the step's last launch counts it
+};
+static_assert(sizeof(AdamwArgs<32>) <= 4096 && sizeof(AdamwArgs<8>) <= 4096, "kernel arguments");
+
+struct AdamwStep {
+  float omb1, omb2, rate, root, eps, decay;   // rate = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t), decay = lr wd
+};
+
+__device__ __forceinline__ void adamw1(float& p, float g, float& m, float& v, const AdamwStep& s) {
+  m = m + (g - m) * s.omb1;
+  v = v + s.omb2 * (g * g - v);
+  p = p - (s.decay * p + (s.rate * m) / (__builtin_sqrtf(v) * s.root + s.eps));
+}
+
+// The same step where the root of v is wanted too.
+__device__ __forceinline__ void adamw1_root(float& p, float g, float& m, float& r, const AdamwStep& s) {
+  float v = r * r;
+  m = m + (g - m) * s.omb1;
+  v = v + s.omb2 * (g * g - v);
+  r = __builtin_sqrtf(v);
+  p = p - (s.decay * p + (s.rate * m) / (r * s.root + s.eps));
+}
+
+// Largest over the wavefront, as a number that all lanes hold: within rows of 16 lanes, then across them.
+__device__ __forceinline__ float dpp_max(float v) {
+#define WF2_DPP(ctrl)                                                                                                  \
+  {                                                                                                                    \
+    const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true);                     \
+    v = fmaxf(v, __builtin_bit_cast(float, o));                                                                        \
+  }
+  WF2_DPP(0xB1)    // lanes 1 0 3 2
+  WF2_DPP(0x4E)    // lanes 2 3 0 1
+  WF2_DPP(0x141)   // halves of a row mirrored
+  WF2_DPP(0x140)   // rows mirrored
+  WF2_DPP(0x142)   // lane 15 of a row to the next row
+  WF2_DPP(0x143)   // lane 31 to the upper half
+#undef WF2_DPP
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
+__device__ __forceinline__ float finite_or_zero(float a) { return a < INFINITY ? a : 0.0f; }   // a >= 0 or NaN
+
+// e4m3 codes of four numbers over `scale` = one for the block; what is not finite becomes NaN and sets no scale.
+__device__ __forceinline__ uint32_t encode4(const float (&a)[4], float* scale) {
+  float top = 0.0f;
+#pragma unroll
+  for (int c = 0; c < 4; c++) top = fmaxf(top, finite_or_zero(__builtin_fabsf(a[c])));
+  top = dpp_max(top);
+  const float s = fmaxf(top / 448.0f, 1.17549435e-38f);
+  *scale = s;
+  const float up = 1.0f / s;
+  float y[4];
+#pragma unroll
+  for (int c = 0; c < 4; c++) {
+    y[c] = a[c] * up;
+    y[c] = __builtin_fabsf(y[c]) < 512.0f ? y[c] : NAN;
+  }
+  int code = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], code, true);
+}
+
+__device__ __forceinline__ void decode4(uint32_t code, float scale, float (&a)[4]) {
+  const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, true);
+  a[0] = lo.x * scale;
+  a[1] = lo.y * scale;
+  a[2] = hi.x * scale;
+  a[3] = hi.y * scale;
+}
+
+template <typename T, bool NT>
+__device__ __forceinline__ T fetch(const T* q) { return NT ? __builtin_nontemporal_load(q) : *q; }
+template <typename T, bool NT>
+__device__ __forceinline__ void put(T v, T* q) {
+  if (NT)
+    __builtin_nontemporal_store(v, q);
+  else
+    *q = v;
+}
+
+// Four elements from i on, as one vector where FULL, one by one up to n otherwise.
+template <bool FULL, bool NT>
+__device__ __forceinline__ f4 fetch4(const float* a, uint32_t i, uint32_t n) {
+  if (FULL) return fetch<f4, NT>(reinterpret_cast<const f4*>(a + i));
+  f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < 4; c++)
+    if (i + c < n) v[c] = a[i + c];
+  return v;
+}
+template <bool FULL, bool NT>
+__device__ __forceinline__ void put4(f4 v, float* a, uint32_t i, uint32_t n) {
+  if (FULL) {
+    put<f4, NT>(v, reinterpret_cast<f4*>(a + i));
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < 4; c++)
+    if (i + c < n) a[i + c] = v[c];
+}
+template <bool FULL, bool NT>
+__device__ __forceinline__ uint32_t fetch_codes(const uint8_t* a, uint32_t i, uint32_t n) {
+  if (FULL) return fetch<uint32_t, NT>(reinterpret_cast<const uint32_t*>(a + i));
+  uint32_t v = 0;
+#pragma unroll
+  for (int c = 0; c < 4; c++)
+    if (i + c < n) v |= (uint32_t)a[i + c] << (8 * c);
+  return v;
+}
+template <bool FULL, bool NT>
+__device__ __forceinline__ void put_codes(uint32_t v, uint8_t* a, uint32_t i, uint32_t n) {
+  if (FULL) {
+    put<uint32_t, NT>(v, reinterpret_cast<uint32_t*>(a + i));
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < 4; c++)
+    if (i + c < n) a[i + c] = (uint8_t)(v >> (8 * c));
+}
+
+struct AdamwTensor {
+  float* p;
+  const float* g;
+  void *m, *v;
+  float *m_scale, *r_scale;
+  uint32_t n, first;
+};
+
+// A workgroup's elements.  The four vectors of a lane are 256 elements apart; every load is issued before the step's
+// numbers, which come from memory too, are waited for.
+template <int BITS, bool FULL, bool NT, typename Numbers>
+__device__ __forceinline__ void adamw_chunk(const AdamwTensor& t, const Numbers& numbers) {
+  constexpr int U = kAdamwUnroll;
+  const int lane = threadIdx.x & (kWave - 1);
+  const uint32_t base = (uint32_t)__builtin_amdgcn_readfirstlane(t.first + (threadIdx.x / kWave) * kWave * 4 * U);
+  f4 p[U], g[U], m[U], v[U];
+  uint32_t mc[U], rc[U];
+  float ms[U], rs[U];
+  const uint32_t blocks = (t.n + kAdamwBlock - 1) / kAdamwBlock;
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const uint32_t i = base + u * kAdamwBlock + lane * 4;
+    p[u] = fetch4<FULL, NT>(t.p, i, t.n);
+    g[u] = fetch4<FULL, NT>(t.g, i, t.n);
+    if (BITS == 32) {
+      m[u] = fetch4<FULL, NT>((const float*)t.m, i, t.n);
+      v[u] = fetch4<FULL, NT>((const float*)t.v, i, t.n);
+    } else {
+      const uint32_t b = base / kAdamwBlock + u;
+      mc[u] = fetch_codes<FULL, NT>((const uint8_t*)t.m, i, t.n);
+      rc[u] = fetch_codes<FULL, NT>((const uint8_t*)t.v, i, t.n);
+      ms[u] = FULL || b < blocks ? t.m_scale[b] : 0.0f;
+      rs[u] = FULL || b < blocks ? t.r_scale[b] : 0.0f;
+    }
+  }
+  const AdamwStep s = numbers();
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const uint32_t i = base + u * kAdamwBlock + lane * 4;
+    if (BITS == 32) {
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        float pe = p[u][c], me = m[u][c], ve = v[u][c];
+        adamw1(pe, g[u][c], me, ve, s);
+        p[u][c] = pe;
+        m[u][c] = me;
+        v[u][c] = ve;
+      }
+      put4<FULL, NT>(p[u], t.p, i, t.n);
+      put4<FULL, NT>(m[u], (float*)t.m, i, t.n);
+      put4<FULL, NT>(v[u], (float*)t.v, i, t.n);
+    } else {
+      const uint32_t b = base / kAdamwBlock + u;
+      if (!FULL && b >= blocks) break;   // the whole wavefront
+      float me[4], re[4];
+      decode4(mc[u], ms[u], me);
+      decode4(rc[u], rs[u], re);
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        float pe = p[u][c];
+        adamw1_root(pe, g[u][c], me[c], re[c], s);
+        p[u][c] = pe;
+        // elements behind the tensor were fetched as zeros: their moments stay zero and set no scale
+      }
+      float m_scale, r_scale;
+      const uint32_t m_code = encode4(me, &m_scale), r_code = encode4(re, &r_scale);
+      put4<FULL, NT>(p[u], t.p, i, t.n);
+      put_codes<FULL, NT>(m_code, (uint8_t*)t.m, i, t.n);
+      put_codes<FULL, NT>(r_code, (uint8_t*)t.v, i, t.n);
+      if (lane == 0) {
+        t.m_scale[b] = m_scale;
+        t.r_scale[b] = r_scale;
+      }
+    }
+  }
+}
+
+template <int BITS, bool NT>
+__global__ __launch_bounds__(kBlock) void adamw_kernel(AdamwArgs<BITS> a) {
+  __shared__ float numbers[2];
+  // the last tensor whose first workgroup is not behind this one
+  const int lane = threadIdx.x & (kWave - 1);
+  int at = -1;
+#pragma unroll
+  for (int t = 0; t < AdamwArgs<BITS>::kTensors; t += kWave)
+    at += __builtin_popcountll(__ballot(t + lane < a.count && a.first[t + lane < a.count ? t + lane : 0] <= blockIdx.x));
+  at = __builtin_amdgcn_readfirstlane(at);
+  AdamwTensor t{a.p[at], a.g[at], a.m[at], a.v[at], a.m_scale[BITS == 8 ? at : 0], a.r_scale[BITS == 8 ? at : 0], a.n[at], (blockIdx.x - a.first[at]) * (uint32_t)kAdamwChunk};
+  const float lr = a.lr_at ? a.lr_at[0] : a.lr;
+  const float weight_decay = a.decay[at];
+  // What the step's number gives, in binary64: b^t from the product that the states carry along.  The last workgroup to
+  // have read it counts the step.
+  if (threadIdx.x == 0) {
+    const double p1 = a.steps[0] * (double)a.beta1, p2 = a.steps[1] * (double)a.beta2;
+    numbers[0] = (float)((double)lr / (1.0 - p1));
+    numbers[1] = (float)(1.0 / __builtin_sqrt(1.0 - p2));
+    if (a.last) {
+      const double done = a.steps[2];
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // read before the arrival is counted
+      unsigned int* arrivals = reinterpret_cast<unsigned int*>(a.steps + 3);
+      if (__hip_atomic_fetch_add(arrivals, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
+        a.steps[0] = p1;
+        a.steps[1] = p2;
+        a.steps[2] = done + 1.0;
+        *arrivals = 0u;
+      }
+    }
+  }
+  auto step = [&]() {
+    __syncthreads();
+    return AdamwStep{1.0f - a.beta1, 1.0f - a.beta2, numbers[0], numbers[1], a.eps, lr * weight_decay};
+  };
+  // whole vectors of every stream, and a whole chunk
+  const bool aligned = (((uintptr_t)t.p | (uintptr_t)t.g) & 15) == 0 &&
+                       (((uintptr_t)t.m | (uintptr_t)t.v) & (BITS == 32 ? 15 : 3)) == 0;
+  if (aligned && t.n - t.first >= kAdamwChunk)
+    adamw_chunk<BITS, true, NT>(t, step);
+  else
+    adamw_chunk<BITS, false, NT>(t, step);
+}
+
+// Launches of as many tensors as their arguments allow; the last one counts the step.
+template <int BITS, bool NT>
+static int adamw_launches(const wf2hip_adamw_desc& d, long count, const wf2hip_adamw_tensor* tensors, double* steps) {
+  long i = 0;
+  while (i < count) {
+    AdamwArgs<BITS> a{};
+    int64_t blocks = 0;
+    for (; i < count && a.count < AdamwArgs<BITS>::kTensors; i++) {
+      const wf2hip_adamw_tensor& t = tensors[i];
+      if (t.n == 0) continue;
+      const int64_t here = ceil_div(t.n, kAdamwChunk);
+      if (blocks + here > INT32_MAX) break;
+      const int k = a.count++;
+      a.p[k] = t.param;
+      a.g[k] = t.grad;
+      a.m[k] = t.m;
+      a.v[k] = t.v;
+      if (BITS == 8) {
+        a.m_scale[k] = t.m_scale;
+        a.r_scale[k] = t.r_scale;
+      }
+      a.n[k] = (uint32_t)t.n;
+      a.first[k] = (uint32_t)blocks;
+      a.decay[k] = t.weight_decay;
+      blocks += here;
+    }
+    while (i < count && tensors[i].n == 0) i++;
+    a.steps = steps;
+    a.lr_at = d.lr_device;
+    a.lr = d.lr;
+    a.beta1 = d.beta1;
+    a.beta2 = d.beta2;
+    a.eps = d.eps;
+    a.last = i == count;
+    adamw_kernel<BITS, NT><<<(uint32_t)blocks, kBlock, 0, rt().stream>>>(a);
+    WF2_TRY(after_launch("adamw_kernel"));
+  }
+  return 0;
+}
+
+}  // namespace wf2
+
+using namespace wf2;
+
+WF2_API int wf2hip_adamw_step(const wf2hip_adamw_desc* d, long count, const wf2hip_adamw_tensor* tensors, double* steps) {
+  const char* name = "adamw step";
+  WF2_TRY(require_init());
+  if (!d || count < 0 || (count && !tensors) || !steps) return fail(WF2HIP_EINVAL, "%s: null pointer or negative count", name);
+  if (d->state_bits != 8 && d->state_bits != 32) return fail(WF2HIP_EINVAL, "%s: states have 8 or 32 bits, not %d", name, d->state_bits);
+  if (!(d->beta1 >= 0.0f && d->beta1 < 1.0f && d->beta2 >= 0.0f && d->beta2 < 1.0f))
+    return fail(WF2HIP_EINVAL, "%s: decay rates must be in [0, 1)", name);
+  const bool bytes8 = d->state_bits == 8;
+  try {
+    struct Range {
+      uintptr_t from, to;
+      bool written;
+    };
+    std::vector<Range> ranges;
+    ranges.reserve(6 * (size_t)count + 2);
+    auto add = [&](const void* q, int64_t bytes, bool written) {
+      if (bytes) ranges.push_back(Range{(uintptr_t)q, (uintptr_t)q + (uintptr_t)bytes, written});
+    };
+    int64_t total = 0;
+    for (long i = 0; i < count; i++) {
+      const wf2hip_adamw_tensor& t = tensors[i];
+      if (t.n < 0) return fail(WF2HIP_EINVAL, "%s: tensor %ld has a negative element count", name, i);
+      if (t.n == 0) continue;
+      if (!t.param || !t.grad || !t.m || !t.v || (bytes8 && (!t.m_scale || !t.r_scale))) return fail(WF2HIP_EINVAL, "%s: null pointer in tensor %ld", name, i);
+      if (t.n >= ((int64_t)1 << 32) - kAdamwChunk) return fail(WF2HIP_EUNSUPPORTED, "%s: tensor %ld has 2^32 elements or more", name, i);
+      if ((((uintptr_t)t.param | (uintptr_t)t.grad) & 3) || (!bytes8 && (((uintptr_t)t.m | (uintptr_t)t.v) & 3)) ||
+          (bytes8 && (((uintptr_t)t.m_scale | (uintptr_t)t.r_scale) & 3)))
+        return fail(WF2HIP_EINVAL, "%s: misaligned pointer in tensor %ld", name, i);
+      add(t.param, t.n * 4, true);
+      add(t.grad, t.n * 4, false);
+      add(t.m, t.n * (bytes8 ? 1 : 4), true);
+      add(t.v, t.n * (bytes8 ? 1 : 4), true);
+      if (bytes8) {
+        add(t.m_scale, ceil_div(t.n, kAdamwBlock) * 4, true);
+        add(t.r_scale, ceil_div(t.n, kAdamwBlock) * 4, true);
+      }
+      total += t.n;
+    }
+    if (total == 0) return 0;   // a model without elements: no step to count
+    add(steps, 32, true);
+    if (d->lr_device) add(d->lr_device, 4, false);
+    std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+    uintptr_t any = 0, written = 0;   // the furthest ends so far
+    for (const Range& r : ranges) {
+      if (r.from < written || (r.written && r.from < any))
+        return fail(WF2HIP_EOVERLAP, "%s: something the step writes overlaps another of its buffers", name);
+      any = std::max(any, r.to);
+      if (r.written) written = std::max(written, r.to);
+    }
+    const bool streaming = total * (bytes8 ? 16 : 28) >= ((int64_t)192 << 20);   // far beyond the Infinity Cache
+    return bytes8 ? (streaming ? adamw_launches<8, true>(*d, count, tensors, steps) : adamw_launches<8, false>(*d, count, tensors, steps))
+                  : (streaming ? adamw_launches<32, true>(*d, count, tensors, steps) : adamw_launches<32, false>(*d, count, tensors, steps));
+  } catch (const std::bad_alloc&) {
+    return fail(WF2HIP_ENOMEM, "%s: out of host memory", name);
+  }
+}

@@ -107,6 +107,24 @@ class AttentionDesc(C.Structure):
     ]
 
 
+class AdamWTensor(C.Structure):
+    """``struct wf2hip_adamw_tensor``"""
+
+    _fields_ = [
+        ("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p),
+        ("r_scale", C.c_void_p), ("n", C.c_int64), ("weight_decay", C.c_float), ("reserved", C.c_int32),
+    ]
+
+
+class AdamWDesc(C.Structure):
+    """``struct wf2hip_adamw_desc``"""
+
+    _fields_ = [
+        ("lr_device", C.c_void_p), ("lr", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float),
+        ("state_bits", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
 _SIGNATURES = {
     "wf2hip_abi_version": ([], C.c_int),
     "wf2hip_init": ([C.c_int], C.c_int),
@@ -196,6 +214,7 @@ _SIGNATURES = {
     "wf2hip_unfold_f32": ([_L] * 10 + [_P, _P], C.c_int),
     "wf2hip_sgd_step_f32": ([_L, _P, _P, _F], C.c_int),
     "wf2hip_adam_step_f32": ([_L, _P, _P, _P, _P, _F, _F, _F, _F], C.c_int),
+    "wf2hip_adamw_step": ([C.POINTER(AdamWDesc), _L, C.POINTER(AdamWTensor), _P], C.c_int),
     "wf2hip_embedding_add_f32": ([_L, _L, _L, _P, _P, _L, _P, _L, _P], C.c_int),
     "wf2hip_linear_cross_entropy_f32": ([_L] * 3 + [_P] * 3 + [C.c_int] + [_P] * 2, C.c_int),
     "wf2hip_linear_cross_entropy_backward_f32": ([_L] * 3 + [_P] * 4 + [C.c_int, _P, _F] + [_P] * 2, C.c_int),

@@ -1,4 +1,4 @@
-"""SGD and Adam on HIPTensor parameters.
+"""SGD, Adam and AdamW on HIPTensor parameters.
 
 Mirror of ``source/optimizers/impls/sgd.lisp`` and ``adam.lisp``: an optimiser
 object owns one parameter (``defoptimizer`` ties it to ``param``) and
@@ -9,6 +9,9 @@ object owns one parameter (``defoptimizer`` ties it to ``param``) and
 ``fused``  one kernel per step (``wf2hip_sgd_step_f32`` / ``wf2hip_adam_step_f32``)
            that performs the same binary32 operations in the same order:
            bit-identical, a few per cent of the memory traffic.
+
+AdamW has no counterpart in the reference: it steps all parameters of a model in
+one call (``wf2hip_adamw_step``), its states in 32 bits or in 8.
 """
 from __future__ import annotations
 
@@ -103,3 +106,89 @@ class Adam:
         _lib.check(_lib.get().wf2hip_adam_step_f32(n, p, g, C.c_void_p(self.m.ptr), C.c_void_p(self.v.ptr),
                                                   omb1, omb2, lr_t, self.eps))
         return self.param
+
+
+class AdamW:
+    """Adam with the weights' decay apart from the gradient, over all parameters at once:
+
+        m <- m + (g - m) (1 - beta1);   v <- v + (1 - beta2) (g g - v)
+        p <- p - lr weight_decay p - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
+
+    ``params``: contiguous :float tensors.  ``weight_decay``: a number, or one per parameter.  ``lr`` may be a
+    one-element :float tensor, read on the device at every step.  ``state_bits=8`` holds m and r = sqrt(v) as e4m3
+    numbers (:uint8 tensors of codes) with a scale per 256 elements: 2 bytes per parameter instead of 8.  The number of steps
+    is kept on the device: a step recorded into a graph counts on with every replay.
+
+    ``state()`` returns what a checkpoint has to hold: ``n`` (steps done) and lists ``m``, ``v`` (32 bits) or ``m``,
+    ``r``, ``m_scale``, ``r_scale`` (8 bits) with a tensor per parameter; ``resume=`` takes such a dict and adopts its
+    tensors."""
+
+    BLOCK = 256   # elements of a tensor that share a scale
+
+    def __init__(self, params, lr: float | HIPTensor = 1e-3, eps: float = 1e-8, beta1: float = 0.9, beta2: float = 0.999,
+                 weight_decay=0.01, state_bits: int = 32, resume: dict | None = None):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: states have 8 or 32 bits, not {state_bits}")
+        self.params, self.lr, self.state_bits = list(params), lr, state_bits
+        self.beta1, self.beta2, self.eps = float(np.float32(beta1)), float(np.float32(beta2)), float(eps)
+        sizes = [self._own("a parameter", p) for p in self.params]
+        decays = [float(weight_decay)] * len(sizes) if isinstance(weight_decay, F.Number) else [float(d) for d in weight_decay]
+        if len(decays) != len(sizes):
+            raise ValueError(f"AdamW: {len(decays)} decays for {len(sizes)} parameters")
+        blocks = [-(-n // self.BLOCK) for n in sizes]
+        kinds = {"m": ("float", sizes), "v": ("float", sizes)} if state_bits == 32 else \
+            {"m": ("uint8", sizes), "r": ("uint8", sizes), "m_scale": ("float", blocks), "r_scale": ("float", blocks)}
+        done = int(resume["n"]) if resume else 0
+        if done < 0:
+            raise ValueError("AdamW: a negative number of steps done")
+        self._states = {}
+        for name, (dtype, counts) in kinds.items():
+            given = list(resume[name]) if resume else [HIPTensor([n], dtype=dtype) if name.endswith("scale") else
+                                                      HIPTensor(p.shape, dtype=dtype) for n, p in zip(counts, self.params)]
+            if len(given) != len(sizes):
+                raise ValueError(f"AdamW: {len(given)} tensors {name} for {len(sizes)} parameters")
+            for t, n in zip(given, counts):
+                if self._own(name, t, dtype) != n:
+                    raise ValueError(f"AdamW: {name} has {t.size} elements where {n} belong")
+            self._states[name] = given
+        b1, b2 = self.beta1, self.beta2
+        self._steps = HIPTensor.from_numpy(np.array([b1 ** done, b2 ** done, done, 0.0]), dtype="double")
+        self._table = (_lib.AdamWTensor * len(sizes))()
+        scales = [self._states[k] if k in self._states else [None] * len(sizes) for k in ("m_scale", "r_scale")]
+        second = self._states["v" if state_bits == 32 else "r"]
+        for row, p, n, d, m, v, ms, rs in zip(self._table, self.params, sizes, decays, self._states["m"], second, *scales):
+            row.param, row.m, row.v, row.n, row.weight_decay = p.ptr, m.ptr, v.ptr, n, d
+            row.m_scale, row.r_scale = ms.ptr if ms else None, rs.ptr if rs else None
+
+    @staticmethod
+    def _own(what: str, t: HIPTensor, dtype: str = "float") -> int:
+        if t.dtype != dtype or not t.is_contiguous():
+            raise ValueError(f"AdamW: {what} must be a contiguous :{dtype} tensor that owns its storage")
+        return t.size
+
+    @property
+    def n(self) -> int:
+        """Steps done (waits for the device)."""
+        return int(self._steps.numpy()[2])
+
+    def state(self) -> dict:
+        return {"n": self.n, **{name: list(tensors) for name, tensors in self._states.items()}}
+
+    def step(self, grads) -> list:
+        """One step with a gradient per parameter (contiguous :float tensors of the parameters' sizes)."""
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError(f"AdamW: {len(grads)} gradients for {len(self.params)} parameters")
+        for row, g in zip(self._table, grads):
+            if g.dtype != "float" or g.size != row.n or not g.is_contiguous():
+                raise ValueError("AdamW: a gradient must be a contiguous :float tensor of its parameter's size")
+            row.grad = g.ptr
+        d = _lib.AdamWDesc(beta1=self.beta1, beta2=self.beta2, eps=self.eps, state_bits=self.state_bits)
+        if isinstance(self.lr, HIPTensor):
+            if self._own("lr", self.lr) != 1:
+                raise ValueError("AdamW: lr must be a number or a one-element tensor")
+            d.lr_device = self.lr.ptr
+        else:
+            d.lr = float(self.lr)
+        _lib.check(_lib.get().wf2hip_adamw_step(C.byref(d), len(grads), self._table, C.c_void_p(self._steps.ptr)))
+        return self.params

@@ -789,6 +789,41 @@ int wf2hip_sgd_step_f32(long n, float* param, float* grad, float lr);
 int wf2hip_adam_step_f32(long n, float* param, const float* grad, float* m, float* v,
                          float one_minus_beta1, float one_minus_beta2, float lr_t, float eps);
 
+/* One AdamW step over `count` tensors in one launch (one per 91 tensors, 67 with 8-bit states), the weights' decay apart from the gradient:
+ *   m <- m + (g - m) (1 - beta1),   v <- v + (1 - beta2) (g g - v),
+ *   param <- param - lr weight_decay param - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps),
+ * t the number of this step.  The reference has Adam only (source/optimizers/impls/adam.lisp:45-117), a tensor
+ * at a time.  state_bits 32: m and v are floats.  state_bits 8: m holds codes of m and v codes of r = sqrt(v),
+ * one byte per element, in blocks of 256 consecutive elements of a tensor: an e4m3 number (sign, 4 bits of
+ * exponent under a bias of 7, 3 of mantissa) times the block's scale, max(largest |element| / 448, 2^-126),
+ * rounded to nearest; m_scale and r_scale hold ceil(n / 256) scales each.  The parameters take the step of the
+ * unrounded moments.  An element that is not finite is left out of its block's scale and becomes NaN.  Zero bytes and scales
+ * are the state before the first step.
+ * steps: four doubles on the device, which the step reads and moves on: beta1^(t-1), beta2^(t-1), t - 1 and a
+ * counter that is zero between steps; {1, 1, 0, 0} before the first one.  They are on the device so that a recorded step counts
+ * on with every replay; lr_device, if not NULL, is a float there that stands for lr.
+ * Contiguous tensors of fewer than 2^32 - 4096 elements; a gradient may serve several tensors, nothing that is written may
+ * overlap anything else (WF2HIP_EOVERLAP). */
+typedef struct wf2hip_adamw_tensor {
+  float* param;
+  const float* grad;
+  void* m;
+  void* v;
+  float* m_scale; /* 8-bit states only */
+  float* r_scale;
+  int64_t n;
+  float weight_decay;
+  int32_t reserved;
+} wf2hip_adamw_tensor;
+typedef struct wf2hip_adamw_desc {
+  const float* lr_device;
+  float lr, beta1, beta2, eps;
+  int32_t state_bits; /* 8 or 32 */
+  int32_t reserved;
+} wf2hip_adamw_desc;
+int wf2hip_adamw_step(const wf2hip_adamw_desc* desc, long count, const wf2hip_adamw_tensor* tensors,
+                      double* steps);
+
 /* ---- attention (extension; no BLAS counterpart) ---------------------------- */
 /* O[b,h,i,:] = sum_j softmax_j(scale * Q[b,h,i,:].K[b,h,j,:] (+ causal mask j <= i)) V[b,h,j,:]
  * in one kernel, replacing the node sequence !matmul, scalar multiply, mask add,

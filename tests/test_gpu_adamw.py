@@ -1,0 +1,379 @@
+"""AdamW over many tensors at once, its states in 32 bits or in 8, against float64.
+
+Tolerances.  One step in binary32, U = 2^-24: m = m + (g - m) c takes three roundings of numbers no larger than
+|m| + |g|, v four of numbers no larger than v + g^2; p two roundings of its own plus the update's, whose factors (root, sum,
+quotient, the two corrections) add up to at most 12 U of its size, and the relative errors of m and v as the
+update passes them on.  8-bit states: half a step of e4m3, 2^-4 of the element or 2^-10 of the scale (subnormal codes),
+and as the rounding border may be met from either side, the binary32 errors on top."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+f32 = np.float32
+U = 2.0 ** -24
+HYPER = dict(lr=6e-3, eps=1e-8, beta1=0.9, beta2=0.95)
+
+
+def e4m3_values():
+    c = np.arange(256)
+    e, f = (c >> 3) & 15, c & 7
+    a = np.where(e == 0, f * 2.0 ** -9, (1.0 + f / 8.0) * 2.0 ** (e - 7.0))
+    a[(c & 127) == 127] = np.nan
+    return np.where(c & 128, -a, a)
+
+
+VALUES = e4m3_values()
+
+
+def decode(codes, scale):
+    flat = VALUES[codes.ravel()]
+    return flat * np.repeat(scale.astype(np.float64), 256)[:flat.size]
+
+
+def reference(p, g, m, v, t, decay, hyper=HYPER):
+    """One step in float64: p, m, v and their bounds for a binary32 implementation."""
+    b1, b2 = float(f32(hyper["beta1"])), float(f32(hyper["beta2"]))
+    lr, eps = float(f32(hyper["lr"])), float(f32(hyper["eps"]))
+    p, g, m, v = (a.astype(np.float64) for a in (p, g, m, v))
+    m1 = m + (g - m) * (1 - b1)
+    v1 = v + (1 - b2) * (g * g - v)
+    root = np.sqrt(v1 / (1 - b2 ** t)) + eps
+    update = lr * (m1 / (1 - b1 ** t)) / root
+    p1 = p - lr * float(f32(decay)) * p - update
+    # 1 - beta in binary32 is itself rounded: U (1 - beta) of the numbers it multiplies
+    em = 4 * U * (np.abs(m) + np.abs(g)) + 1e-45
+    ev = 6 * U * (v + g * g) + 1e-45
+    eu = lr / (1 - b1 ** t) * em / root + np.abs(update) * (0.5 * ev / np.maximum(v1, 1e-300) + 12 * U)
+    ep = 3 * U * (np.abs(p) + np.abs(p1)) + 4 * U * lr * float(decay) * np.abs(p) + eu
+    return p1, m1, v1, ep, em, ev
+
+
+def numbers(n, seed, first=False):
+    rng = np.random.default_rng(seed)
+    size = np.exp(2.0 * rng.standard_normal(n)) * 1e-3
+    p = rng.standard_normal(n) * 0.05
+    g = rng.standard_normal(n) * size
+    m = np.zeros(n) if first else rng.standard_normal(n) * size * 0.3
+    v = np.zeros(n) if first else (size * rng.uniform(0.5, 1.5, n)) ** 2
+    return tuple(a.astype(f32) for a in (p, g, m, v))
+
+
+# one element, a vector's and a block's ends, a chunk's ends (4096), several chunks, two dimensions
+SIZES = [1, 3, 4, 5, 255, 256, 257, 260, 511, 513, 1000, 4095, 4096, 4097, 8192, 12289, 70000]
+
+
+def test_e4m3_values():
+    """The table: 126 positive numbers, the largest 448, steps of one eighth of the power of two below."""
+    a = VALUES[:127]
+    assert a[0] == 0 and a[1] == 2.0 ** -9 and a[126] == 448 and np.all(np.diff(a) > 0)
+    assert np.all((np.diff(a) / a[1:])[8:] <= 2.0 ** -3)
+
+
+def test_reference_matches_a_spelt_out_step():
+    p, g, m, v = numbers(5, 0)
+    t, d = 3, 0.1
+    p1, m1, v1, *_ = reference(p, g, m, v, t, d)
+    for i in range(5):
+        b1, b2 = float(f32(0.9)), float(f32(0.95))
+        mm = b1 * float(m[i]) + (1 - b1) * float(g[i])
+        vv = b2 * float(v[i]) + (1 - b2) * float(g[i]) ** 2
+        want = float(p[i]) * (1 - float(f32(6e-3)) * float(f32(d))) - float(f32(6e-3)) * (mm / (1 - b1 ** t)) / (np.sqrt(vv / (1 - b2 ** t)) + float(f32(1e-8)))
+        assert abs(want - p1[i]) < 1e-15 and abs(mm - m1[i]) < 1e-18 and abs(vv - v1[i]) < 1e-18
+
+
+def tensors(W, arrays, dtype="float"):
+    return [W.functional.from_numpy(a, dtype=dtype) for a in arrays]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 2, 1000])
+def test_states_in_32_bits(gpu, t):
+    W = gpu
+    O = W.optimizers
+    data = [numbers(n, n, first=t == 1) for n in SIZES]
+    decays = [0.1 if i % 2 else 0.0 for i in range(len(SIZES))]
+    p, g, m, v = (tensors(W, [d[k] for d in data]) for k in range(4))
+    opt = O.AdamW(p, weight_decay=decays, resume=dict(n=t - 1, m=m, v=v), **HYPER)
+    assert opt.step(g) == p and opt.n == t
+    for i, d in enumerate(data):
+        p1, m1, v1, ep, em, ev = reference(*d, t, decays[i])
+        for got, want, err in ((p[i], p1, ep), (m[i], m1, em), (v[i], v1, ev)):
+            assert np.all(np.abs(got.numpy() - want) <= err), (SIZES[i], np.max(np.abs(got.numpy() - want) / err))
+        assert np.array_equal(g[i].numpy(), d[1])
+
+
+def check_codes(codes, scale, want, err, what):
+    """codes * scale against the unrounded float64 elements."""
+    n = want.size
+    blocks = -(-n // 256)
+    pad = np.zeros(blocks * 256)
+    pad[:n] = np.abs(want)
+    perr = np.zeros(blocks * 256)
+    perr[:n] = err
+    top = pad.reshape(blocks, 256).max(axis=1)
+    true_scale = np.maximum(top / 448.0, 2.0 ** -126)
+    slack = perr.reshape(blocks, 256).max(axis=1) / 448.0 + 2 * U * true_scale
+    assert np.all(np.abs(scale - true_scale) <= slack), what
+    got = decode(codes, scale)
+    s = np.repeat(true_scale, 256)[:n]
+    e = np.repeat(slack, 256)[:n]
+    bound = np.maximum(2.0 ** -4 * np.abs(want), 2.0 ** -10 * s) * (1 + 8 * U) + err + 449 * e + 4 * U * np.abs(want)
+    assert np.all(np.abs(got - want) <= bound), (what, np.max(np.abs(got - want) / bound))
+    # rounded to nearest: the neighbouring codes are no nearer, but for the binary32 error
+    grid = np.sort(VALUES[np.isfinite(VALUES)])
+    y = want / s
+    near = grid[np.clip(np.searchsorted(grid, y), 1, len(grid) - 1)]
+    below = grid[np.clip(np.searchsorted(grid, y) - 1, 0, len(grid) - 1)]
+    best = np.minimum(np.abs(near - y), np.abs(below - y))
+    mine = np.abs(VALUES[codes.ravel()] - y)
+    assert np.all(mine <= best + 2 * ((err + 449 * e) / s + 16 * U * np.abs(y)) + 1e-12), what
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 2, 1000])
+def test_states_in_8_bits(gpu, t):
+    W = gpu
+    O, F = W.optimizers, W.functional
+    rng = np.random.default_rng(t)
+    data = [numbers(n, 7 * n + t, first=t == 1) for n in SIZES]
+    p, g = (tensors(W, [d[k] for d in data]) for k in (0, 1))
+    if t == 1:
+        opt = O.AdamW(p, weight_decay=0.1, state_bits=8, **HYPER)
+        codes = [(np.zeros(n, np.uint8), np.zeros(n, np.uint8), np.zeros(-(-n // 256), f32), np.zeros(-(-n // 256), f32)) for n in SIZES]
+    else:
+        codes = []
+        for n, d in zip(SIZES, data):
+            blocks = -(-n // 256)
+            mc = rng.integers(0, 256, n).astype(np.uint8)
+            mc[(mc & 127) == 127] = 5
+            rc = rng.integers(0, 127, n).astype(np.uint8)
+            codes.append((mc, rc, np.exp(rng.standard_normal(blocks) - 12).astype(f32), np.exp(rng.standard_normal(blocks) - 11).astype(f32)))
+        opt = O.AdamW(p, weight_decay=0.1, state_bits=8, resume=dict(
+            n=t - 1, m=tensors(W, [c[0] for c in codes], "uint8"), r=tensors(W, [c[1] for c in codes], "uint8"),
+            m_scale=tensors(W, [c[2] for c in codes]), r_scale=tensors(W, [c[3] for c in codes])), **HYPER)
+    opt.step(g)
+    s = opt.state()
+    assert s["n"] == t
+    for i, d in enumerate(data):
+        m = decode(codes[i][0], codes[i][2])
+        v = decode(codes[i][1], codes[i][3]) ** 2
+        p1, m1, v1, ep, em, ev = reference(d[0], d[1], m, v, t, 0.1)
+        em, ev = em + 2 * U * np.abs(m), ev + 4 * U * v      # the decoded states are products, rounded
+        b1, b2 = float(f32(HYPER["beta1"])), float(f32(HYPER["beta2"]))
+        root = np.sqrt(v1 / (1 - b2 ** t)) + 1e-8
+        ep = ep + 6e-3 / (1 - b1 ** t) * (2 * U * np.abs(m) + np.abs(m1) * 2 * U * v / np.maximum(v1, 1e-300)) / root
+        assert np.all(np.abs(p[i].numpy() - p1) <= ep), (SIZES[i], np.max(np.abs(p[i].numpy() - p1) / ep))
+        r1 = np.sqrt(v1)
+        check_codes(s["m"][i].numpy(), s["m_scale"][i].numpy(), m1, em, f"m {SIZES[i]}")
+        check_codes(s["r"][i].numpy(), s["r_scale"][i].numpy(), r1, 0.5 * ev / np.maximum(r1, 1e-30) + U * r1, f"r {SIZES[i]}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_tensors_take_several_launches(gpu, bits):
+    """More tensors than one launch's arguments hold, empty ones among them: each as if it were alone."""
+    W = gpu
+    O = W.optimizers
+    rng = np.random.default_rng(bits)
+    sizes = [int(n) for n in rng.integers(1, 3000, 200)]
+    sizes[5] = sizes[90] = sizes[199] = 0
+    data = [numbers(n, 1000 + i, first=True) for i, n in enumerate(sizes)]
+    p, g = (tensors(W, [d[k] for d in data]) for k in (0, 1))
+    opt = O.AdamW(p, state_bits=bits, weight_decay=0.05, **HYPER)
+    for _ in range(3):
+        opt.step(g)
+    assert opt.n == 3
+    for i in (0, 4, 66, 67, 68, 91, 92, 133, 134, 198):
+        q, h = tensors(W, data[i][:2])
+        alone = O.AdamW([q], state_bits=bits, weight_decay=0.05, **HYPER)
+        for _ in range(3):
+            alone.step([h])
+        assert np.array_equal(q.numpy(), p[i].numpy())
+        a, b = opt.state(), alone.state()
+        for k in a:
+            if k != "n":
+                assert np.array_equal(a[k][i].numpy(), b[k][0].numpy())
+
+
+@pytest.mark.gpu
+def test_unaligned_storage_gives_the_same_bits(gpu):
+    """Tensors whose storages start 4 bytes (codes: 1 byte) behind a vector's border."""
+    W = gpu
+    lib = W.lib
+    n = 9001
+    p, g, m, v = numbers(n, 3)
+    for bits in (32, 8):
+        results = []
+        for shift in (0, 1):
+            bufs = [W.HIPTensor([n + 8]) for _ in range(6)]
+            codes = [W.HIPTensor([n + 8], dtype="uint8") for _ in range(2)]
+            for b, a in zip(bufs, (p, g, m, v)):
+                lib.check(lib.get().wf2hip_memcpy_h2d(C.c_void_p(b.ptr + 4 * shift), a.ctypes.data_as(C.c_void_p), 4 * n))
+            steps = W.HIPTensor.from_numpy(np.array([0.9, 0.95, 1, 0]), dtype="double")
+            row = lib.AdamWTensor(n=n, weight_decay=0.1)
+            row.param, row.grad = bufs[0].ptr + 4 * shift, bufs[1].ptr + 4 * shift
+            if bits == 32:
+                row.m, row.v = bufs[2].ptr + 4 * shift, bufs[3].ptr + 4 * shift
+            else:
+                row.m, row.v = codes[0].ptr + shift, codes[1].ptr + shift
+                row.m_scale, row.r_scale = bufs[4].ptr + 4 * shift, bufs[5].ptr + 4 * shift
+            d = lib.AdamWDesc(lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, state_bits=bits)
+            for _ in range(2):
+                lib.check(lib.get().wf2hip_adamw_step(C.byref(d), 1, C.byref(row), C.c_void_p(steps.ptr)))
+            out = [bufs[0].numpy()[shift:shift + n]]
+            out += [b.numpy()[shift:shift + n] for b in (bufs[2:4] if bits == 32 else codes)]
+            out += [b.numpy()[shift:shift + 36] for b in bufs[4:]]
+            results.append(out)
+            # what lies around the tensor is left alone
+            assert not bufs[0].numpy()[shift + n:].any() and not bufs[0].numpy()[:shift].any()
+            assert not codes[0].numpy()[shift + n:].any() and not codes[0].numpy()[:shift].any()
+        for a, b in zip(*results):
+            assert np.array_equal(a, b)
+
+
+@pytest.mark.gpu
+def test_replayed_steps_count_on(gpu):
+    """A recorded step: every replay is the next step, bit for bit, and follows the gradient and the rate."""
+    W = gpu
+    O, F = W.optimizers, W.functional
+    for bits in (32, 8):
+        data = [numbers(n, 40 + n, first=True) for n in (300, 5000, 7)]
+        p, g = (tensors(W, [d[k] for d in data]) for k in (0, 1))
+        q, h = (tensors(W, [d[k] for d in data]) for k in (0, 1))
+        rate = F.from_numpy(np.array([1e-3], f32))
+        opt = O.AdamW(p, lr=rate, state_bits=bits)
+        ref = O.AdamW(q, lr=1e-3, state_bits=bits)
+        opt.step(g)
+        ref.step(h)
+        with W.lib.Graph() as graph:
+            opt.step(g)
+        assert opt.n == 1
+        for i in range(4):
+            if i == 2:
+                F.move_(rate, F.from_numpy(np.array([5e-4], f32)))
+                ref.lr = 5e-4
+                F.mul_(g[1], -2.0)
+                F.mul_(h[1], -2.0)
+            graph.launch()
+            ref.step(h)
+            assert opt.n == ref.n == i + 2
+            for a, b in zip(p, q):
+                assert np.array_equal(a.numpy(), b.numpy()), (bits, i)
+        graph.destroy()
+        opt.step(g)      # and an eager step goes on from there
+        ref.step(h)
+        assert opt.n == ref.n and all(np.array_equal(a.numpy(), b.numpy()) for a, b in zip(p, q))
+
+
+@pytest.mark.gpu
+def test_resume_from_a_state(gpu):
+    W = gpu
+    O = W.optimizers
+    for bits in (32, 8):
+        data = [numbers(n, 60 + n, first=True) for n in (700, 33)]
+        p, g = (tensors(W, [d[k] for d in data]) for k in (0, 1))
+        opt = O.AdamW(p, state_bits=bits, **HYPER)
+        for _ in range(5):
+            opt.step(g)
+        s = opt.state()
+        copies = {k: (v if k == "n" else [W.HIPTensor.from_numpy(t.numpy(), dtype=t.dtype) for t in v]) for k, v in s.items()}
+        q = [W.HIPTensor.from_numpy(t.numpy()) for t in p]
+        again = O.AdamW(q, state_bits=bits, resume=copies, **HYPER)
+        opt.step(g)
+        again.step(g)
+        for a, b in zip(p, q):
+            # b^t from the product carried along and from one power: apart by a few 2^-53
+            assert np.allclose(a.numpy(), b.numpy(), rtol=4 * U, atol=1e-12)
+
+
+@pytest.mark.gpu
+def test_what_is_not_finite_stays_where_it_is(gpu):
+    """A gradient that is infinite or not a number costs its own element, not the block that shares its scale."""
+    W = gpu
+    O = W.optimizers
+    for bits in (32, 8):
+        p0, g0, _, _ = numbers(600, 9, first=True)
+        # sizes within a factor of two: every code is a normal number, 2^-4 of its element at most
+        g0 = (np.sign(g0) * np.random.default_rng(2).uniform(0.5, 1.0, 600) * 1e-3).astype(f32)
+        bad = g0.copy()
+        bad[[3, 300]] = np.nan, np.inf
+        got = []
+        for grad in (g0, bad):
+            p, g = tensors(W, [p0, grad])
+            opt = O.AdamW([p], state_bits=bits, **HYPER)
+            opt.step([g])
+            opt.step([g])
+            got.append(p.numpy())
+        keep = np.setdiff1d(np.arange(600), [3, 300])
+        assert np.array_equal(got[0][keep], got[1][keep]) or bits == 8
+        # 8 bits: the block's largest may have been the element that is gone, which moves the others' codes.  The first
+        # step does not see codes; in the second m and r are each within 2^-4 of their unrounded values in both runs, and the step,
+        # their quotient times lr and at most about lr, within 4 2^-4 lr and what that leaves out
+        assert np.all(np.abs(got[0][keep] - got[1][keep]) <= HYPER["lr"] * (4 * 2.0 ** -4 * 1.2))
+        assert np.isfinite(got[1][keep]).all() and np.isnan(got[1][3])
+
+
+@pytest.mark.gpu
+def test_extreme_sizes(gpu):
+    """Zero gradients leave p to the decay; the smallest and largest numbers give no NaN."""
+    W = gpu
+    O = W.optimizers
+    for bits in (32, 8):
+        p0 = np.linspace(-1, 1, 520).astype(f32)
+        for g0 in (np.zeros(520, f32), np.full(520, 1e-38, f32), np.full(520, 1e-44, f32), np.full(520, 1e18, f32)):
+            p, g = tensors(W, [p0, g0])
+            opt = O.AdamW([p], state_bits=bits, weight_decay=0.0, **HYPER)
+            for _ in range(3):
+                opt.step([g])
+            assert np.isfinite(p.numpy()).all()
+            if not g0.any():
+                assert np.array_equal(p.numpy(), p0)
+            assert np.all(np.abs(p.numpy() - p0) <= 3 * HYPER["lr"] * 1.2)
+
+
+@pytest.mark.gpu
+def test_argument_checks(gpu):
+    W = gpu
+    O, lib = W.optimizers, W.lib
+    p, g = W.HIPTensor([64]), W.HIPTensor([64])
+    opt = O.AdamW([p])
+    for bad in (lambda: opt.step([]), lambda: opt.step([W.HIPTensor([63])]), lambda: opt.step([W.HIPTensor([64], dtype="double")]),
+                lambda: opt.step([W.HIPTensor([128]).view((0, 64))]), lambda: O.AdamW([W.HIPTensor([64], dtype="double")]),
+                lambda: O.AdamW([p], state_bits=16), lambda: O.AdamW([p], weight_decay=[0.1, 0.1]),
+                lambda: O.AdamW([p], resume=dict(n=1, m=[W.HIPTensor([63])], v=[W.HIPTensor([64])])),
+                lambda: O.AdamW([p], resume=dict(n=-1, m=[W.HIPTensor([64])], v=[W.HIPTensor([64])])),
+                lambda: O.AdamW([p], resume=dict(n=1, m=[], v=[W.HIPTensor([64])])),
+                lambda: O.AdamW([p], state_bits=8, resume=dict(n=1, m=[W.HIPTensor([64])], r=[W.HIPTensor([64])],
+                                                              m_scale=[W.HIPTensor([1])], r_scale=[W.HIPTensor([1])])),
+                lambda: O.AdamW([p], lr=W.HIPTensor([2])).step([g])):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(W.HIPError) as e:
+        O.AdamW([p, p]).step([g, W.HIPTensor([64])])       # a parameter twice
+    assert e.value.code == lib.EOVERLAP
+    with pytest.raises(W.HIPError) as e:
+        opt.step([p])                                      # a parameter as its gradient
+    assert e.value.code == lib.EOVERLAP
+    q = W.HIPTensor([64])
+    O.AdamW([p, q]).step([g, g])                           # one gradient for two parameters
+    step = lib.get().wf2hip_adamw_step
+    steps = W.HIPTensor.from_numpy(np.array([1.0, 1.0, 0, 0]), dtype="double")
+    m, v = W.HIPTensor([64]), W.HIPTensor([64])
+
+    def call(count=1, null=None, steps_ptr=C.c_void_p(steps.ptr), desc=True, **kw):
+        row = lib.AdamWTensor(param=p.ptr, grad=g.ptr, m=m.ptr, v=v.ptr, n=kw.pop("n", 64))
+        if null:
+            setattr(row, null, None)
+        d = lib.AdamWDesc(lr=1e-3, beta1=kw.pop("beta1", 0.9), beta2=0.95, eps=1e-8, state_bits=kw.pop("bits", 32))
+        return step(C.byref(d) if desc else None, count, C.byref(row), steps_ptr)
+
+    assert call() == 0 and call(n=0) == 0 and call(count=0) == 0
+    assert call(n=-1) == lib.EINVAL and call(count=-1) == lib.EINVAL and call(bits=16) == lib.EINVAL
+    assert call(beta1=1.0) == lib.EINVAL and call(beta1=-0.1) == lib.EINVAL and call(desc=False) == lib.EINVAL
+    assert call(bits=8) == lib.EINVAL and call(steps_ptr=None) == lib.EINVAL
+    for name in ("param", "grad", "m", "v"):
+        assert call(null=name) == lib.EINVAL
+    assert call(n=2 ** 32) == lib.EUNSUPPORTED
+    assert call(steps_ptr=C.c_void_p(m.ptr)) == lib.EOVERLAP
+    assert np.array_equal(steps.numpy()[2:], [1.0, 0.0])
