@@ -38,6 +38,265 @@ __global__ __launch_bounds__(kBlock) void embedding_add_kernel(const float* __re
   }
 }
 
+// The token of an id as the forward pass reads it.
+__device__ __forceinline__ int32_t token_of(float id, int32_t vocab) {
+  const float nearest = __builtin_rintf(id);
+  const int32_t t = (int32_t)fminf(fmaxf(nearest, 0.0f), 2147483520.0f);   // NaN -> 0
+  return nearest >= (float)vocab ? vocab - 1 : t;
+}
+
+// The gradient of the lookup, added into the tables' gradients:
+//   dwte[token(ctx[r])] += dout[r],   dwpe[p] += sum of dout over the rows of position p,
+// every sum in an order that the rows alone decide, without atomics, so that the same call gives the same bits.
+//
+// The token table's part: the tokens are dealt out to `classes` classes by their low bits, and a workgroup of sixteen
+// wavefronts owns a class, hence every element it adds to.  It reads all ids (they stay in L2), keeps the rows of its
+// class in LDS in their order, sorts them by token (stable) and deals the sorted list out in equal runs to its
+// wavefronts, 64 vectors of the columns to each: a wavefront reads its rows eight at a time and touches the table once per token,
+// however often that occurs; a token whose rows span several runs is put together from the wavefronts' parts in LDS.
+// (A text's most frequent word is a few per cent of it, a padded batch's padding most of it.)  The position table's part runs in
+// the same launch, a thread per vector.  Bound by HBM: dout once, and the rows of dwte it meets twice; short calls by
+// the length of the chain ids -> rows -> table.
+constexpr int kGradBlock = 1024, kGradWaves = kGradBlock / kWave;
+constexpr int kGatherStep = 4 * kGradBlock;   // ids that a workgroup looks at at a time
+constexpr int kGather = 2 * kGatherStep;      // rows of a class that LDS holds at a time
+constexpr int kGatherTurns = kGather / kGradBlock;
+constexpr int kRankMost = 256;                // longer lists are sorted bit by bit
+
+struct EmbeddingGradient {
+  const float *ctx, *dout;
+  float *dwte, *dwpe;
+  int64_t rows, seq, dim;
+  int32_t vocab;
+  uint32_t classes;       // a power of two
+  int token_bits;         // bits of a token above those of its class
+};
+
+struct GatherLds {
+  __attribute__((aligned(16))) int32_t row[kGather];
+  __attribute__((aligned(16))) int32_t token[kGather];
+  int32_t votes[kGatherTurns * kGradWaves];   // of a turn's wavefronts
+};
+
+// Stable sort of the first `count` entries by token.  Short lists: an entry's rank is the number of entries that go before
+// it.  Long ones: a pass per bit of the token above the class, zeros before ones.
+__device__ __forceinline__ void gather_sort(GatherLds& s, int count, uint32_t classes, int token_bits) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  if (count <= kRankMost) {
+    int rank = 0, row = 0, t = 0;
+    const int i = threadIdx.x;
+    if (i < count) {
+      t = s.token[i];
+      row = s.row[i];
+      int j = 0;
+#pragma unroll 4
+      for (; j + 3 < count; j += 4) {
+        const int4 u = *reinterpret_cast<const int4*>(s.token + j);
+        rank += (u.x < t || (u.x == t && j < i)) + (u.y < t || (u.y == t && j + 1 < i)) +
+                (u.z < t || (u.z == t && j + 2 < i)) + (u.w < t || (u.w == t && j + 3 < i));
+      }
+      for (; j < count; j++) rank += s.token[j] < t || (s.token[j] == t && j < i);
+    }
+    __syncthreads();
+    if (i < count) {
+      s.row[rank] = row;
+      s.token[rank] = t;
+    }
+    __syncthreads();
+    return;
+  }
+  const int turns = (count + kGradBlock - 1) / kGradBlock;
+  for (int bit = 0; bit < token_bits; bit++) {
+    const uint32_t mask = classes << bit;
+    int32_t row[kGatherTurns], t[kGatherTurns], before[kGatherTurns];
+#pragma unroll
+    for (int q = 0; q < kGatherTurns; q++) {
+      if (q >= turns) break;
+      const int i = q * kGradBlock + threadIdx.x;
+      t[q] = i < count ? s.token[i] : -1;   // behind the list: counted as ones, never written
+      row[q] = i < count ? s.row[i] : 0;
+      const uint64_t zeros = __ballot(i < count && !((uint32_t)t[q] & mask));
+      before[q] = __builtin_popcountll(zeros & ((1ull << lane) - 1));
+      if (lane == 0) s.votes[q * kGradWaves + wave] = __builtin_popcountll(zeros);
+    }
+    __syncthreads();
+    int sum = 0, ahead[kGatherTurns];
+#pragma unroll
+    for (int q = 0; q < kGatherTurns; q++) {
+      if (q >= turns) break;
+      // zeros of this turn's wavefronts before this one, and of the turns before
+      const int v = lane < kGradWaves ? s.votes[q * kGradWaves + lane] : 0;
+      int inclusive = v;
+#pragma unroll
+      for (int o = 1; o < kGradWaves; o <<= 1) {
+        const int other = __shfl_up(inclusive, o);
+        inclusive += lane >= o ? other : 0;
+      }
+      ahead[q] = sum + __builtin_amdgcn_readlane(inclusive, wave) - __builtin_amdgcn_readlane(v, wave);
+      sum += __builtin_amdgcn_readlane(inclusive, kGradWaves - 1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kGatherTurns; q++) {
+      if (q >= turns) break;
+      const int i = q * kGradBlock + threadIdx.x;
+      if (i < count) {
+        const int zeros = ahead[q] + before[q];
+        const int at = ((uint32_t)t[q] & mask) ? sum + i - zeros : zeros;
+        s.row[at] = row[q];
+        s.token[at] = t[q];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(kGradBlock) void embedding_gradient_kernel(EmbeddingGradient p) {
+  typedef float fv __attribute__((ext_vector_type(VEC ? 4 : 1)));
+  constexpr int V = VEC ? 4 : 1;
+  constexpr int kBatch = 8;
+  const int64_t per_row = p.dim / V;   // vectors of a row
+  if (blockIdx.x >= p.classes) {
+    // positions: vector i of dwpe's first seq rows
+    const int64_t i = (int64_t)(blockIdx.x - p.classes) * kGradBlock + threadIdx.x;
+    if (i >= p.seq * per_row) return;
+    const int64_t step = p.seq * p.dim;
+    const float* q = p.dout + i * V;
+    fv sum = *reinterpret_cast<const fv*>(q);
+#pragma unroll 4
+    for (int64_t n = step; n < p.rows * p.dim; n += step) sum += *reinterpret_cast<const fv*>(q + n);
+    fv* out = reinterpret_cast<fv*>(p.dwpe + i * V);
+    *out = *out + sum;
+    return;
+  }
+  __shared__ GatherLds s;
+  __shared__ fv part[kGradWaves][2][kWave];   // sums of tokens whose rows began before a wavefront's run, or go on behind it
+  const uint32_t mine = blockIdx.x;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  // the wavefronts: `across` of them side by side along the columns, `runs` runs of the list
+  const int64_t slices = (per_row + kWave - 1) / kWave;
+  const int across = slices < kGradWaves ? (int)slices : kGradWaves, runs = kGradWaves / across;
+  const int me = wave / across;   // this wavefront's run; runs and more: none
+  const uint64_t below = (1ull << lane) - 1;
+  // this thread's four ids of the step that begins at row `at`; fetched a step ahead
+  float ids[4];
+  auto fetch = [&](int64_t at) {
+    const int64_t r = at + threadIdx.x * 4;
+#pragma unroll
+    for (int k = 0; k < 4; k++) ids[k] = p.ctx[r + k < p.rows ? r + k : p.rows - 1];
+  };
+  int64_t next = 0;   // rows looked at so far
+  fetch(0);
+  while (next < p.rows) {
+    // keep rows of this class while another step's fit
+    int count = 0;
+    while (next < p.rows && count + kGatherStep <= kGather) {
+      const int64_t r = next + threadIdx.x * 4;
+      int32_t t[4];
+      bool hit[4];
+      int before = count, all = 0;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        t[k] = token_of(ids[k], p.vocab);
+        hit[k] = r + k < p.rows && ((uint32_t)t[k] & (p.classes - 1)) == mine;
+        const uint64_t votes = __ballot(hit[k]);
+        before += __builtin_popcountll(votes & below);
+        all += __builtin_popcountll(votes);
+      }
+      next += kGatherStep;
+      fetch(next);
+      if (lane == 0) s.votes[wave] = all;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kGradWaves; w++) {
+        const int v = s.votes[w];
+        if (w < wave) before += v;
+        count += v;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (hit[k]) {
+          s.row[before] = (int32_t)(r + k);
+          s.token[before] = t[k];
+          before++;
+        }
+      __syncthreads();
+    }
+    count = __builtin_amdgcn_readfirstlane(count);
+    if (count == 0) continue;
+    gather_sort(s, count, p.classes, p.token_bits);
+    const int run = (count + runs - 1) / runs;
+    auto first_of = [&](int w) { return w * run < count ? w * run : count; };
+    const int e0 = first_of(me), e1 = me < runs ? first_of(me + 1) : e0;
+    auto same = [&](int e) { return e > 0 && e < count && s.token[e] == s.token[e - 1]; };   // e belongs to the token before it
+    for (int64_t turn = 0; turn < slices; turn += across) {   // the same number of turns for every wavefront
+      const int64_t vec = (turn + wave % across) * kWave + lane;
+      const bool column = vec < per_row;
+      const int64_t c = (column ? vec : per_row - 1) * V;   // lanes behind the row read its last vector and write nothing
+      if (e0 < e1) {
+        bool lead = same(e0);   // the run's first token began before it
+        fv sum = {}, table = {};
+        int32_t of = 0;
+        // Eight rows, and the table's rows they go to, at a time: the loads carry no test (rows behind the run are its
+        // last one again), so that all of them are in flight before the first addition.
+        for (int e = e0; e < e1; e += kBatch) {
+          const int at = e + (lane & (kBatch - 1));
+          const int at8 = at < e1 ? at : e1 - 1;
+          const int32_t rows8 = s.row[at8], tokens8 = s.token[at8];
+          const uint64_t heads = __ballot(at < e1 && (at8 == e0 || s.token[at8 ? at8 - 1 : 0] != tokens8));
+          fv r[kBatch], t[kBatch];
+#pragma unroll
+          for (int u = 0; u < kBatch; u++) {
+            r[u] = *reinterpret_cast<const fv*>(p.dout + (int64_t)__builtin_amdgcn_readlane(rows8, u) * p.dim + c);
+            t[u] = *reinterpret_cast<const fv*>(p.dwte + (int64_t)__builtin_amdgcn_readlane(tokens8, u) * p.dim + c);
+          }
+#pragma unroll
+          for (int u = 0; u < kBatch; u++) {
+            if (e + u < e1) {
+              if ((heads >> u) & 1) {
+                if (e + u > e0) {   // the token before is complete, but for what came before the run
+                  if (lead)
+                    part[wave][0][lane] = sum;
+                  else if (column)
+                    *reinterpret_cast<fv*>(p.dwte + (int64_t)of * p.dim + c) = table + sum;
+                  lead = false;
+                }
+                sum = r[u];
+              } else {
+                sum += r[u];
+              }
+              of = __builtin_amdgcn_readlane(tokens8, u);
+              table = t[u];
+            }
+          }
+        }
+        if (lead)
+          part[wave][0][lane] = sum;
+        else if (same(e1))
+          part[wave][1][lane] = sum;
+        else if (column)
+          *reinterpret_cast<fv*>(p.dwte + (int64_t)of * p.dim + c) = table + sum;
+      }
+      __syncthreads();
+      // a token that began in this run and goes on behind it
+      if (e0 < e1 && column && same(e1) && !(same(e0) && s.token[e0] == s.token[e1 - 1])) {
+        const int32_t of = s.token[e1 - 1];
+        fv sum = part[wave][1][lane];
+        for (int w = me + 1; w < runs && same(first_of(w)); w++) {
+          sum += part[wave + (w - me) * across][0][lane];
+          if (s.token[first_of(w + 1) - 1] != of) break;   // it ends within run w
+        }
+        fv* out = reinterpret_cast<fv*>(p.dwte + (int64_t)of * p.dim + c);
+        *out = *out + sum;
+      }
+      __syncthreads();   // the parts are free
+    }
+    __syncthreads();   // the lists are free, and what this turn added is seen by the next one's threads
+  }
+}
+
 }  // namespace wf2
 
 using namespace wf2;
@@ -65,4 +324,39 @@ WF2_API int wf2hip_embedding_add_f32(long rows, long seq, long dim, const float*
   else
     embedding_add_kernel<false><<<(uint32_t)blocks, kBlock, 0, rt().stream>>>(ctx, wte, wpe, out, rows, seq, dim, vocab);
   return after_launch("embedding_add_kernel");
+}
+
+WF2_API int wf2hip_embedding_gradient_f32(long rows, long seq, long dim, const float* ctx, const float* dout, float* dwte,
+                                          long vocab, float* dwpe, long n_ctx) {
+  WF2_TRY(require_init());
+  const char* name = "embedding gradient";
+  if (rows < 0 || seq < 0 || dim < 0 || vocab < 0 || n_ctx < 0) return fail(WF2HIP_EINVAL, "%s: negative extent", name);
+  if (rows == 0 || dim == 0) return 0;
+  if (!ctx || !dout || !dwte || !dwpe) return fail(WF2HIP_EINVAL, "%s: null pointer", name);
+  if (seq < 1 || rows % seq != 0) return fail(WF2HIP_EINVAL, "%s: rows %ld is not a multiple of the sentence length %ld", name, rows, seq);
+  if (seq > n_ctx) return fail(WF2HIP_EINVAL, "%s: sentence length %ld beyond the %ld positions of dwpe", name, seq, n_ctx);
+  if (vocab < 1) return fail(WF2HIP_EINVAL, "%s: empty token table", name);
+  if (rows >= INT32_MAX - 2 * kGather || vocab >= ((int64_t)1 << 30) || dim > ((int64_t)1 << 28)) return fail(WF2HIP_EUNSUPPORTED, "%s: 2^31 rows, 2^30 words, or rows of more than 2^28 elements", name);
+  const struct {
+    const float* at;
+    int64_t n;
+  } in[2] = {{ctx, rows}, {dout, (int64_t)rows * dim}}, out[2] = {{dwte, (int64_t)vocab * dim}, {dwpe, (int64_t)n_ctx * dim}};
+  auto meet = [](auto& a, auto& b) { return a.at < b.at + b.n && b.at < a.at + a.n; };
+  for (auto& o : out)
+    for (auto& i : in)
+      if (meet(o, i)) return fail(WF2HIP_EOVERLAP, "%s: a table's gradient overlaps an input", name);
+  if (meet(out[0], out[1])) return fail(WF2HIP_EOVERLAP, "%s: the tables' gradients overlap", name);
+  const bool vec = dim % 4 == 0 && ((uintptr_t)dout | (uintptr_t)dwte | (uintptr_t)dwpe) % 16 == 0;
+  const int64_t per_row = vec ? dim / 4 : dim;
+  EmbeddingGradient p{ctx, dout, dwte, dwpe, rows, seq, dim, (int32_t)vocab, 1, 0};
+  // about sixteen rows to a class, at most a class per compute unit: every workgroup reads all the ids
+  while (p.classes < 256 && (int64_t)p.classes * 16 < rows) p.classes *= 2;
+  while (((int64_t)p.classes << p.token_bits) < vocab) p.token_bits++;
+  const int64_t positions = ceil_div((int64_t)seq * per_row, kGradBlock), blocks = (int64_t)p.classes + positions;
+  if (blocks >= ((int64_t)1 << 31)) return fail(WF2HIP_EUNSUPPORTED, "%s: too many elements for one launch", name);
+  if (vec)
+    embedding_gradient_kernel<true><<<(uint32_t)blocks, kGradBlock, 0, rt().stream>>>(p);
+  else
+    embedding_gradient_kernel<false><<<(uint32_t)blocks, kGradBlock, 0, rt().stream>>>(p);
+  return after_launch("embedding_gradient_kernel");
 }

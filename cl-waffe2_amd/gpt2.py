@@ -209,6 +209,14 @@ def positional_embedding(ctx: HIPTensor, wte: HIPTensor, wpe: HIPTensor) -> HIPT
     return nodes.forward("GPT2PositionalEmbedding", ctx, wte, wpe, out)
 
 
+def positional_embedding_backward(ctx: HIPTensor, dout: HIPTensor, dwte: HIPTensor, dwpe: HIPTensor):
+    """The gradient of :func:`positional_embedding`, added into the tables' gradients in one launch:
+    ``dwte[id] += dout``, ``dwpe[position] +=`` its sum over the sentences.  A token's rows are added up in
+    their order, so the result is the same in every run.  Returns ``(dwte, dwpe)``."""
+    from . import nodes
+    return nodes.forward("GPT2PositionalEmbedding-backward", F.to_contiguous(dout), F.to_contiguous(ctx), dwte, dwpe)
+
+
 def model_forward(tokens: HIPTensor, model: dict, cfg: dict = CONFIG, mode: str = "fused") -> HIPTensor:
     """The GPT2 model of the example (``examples/gpt-2/model.lisp:137-196``): positional embedding,
     the layers, the final LayerNorm and the language-model head ``x . wte^T`` (``lm-head``), with the

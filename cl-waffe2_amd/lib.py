@@ -218,6 +218,7 @@ _SIGNATURES = {
     "wf2hip_embedding_add_f32": ([_L, _L, _L, _P, _P, _L, _P, _L, _P], C.c_int),
     "wf2hip_linear_cross_entropy_f32": ([_L] * 3 + [_P] * 3 + [C.c_int] + [_P] * 2, C.c_int),
     "wf2hip_linear_cross_entropy_backward_f32": ([_L] * 3 + [_P] * 4 + [C.c_int, _P, _F] + [_P] * 2, C.c_int),
+    "wf2hip_embedding_gradient_f32": ([_L] * 3 + [_P] * 3 + [_L, _P, _L], C.c_int),
     "wf2hip_attention_f32": ([C.POINTER(AttentionDesc), _P, _P, _P, _P], C.c_int),
     "wf2hip_attention_forward_f32": ([C.POINTER(AttentionDesc), _P, _P, _P, _P, _P], C.c_int),
     "wf2hip_attention_backward_f32": ([C.POINTER(AttentionDesc)] + [_P] * 9, C.c_int),

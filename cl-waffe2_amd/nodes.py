@@ -44,7 +44,7 @@ NODE_NAMES = (
     "HIP-LayerNorm-Node-backward", "HIP-Attention-Node-backward", "HIP-Softmax-Cross-Entropy-Node-backward",
     "HIP-Linear-Cross-Entropy-Node-backward",
     # the node of the reference's GPT-2 example (examples/gpt-2/utils.lisp:68-72)
-    "GPT2PositionalEmbedding",
+    "GPT2PositionalEmbedding", "GPT2PositionalEmbedding-backward",
 )
 
 DEVICE_FEATURES: dict[type, dict[str, tuple]] = {}
@@ -784,3 +784,21 @@ def _gpt2_positional_embedding(ctx: HIPTensor, wte: HIPTensor, wpe: HIPTensor, o
     _lib.check(_lib.get().wf2hip_embedding_add_f32(n * t, t, dim, C.c_void_p(ctx.ptr), C.c_void_p(wte.ptr), vocab,
                                                   C.c_void_p(wpe.ptr), wpe.shape[0], C.c_void_p(out.ptr)))
     return out
+
+
+@define_impl("GPT2PositionalEmbedding-backward", HIPTensor, _only_float)
+def _gpt2_positional_embedding_backward(dout: HIPTensor, ctx: HIPTensor, dwte: HIPTensor, dwpe: HIPTensor):
+    """``dout[N sentence-length embedding-size] ctx[N sentence-length] dwte[vocab-size embedding-size]
+    dwpe[n-ctx embedding-size] -> dwte dwpe``: the node's gradient, added into those of its tables."""
+    name = "GPT2PositionalEmbedding-backward"
+    if len(ctx.shape) != 2 or len(dwte.shape) != 2 or len(dwpe.shape) != 2:
+        raise ValueError(f"{name}: ctx, dwte, dwpe must be matrices")
+    n, t = ctx.shape
+    vocab, dim = dwte.shape
+    _require_rows(f"{name}: ctx", ctx)
+    _require_rows(f"{name}: dout", dout, [n, t, dim])
+    _require_rows(f"{name}: dwte", dwte)
+    _require_rows(f"{name}: dwpe", dwpe, [dwpe.shape[0], dim])
+    _lib.check(_lib.get().wf2hip_embedding_gradient_f32(n * t, t, dim, C.c_void_p(ctx.ptr), C.c_void_p(dout.ptr),
+                                                       C.c_void_p(dwte.ptr), vocab, C.c_void_p(dwpe.ptr), dwpe.shape[0]))
+    return dwte, dwpe

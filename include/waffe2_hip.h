@@ -900,6 +900,13 @@ int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long vocab, co
  * seq <= n_ctx.  Bit-exact: one binary32 add per element. */
 int wf2hip_embedding_add_f32(long rows, long seq, long dim, const float* ctx, const float* wte,
                              long vocab, const float* wpe, long n_ctx, float* out);
+/* The gradient of that node, added into the gradients of its tables (the token table's other gradient is that of
+ * the lm-head, whose matrix it is): dwte[token(ctx[r]), :] += dout[r, :],
+ * dwpe[p, :] += sum of dout over the rows of position p < seq.  Ids are rounded and clamped as above.  A token's rows are
+ * added up in an order that the rows alone decide, without atomics: the same call gives the same bits.  One launch; fewer than
+ * 2^31 - 16384 rows and 2^30 words, dim at most 2^28; the tables' gradients overlap nothing else. */
+int wf2hip_embedding_gradient_f32(long rows, long seq, long dim, const float* ctx, const float* dout,
+                                  float* dwte, long vocab, float* dwpe, long n_ctx);
 
 #ifdef __cplusplus
 }
