@@ -13,8 +13,11 @@
 //             piece's rows of dw and its share of dx are formed.
 // All products run on the 16-bit matrix cores on pairs of binary16 numbers (wf2_pairs.h): they are what bounds the
 // operator beyond a few hundred rows.
+#include <stdlib.h>
+
 #include <utility>
 
+#include "wf2_direct.h"
 #include "wf2_pairs.h"
 #include "wf2_rows.h"
 
@@ -28,6 +31,11 @@ struct XentHead {
   int eg;          // the rows' gradients are held over 2^eg
   float weight;    // 1 / number of rows with a label (mean), 1 otherwise
   float alpha;     // what the rows' gradients have in common
+};
+
+// What the last kernel of a forward call counts its workgroups with; zeroed by the call's first kernel.
+struct XentSum {
+  unsigned int arrived;
 };
 
 constexpr int kLargestW = 1024, kLargestX = 256;   // workgroups (and partial maxima) of xent_largest
@@ -122,6 +130,7 @@ struct XentSplit {
   float scale;
   float* g;
   XentHead* head;
+  XentSum* total;         // PER_ROW
 };
 
 template <bool PER_ROW, bool VEC>
@@ -138,6 +147,7 @@ __global__ __launch_bounds__(kBlock) void xent_split(XentSplit p) {
   bool live = inside;
   int e;
   if (PER_ROW) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.total->arrived = 0u;
     float m = 0.0f;
     if (inside) {
       if (VEC) {
@@ -293,54 +303,77 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   }
 }
 
-// The tiles' maxima and sums of 64 rows of x: sixteen wavefronts take every sixteenth tile each and meet in LDS.
-constexpr int kFoldBlock = 1024;
-__global__ __launch_bounds__(kFoldBlock) void xent_fold(long rows, long vocab, uint32_t tiles, const float2* __restrict__ part,
-                                                        const float* __restrict__ at, const int32_t* __restrict__ labels,
-                                                        float* __restrict__ loss, float* __restrict__ lse) {
-  __shared__ float2 meet[kFoldBlock];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int64_t n = (int64_t)blockIdx.x * kWave + lane;
-  float top = -INFINITY, sum = 0.0f;
-  if (n < rows) {
-    for (uint32_t t = wave; t < tiles; t += kFoldBlock / kWave) {
-      const float2 a = part[(int64_t)t * rows + n];
-      const float both = fmaxf(top, a.x);
-      const float safe = both == -INFINITY ? 0.0f : both;
-      sum = sum * __builtin_amdgcn_exp2f((top - safe) * kLog2eF) + a.y * __builtin_amdgcn_exp2f((a.x - safe) * kLog2eF);
-      top = both;
-    }
-  }
-  meet[threadIdx.x] = float2{top, sum};
-  __syncthreads();
-  if (wave != 0 || n >= rows) return;
-  for (int i = 1; i < kFoldBlock / kWave; i++) {
-    const float2 a = meet[i * kWave + lane];
-    const float both = fmaxf(top, a.x);
-    const float safe = both == -INFINITY ? 0.0f : both;
-    sum = sum * __builtin_amdgcn_exp2f((top - safe) * kLog2eF) + a.y * __builtin_amdgcn_exp2f((a.x - safe) * kLog2eF);
-    top = both;
-  }
-  const float l = top + logf(sum);
-  const int32_t label = labels[n];
-  lse[n] = l;
-  loss[n] = label < 0 ? 0.0f : label >= vocab ? NAN : l - at[n];   // a label behind the vocabulary has no logit
+// Folds a maximum and a sum of exponentials into another.
+__device__ __forceinline__ void fold_in(float& top, float& sum, float2 a) {
+  const float both = fmaxf(top, a.x);
+  const float safe = both == -INFINITY ? 0.0f : both;
+  sum = sum * __builtin_amdgcn_exp2f((top - safe) * kLog2eF) + a.y * __builtin_amdgcn_exp2f((a.x - safe) * kLog2eF);
+  top = both;
 }
 
-// out[0] = sum of the losses (over the number of rows with a label)
-__global__ __launch_bounds__(kBlock) void xent_reduce(long rows, const float* __restrict__ loss,
-                                                      const int32_t* __restrict__ labels, bool mean,
-                                                      float* __restrict__ out) {
-  __shared__ double part[kWavesPerBlock];
-  double sum = 0.0, count = 0.0;
-  for (long i = threadIdx.x; i < rows; i += kBlock) {
-    sum += loss[i];
-    count += labels[i] >= 0;
+// The tiles' maxima and sums of a row.  MANY rows: 64 to a workgroup, a lane each, sixteen wavefronts taking every sixteenth
+// tile and meeting in LDS; few rows: a workgroup to each, a thread to every 256th tile (rows 61, 786 tiles: 20 -> FOLD us).
+// With a reduction the workgroup that arrives last adds up the workgroups' shares in their order.
+constexpr int kFoldRows = 2048;   // up to here a workgroup per row
+template <bool MANY>
+__global__ __launch_bounds__(MANY ? 1024 : kBlock) void xent_fold(
+    long rows, long vocab, uint32_t tiles, const float2* __restrict__ part, const float* __restrict__ at,
+    const int32_t* __restrict__ labels, int reduction, float* __restrict__ loss, float* __restrict__ lse,
+    XentSum* __restrict__ total, double* __restrict__ share) {
+  constexpr int kThreads = MANY ? 1024 : kBlock, kWaves = kThreads / kWave;
+  __shared__ float2 meet[MANY ? kThreads : kWaves];
+  __shared__ bool last;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int64_t n = MANY ? (int64_t)blockIdx.x * kWave + lane : blockIdx.x;
+  float top = -INFINITY, sum = 0.0f;
+  if (n < rows)
+    for (uint32_t t = MANY ? wave : threadIdx.x; t < tiles; t += MANY ? kWaves : kThreads)
+      fold_in(top, sum, part[(int64_t)t * rows + n]);
+  if (!MANY) {
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) fold_in(top, sum, float2{__shfl_xor(top, o), __shfl_xor(sum, o)});
   }
-  sum = block_sum(sum, part);
+  if (MANY)
+    meet[threadIdx.x] = float2{top, sum};
+  else if (lane == 0)
+    meet[wave] = float2{top, sum};
   __syncthreads();
-  count = block_sum(count, part);
-  if (threadIdx.x == 0) out[0] = (float)(mean ? sum / count : sum);
+  if (wave == 0) {
+    float each = 0.0f, held = 0.0f;
+    if (n < rows && (MANY || lane == 0)) {
+      top = -INFINITY;
+      sum = 0.0f;
+#pragma unroll 4
+      for (int i = 0; i < kWaves; i++) fold_in(top, sum, meet[MANY ? i * kWave + lane : i]);
+      const float l = top + logf(sum);
+      const int32_t label = labels[n];
+      lse[n] = l;
+      each = label < 0 ? 0.0f : label >= vocab ? NAN : l - at[n];   // a label behind the vocabulary has no logit
+      held = label < 0 ? 0.0f : 1.0f;
+      if (reduction == WF2HIP_REDUCE_NONE) loss[n] = each;
+    }
+    if (reduction != WF2HIP_REDUCE_NONE) {
+      const double s = wave_sum((double)each), c = wave_sum((double)held);
+      if (lane == 0) {
+        // past the caches, waited for, then the arrival: whoever sees all arrivals sees all shares
+        __hip_atomic_store(&share[2 * blockIdx.x], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&share[2 * blockIdx.x + 1], c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        last = __hip_atomic_fetch_add(&total->arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+      }
+    }
+  }
+  if (reduction == WF2HIP_REDUCE_NONE) return;
+  __syncthreads();
+  if (!last || wave != 0) return;
+  double s = 0.0, c = 0.0;
+  for (uint32_t i = lane; i < gridDim.x; i += kWave) {
+    s += __hip_atomic_load(&share[2 * i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    c += __hip_atomic_load(&share[2 * i + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  s = wave_sum(s);
+  c = wave_sum(c);
+  if (lane == 0) loss[0] = (float)(reduction == WF2HIP_REDUCE_MEAN ? s / c : s);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------
@@ -470,6 +503,302 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   }
 }
 
+// ---- straight from binary32: few rows, small products -----------------------------------------------------------
+
+struct XentDirect {
+  const float *x, *w;
+  const int32_t* labels;
+  long rows, dim, vocab;
+  uint32_t tiles_v, tiles_n;   // 128 or 32 words, 32 NB rows of x each
+  float2* part;                // forward, as XentLoss
+  float* at;
+  XentSum* total;
+  float *loss, *lse_out;
+  int reduction;
+  const float *lse, *dloss;    // backward
+  bool per_row, mean;
+  float scale;
+  float* ds;                   // (vocab, pitch)
+  int64_t pitch;
+  uint32_t tiles_dw;           // dw: columns of x
+  uint32_t tiles_dx, tiles_nx; // dx: columns, rows of x
+  uint32_t dw_units;           // workgroups of dw; those of dx follow
+  int64_t share;               // words of a share of dx's K
+  float *dx, *dw;              // dx: a plane per share
+};
+
+// A tile of 128 words x 32 NB rows of x.
+template <int NB>
+__global__ __launch_bounds__(kBlock) void xent_direct_loss(XentDirect p) {
+  __shared__ __attribute__((aligned(16))) char smem[kSkinnyLds<NB>];
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.total->arrived = 0u;
+  const uint32_t tn = blockIdx.x % p.tiles_n, tv = blockIdx.x / p.tiles_n;
+  const int64_t m0 = (int64_t)tv * kSkinnyRows, n0 = (int64_t)tn * 32 * NB;
+  f16v acc[NB];
+  skinny_product<NB, false>(DirectMatrix{p.w, p.dim, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.rows, nullptr}, m0, n0, p.dim,
+                            smem, acc);
+  lds_barrier();   // the stages are free
+  float2* fold = reinterpret_cast<float2*>(smem);   // [wavefront][row of x]
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < NB; j++) {
+    const int64_t n = n0 + j * 32 + (lane & 31);
+    const int64_t label = n < p.rows ? p.labels[n] : -1;
+    float top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int64_t v = m0 + wave * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
+      if (v == label) p.at[n] = acc[j][r];   // not read for a label behind the vocabulary
+      if (v >= p.vocab) acc[j][r] = -INFINITY;
+      top = fmaxf(top, acc[j][r]);
+    }
+    const float base = (top == -INFINITY ? 0.0f : top) * kLog2eF;
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; r++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][r], kLog2eF, -base));
+    fold_in(top, sum, float2{__shfl_xor(top, 32), __shfl_xor(sum, 32)});
+    if (h == 0) fold[wave * 32 * NB + j * 32 + lane] = float2{top, sum};
+  }
+  __syncthreads();
+  const int64_t n = n0 + threadIdx.x;
+  if (threadIdx.x < 32 * NB && n < p.rows) {
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWavesPerBlock; w++) fold_in(top, sum, fold[w * 32 * NB + threadIdx.x]);
+    p.part[(int64_t)tv * p.rows + n] = float2{top, sum};
+  }
+}
+
+// What multiplies a row's ds: the common factor and, in the mean, one over the number of rows with a label, which every
+// workgroup counts for itself.
+__device__ __forceinline__ float xent_weight(const XentDirect& p) {
+  if (!p.mean) return p.scale;
+  __shared__ double dpart[kWavesPerBlock];
+  double count = 0.0;
+  for (long r = threadIdx.x; r < p.rows; r += kBlock) count += p.labels[r] >= 0;
+  count = block_sum(count, dpart);
+  if (threadIdx.x == 0) dpart[0] = count;
+  __syncthreads();
+  return p.scale * (float)(1.0 / dpart[0]);
+}
+
+// ds of a tile of 128 words x 32 NB rows of x, everything the gradients have in common included; a word's rows run along
+// the storage.
+template <int NB>
+__global__ __launch_bounds__(kBlock) void xent_direct_ds(XentDirect p) {
+  __shared__ __attribute__((aligned(16))) char smem[kSkinnyLds<NB>];
+  const uint32_t tn = blockIdx.x % p.tiles_n, tv = blockIdx.x / p.tiles_n;
+  const int64_t m0 = (int64_t)tv * kSkinnyRows, n0 = (int64_t)tn * 32 * NB;
+  const float weight = xent_weight(p);
+  f16v acc[NB];
+  skinny_product<NB, false>(DirectMatrix{p.w, p.dim, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.rows, nullptr}, m0, n0, p.dim,
+                            smem, acc);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < NB; j++) {
+    const int64_t n = n0 + j * 32 + (lane & 31);
+    if (n < p.rows) {
+      const int32_t label = p.labels[n];
+      const float base = p.lse[n] * kLog2eF;
+      const float g = label >= p.vocab ? NAN : p.dloss ? weight * p.dloss[p.per_row ? n : 0] : weight;
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int64_t v = m0 + wave * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
+        float d = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[j][r], kLog2eF, -base));
+        if (v == label) d -= 1.0f;
+        if (v < p.vocab) p.ds[v * p.pitch + n] = label < 0 ? 0.0f : d * g;
+      }
+    }
+  }
+}
+
+// A tile of 32 words x 32 NB rows of x.  LAST: few enough tiles and rows for the workgroup that arrives last to finish the
+// call (loss, lse, the reduction), which saves a launch.  `arrived` is zero between calls.
+__device__ unsigned int g_xent_arrived;
+
+template <int NB, bool LAST>
+__global__ __launch_bounds__(kBlock) void xent_small_loss(XentDirect p) {
+  __shared__ __attribute__((aligned(16))) char smem[kSmallLds<NB>];
+  if (!LAST && blockIdx.x == 0 && threadIdx.x == 0) p.total->arrived = 0u;
+  const uint32_t tn = blockIdx.x % p.tiles_n, tv = blockIdx.x / p.tiles_n;
+  const int64_t m0 = (int64_t)tv * 32, n0 = (int64_t)tn * 32 * NB;
+  float s[NB][4];
+  small_product<NB, false, false>(DirectMatrix{p.w, p.dim, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.rows, nullptr}, m0, n0, 0,
+                                  p.dim, smem, s);
+  float2* fold = reinterpret_cast<float2*>(smem);   // [wavefront][row of x]
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < NB; j++) {
+    const int64_t n = n0 + j * 32 + (lane & 31);
+    const int64_t label = n < p.rows ? p.labels[n] : -1;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const int64_t v = m0 + wave * 8 + h * 4 + c;
+      if (v == label) {   // not read for a label behind the vocabulary
+        if (LAST)
+          __hip_atomic_store(&p.at[n], s[j][c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        else
+          p.at[n] = s[j][c];
+      }
+      if (v >= p.vocab) s[j][c] = -INFINITY;
+      top = fmaxf(top, s[j][c]);
+    }
+    const float base = (top == -INFINITY ? 0.0f : top) * kLog2eF;
+#pragma unroll
+    for (int c = 0; c < 4; c++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][c], kLog2eF, -base));
+    fold_in(top, sum, float2{__shfl_xor(top, 32), __shfl_xor(sum, 32)});
+    if (h == 0) fold[wave * 32 * NB + j * 32 + lane] = float2{top, sum};
+  }
+  __syncthreads();
+  const int64_t n = n0 + threadIdx.x;
+  if (threadIdx.x < 32 * NB && n < p.rows) {
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWavesPerBlock; w++) fold_in(top, sum, fold[w * 32 * NB + threadIdx.x]);
+    const int64_t at = (int64_t)tv * p.rows + n;
+    if (LAST)   // past the caches, for a workgroup that may sit anywhere
+      __hip_atomic_store(reinterpret_cast<unsigned long long*>(&p.part[at]),
+                         __builtin_bit_cast(unsigned long long, float2{top, sum}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else
+      p.part[at] = float2{top, sum};
+  }
+  if (!LAST) return;
+  __shared__ bool last;
+  __shared__ double dpart[kWavesPerBlock];
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // written before the arrival is counted
+  __syncthreads();
+  if (threadIdx.x == 0)
+    last = __hip_atomic_fetch_add(&g_xent_arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  if (threadIdx.x == 0) __hip_atomic_store(&g_xent_arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint32_t tiles = gridDim.x / p.tiles_n;
+  double total = 0.0, held = 0.0;
+  for (int64_t r = threadIdx.x; r < p.rows; r += kBlock) {
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 4
+    for (uint32_t t = 0; t < tiles; t++)
+      fold_in(top, sum, __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<unsigned long long*>(&p.part[(int64_t)t * p.rows + r]),
+                                                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)));
+    const float l = top + logf(sum);
+    const int32_t label = p.labels[r];
+    p.lse_out[r] = l;
+    const float each = label < 0 ? 0.0f : label >= p.vocab ? NAN
+                       : l - __hip_atomic_load(&p.at[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (p.reduction == WF2HIP_REDUCE_NONE) p.loss[r] = each;
+    total += each;
+    held += label >= 0;
+  }
+  if (p.reduction == WF2HIP_REDUCE_NONE) return;
+  total = block_sum(total, dpart);
+  __syncthreads();
+  held = block_sum(held, dpart);
+  if (threadIdx.x == 0) p.loss[0] = (float)(p.reduction == WF2HIP_REDUCE_MEAN ? total / held : total);
+}
+
+// ds of a tile of 32 words x 32 NB rows of x, as xent_direct_ds leaves it.
+template <int NB>
+__global__ __launch_bounds__(kBlock) void xent_small_ds(XentDirect p) {
+  __shared__ __attribute__((aligned(16))) char smem[kSmallLds<NB>];
+  const uint32_t tn = blockIdx.x % p.tiles_n, tv = blockIdx.x / p.tiles_n;
+  const int64_t m0 = (int64_t)tv * 32, n0 = (int64_t)tn * 32 * NB;
+  const float weight = xent_weight(p);
+  float s[NB][4];
+  small_product<NB, false, false>(DirectMatrix{p.w, p.dim, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.rows, nullptr}, m0, n0, 0,
+                                  p.dim, smem, s);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < NB; j++) {
+    const int64_t n = n0 + j * 32 + (lane & 31);
+    if (n < p.rows) {
+      const int32_t label = p.labels[n];
+      const float base = p.lse[n] * kLog2eF;
+      const float g = label >= p.vocab ? NAN : p.dloss ? weight * p.dloss[p.per_row ? n : 0] : weight;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const int64_t v = m0 + wave * 8 + h * 4 + c;
+        float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][c], kLog2eF, -base));
+        if (v == label) d -= 1.0f;
+        if (v < p.vocab) p.ds[v * p.pitch + n] = label < 0 ? 0.0f : d * g;
+      }
+    }
+  }
+}
+
+// Tiles of dw -- NBW 0: 32 words x 32 columns; otherwise 128 words x 32 NBW columns; K the rows of x -- and, behind them, of
+// dx (32 columns x 32 NBX rows of x, K a share of the words).
+template <int NBW, int NBX>
+__global__ __launch_bounds__(kBlock) void xent_direct_gradients(XentDirect p) {
+  constexpr int kLdsW = NBW ? kSkinnyLds<NBW> : kSmallLds<1>, kLdsX = kSmallLds<NBX>;
+  __shared__ __attribute__((aligned(16))) char smem[kLdsW > kLdsX ? kLdsW : kLdsX];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
+  if (blockIdx.x < p.dw_units) {
+    const uint32_t td = blockIdx.x % p.tiles_dw, tv = blockIdx.x / p.tiles_dw;
+    const DirectMatrix ds{p.ds, p.pitch, p.vocab, nullptr}, x{p.x, p.dim, p.dim, p.labels};
+    if constexpr (NBW == 0) {
+      const int64_t m0 = (int64_t)tv * 32, d = (int64_t)td * 32 + (lane & 31);
+      float s[1][4];
+      small_product<1, false, true>(ds, x, m0, (int64_t)td * 32, 0, p.rows, smem, s);
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const int64_t v = m0 + wave * 8 + h * 4 + c;
+        if (v < p.vocab && d < p.dim) p.dw[v * p.dim + d] = s[0][c];
+      }
+    } else {
+      const int64_t m0 = (int64_t)tv * kSkinnyRows, d0 = (int64_t)td * 32 * NBW;
+      f16v acc[NBW ? NBW : 1];
+      skinny_product<NBW ? NBW : 1, true>(ds, x, m0, d0, p.rows, smem, acc);
+#pragma unroll
+      for (int j = 0; j < NBW; j++) {
+        const int64_t d = d0 + j * 32 + (lane & 31);
+        if (d < p.dim) {
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const int64_t v = m0 + wave * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
+            if (v < p.vocab) p.dw[v * p.dim + d] = acc[j][r];
+          }
+        }
+      }
+    }
+    return;
+  }
+  const uint32_t unit = blockIdx.x - p.dw_units;
+  const uint32_t td = unit % p.tiles_dx, rest = unit / p.tiles_dx;
+  const uint32_t tn = rest % p.tiles_nx, share = rest / p.tiles_nx;
+  const int64_t d0 = (int64_t)td * 32, n0 = (int64_t)tn * 32 * NBX;
+  const int64_t k0 = share * p.share, k1 = k0 + p.share < p.vocab ? k0 + p.share : p.vocab;
+  float s[NBX][4];
+  small_product<NBX, true, true>(DirectMatrix{p.w, p.dim, p.dim, nullptr}, DirectMatrix{p.ds, p.pitch, p.rows, nullptr}, d0, n0, k0, k1,
+                                 smem, s);
+  float* out = p.dx + (int64_t)share * p.rows * p.dim;
+#pragma unroll
+  for (int j = 0; j < NBX; j++) {
+    const int64_t n = n0 + j * 32 + (lane & 31);
+    if (n < p.rows) {
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const int64_t d = d0 + wave * 8 + h * 4 + c;
+        if (d < p.dim) out[n * p.dim + d] = s[j][c];
+      }
+    }
+  }
+}
+
+// dx <- the planes' sum
+__global__ __launch_bounds__(kBlock) void xent_direct_fold(int64_t n, int planes, const float* __restrict__ part,
+                                                           float* __restrict__ dx) {
+  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+  if (i >= n) return;
+  float sum = part[i];
+#pragma unroll 8
+  for (int s = 1; s < planes; s++) sum += part[s * n + i];
+  dx[i] = sum;
+}
+
+// Tiles times rows up to which the last workgroup finishes a small call.
+constexpr int64_t kLastMost = 4096;
+
 // ---- host -----------------------------------------------------------------------------------------------------
 
 static bool meets(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -520,6 +849,91 @@ static int64_t xent_words(int64_t rows, int64_t vocab) {
   return ceil_div(tiles, pieces) * kTileM;
 }
 
+// Which route a call takes.
+//   kPairs    operands written as pairs first: many rows
+//   kSkinny   straight from binary32, tiles of 128 words: few rows against a long table
+//   kSmall    straight from binary32, tiles of 32 words with K shared out: where the others have too few tiles
+// WF2HIP_XENT_ROUTE=0 / 1 / 2 in the environment: always that one (as far as ds of the whole vocabulary fits its
+// workspace); for measurements and tests.
+enum XentRoute { kPairs, kSkinny, kSmall };
+static XentRoute xent_route(int64_t rows, int64_t dim, int64_t vocab, bool backward) {
+  const bool fits = !backward || ceil_div(rows, 32) * 32 * vocab <= ((int64_t)1 << 28);
+  if (!fits) return kPairs;
+  if (const char* env = getenv("WF2HIP_XENT_ROUTE"))
+    if (env[0] >= '0' && env[0] <= '2') return (XentRoute)(env[0] - '0');
+  if (rows > 256 && rows * dim * vocab > ((int64_t)1 << 30)) return kPairs;
+  return ceil_div(vocab, kSkinnyRows) * ceil_div(rows, 128) >= rt().num_cus ? kSkinny : kSmall;
+}
+
+// Width of a tile in blocks of 32: no wider than the operand, `most` where that is longer.
+static int xent_blocks(int64_t extent, int most) { return extent <= 32 ? 1 : extent <= 64 || most == 2 ? 2 : 4; }
+
+static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int64_t vocab, const float* x, const float* w,
+                                const int32_t* labels, const float* lse, int reduction, const float* dloss, float scale,
+                                float* dx, float* dw) {
+  hipStream_t st = rt().stream;
+  const bool small = route == kSmall;
+  const int nb = xent_blocks(rows, small ? 2 : 4), nbw = small ? 0 : xent_blocks(dim, 4), nbx = xent_blocks(rows, 2);
+  XentDirect p{};
+  p.x = x; p.w = w; p.labels = labels;
+  p.rows = rows; p.dim = dim; p.vocab = vocab;
+  p.tiles_v = (uint32_t)ceil_div(vocab, small ? 32 : kSkinnyRows);
+  p.tiles_n = (uint32_t)ceil_div(rows, 32 * nb);
+  p.tiles_dw = (uint32_t)ceil_div(dim, small ? 32 : 32 * nbw);
+  p.tiles_dx = (uint32_t)ceil_div(dim, 32);
+  p.tiles_nx = (uint32_t)ceil_div(rows, 32 * nbx);
+  p.lse = lse; p.dloss = dloss;
+  p.per_row = reduction == WF2HIP_REDUCE_NONE;
+  p.mean = reduction == WF2HIP_REDUCE_MEAN;
+  p.scale = scale;
+  p.pitch = ceil_div(rows, 32) * 32;
+  // shares of dx's K: enough workgroups to fill the device four times, of at least eight K steps
+  const int64_t dx_tiles = (int64_t)p.tiles_nx * p.tiles_dx, all_steps = ceil_div(vocab, kDirectStep);
+  int64_t shares = ceil_div(4 * rt().num_cus, dx_tiles);
+  if (shares > all_steps / 8) shares = all_steps / 8;
+  if (shares < 1) shares = 1;
+  p.share = ceil_div(all_steps, shares) * kDirectStep;
+  shares = ceil_div(vocab, p.share);
+  const int64_t dw_units = (int64_t)p.tiles_v * p.tiles_dw, most = ((int64_t)1 << 31) - 1;
+  if (dw_units + dx_tiles * shares > most || (int64_t)p.tiles_v * p.tiles_n > most)
+    return fail(WF2HIP_EUNSUPPORTED, "linear cross entropy backward: too many tiles for one launch");
+  p.dw_units = (uint32_t)dw_units;
+  Blocks blocks;
+  p.ds = blocks.take<float>(vocab * p.pitch * 4);
+  p.dx = shares > 1 ? blocks.take<float>(shares * rows * dim * 4) : dx;
+  p.dw = dw;
+  WF2_TRY(blocks.rc);
+  const uint32_t tiles = p.tiles_v * p.tiles_n, units = (uint32_t)(dw_units + dx_tiles * shares);
+  if (small)
+    nb == 1 ? xent_small_ds<1><<<tiles, kBlock, 0, st>>>(p) : xent_small_ds<2><<<tiles, kBlock, 0, st>>>(p);
+  else if (nb == 4)
+    xent_direct_ds<4><<<tiles, kBlock, 0, st>>>(p);
+  else
+    nb == 1 ? xent_direct_ds<1><<<tiles, kBlock, 0, st>>>(p) : xent_direct_ds<2><<<tiles, kBlock, 0, st>>>(p);
+  WF2_TRY(after_launch("xent ds"));
+  auto gradients = [&](auto wide, auto rows_wide) {
+    xent_direct_gradients<decltype(wide)::value, decltype(rows_wide)::value><<<units, kBlock, 0, st>>>(p);
+  };
+  auto with_rows = [&](auto wide) {
+    if (nbx == 1)
+      gradients(wide, std::integral_constant<int, 1>());
+    else
+      gradients(wide, std::integral_constant<int, 2>());
+  };
+  if (nbw == 0)
+    with_rows(std::integral_constant<int, 0>());
+  else if (nbw == 1)
+    with_rows(std::integral_constant<int, 1>());
+  else if (nbw == 2)
+    with_rows(std::integral_constant<int, 2>());
+  else
+    with_rows(std::integral_constant<int, 4>());
+  WF2_TRY(after_launch("xent_direct_gradients"));
+  if (shares == 1) return 0;
+  xent_direct_fold<<<(uint32_t)ceil_div(rows * dim, kBlock), kBlock, 0, st>>>(rows * dim, (int)shares, p.dx, dx);
+  return after_launch("xent_direct_fold");
+}
+
 template <bool PER_ROW>
 static int split_operands(const XentSplit& p, hipStream_t st) {
   const uint32_t blocks = p.wblocks + (uint32_t)ceil_div(p.rows, 32);
@@ -547,21 +961,47 @@ WF2_API int wf2hip_linear_cross_entropy_f32(long rows, long dim, long vocab, con
       return fail(WF2HIP_EOVERLAP, "%s: an output overlaps an input", name);
   if (meets(loss, losses, lse, rows)) return fail(WF2HIP_EOVERLAP, "%s: the loss overlaps the row statistics", name);
   hipStream_t st = rt().stream;
+  if (rows == 0) return each ? 0 : wf2hip_fill_f32(loss, 1, reduction == WF2HIP_REDUCE_MEAN ? NAN : 0.0f);
   Blocks blocks;
-  float* per_row = loss;
-  if (rows) {
+  const XentRoute route = xent_route(rows, dim, vocab, false);
+  const int nb = route == kPairs ? kTileN / 32 : xent_blocks(rows, route == kSmall ? 2 : 4);
+  static_assert(kTileM == kSkinnyRows, "one height of tiles on both routes");
+  const int64_t tiles_v = ceil_div(vocab, route == kSmall ? 32 : kTileM), tiles_n = ceil_div(rows, 32 * nb);
+  if (tiles_v * tiles_n >= ((int64_t)1 << 31)) return fail(WF2HIP_EUNSUPPORTED, "%s: too many tiles for one launch", name);
+  const uint32_t folds = (uint32_t)(rows <= kFoldRows ? rows : ceil_div(rows, kWave));
+  const bool one_launch = route == kSmall && tiles_v * rows <= kLastMost;
+  float2* part = blocks.take<float2>(tiles_v * rows * 8);
+  float* at = blocks.take<float>(rows * (int64_t)4);
+  XentSum* total = one_launch ? nullptr : blocks.take<XentSum>(sizeof(XentSum));
+  double* share = each || one_launch ? nullptr : blocks.take<double>(folds * (int64_t)16);
+  if (route != kPairs) {
+    WF2_TRY(blocks.rc);
+    XentDirect p{};
+    p.x = x; p.w = w; p.labels = labels;
+    p.rows = rows; p.dim = dim; p.vocab = vocab;
+    p.tiles_v = (uint32_t)tiles_v; p.tiles_n = (uint32_t)tiles_n;
+    p.part = part; p.at = at; p.total = total;
+    p.loss = loss; p.lse_out = lse; p.reduction = reduction;
+    const uint32_t tiles = (uint32_t)(tiles_v * tiles_n);
+    if (one_launch) {
+      nb == 1 ? xent_small_loss<1, true><<<tiles, kBlock, 0, st>>>(p) : xent_small_loss<2, true><<<tiles, kBlock, 0, st>>>(p);
+      return after_launch("xent_small_loss");
+    }
+    if (route == kSmall)
+      nb == 1 ? xent_small_loss<1, false><<<tiles, kBlock, 0, st>>>(p) : xent_small_loss<2, false><<<tiles, kBlock, 0, st>>>(p);
+    else if (nb == 4)
+      xent_direct_loss<4><<<tiles, kBlock, 0, st>>>(p);
+    else
+      nb == 1 ? xent_direct_loss<1><<<tiles, kBlock, 0, st>>>(p) : xent_direct_loss<2><<<tiles, kBlock, 0, st>>>(p);
+    WF2_TRY(after_launch("xent loss"));
+  } else {
     XentLoss p{};
     p.w = pair_matrix(nullptr, vocab, dim);
     p.x = pair_matrix(nullptr, rows, dim);
-    p.tiles_m = (uint32_t)ceil_div(vocab, kTileM);
-    p.tiles_n = (uint32_t)ceil_div(rows, kTileN);
-    if ((int64_t)p.tiles_m * p.tiles_n >= ((int64_t)1 << 31)) return fail(WF2HIP_EUNSUPPORTED, "%s: too many tiles for one launch", name);
+    p.tiles_m = (uint32_t)tiles_v; p.tiles_n = (uint32_t)tiles_n;
     p.w.base = blocks.take<char>(pair_bytes(p.w));
     p.x.base = blocks.take<char>(pair_bytes(p.x));
     int* exponent = blocks.take<int>((p.w.row_blocks + p.x.row_blocks) * (int64_t)32 * 4);
-    p.part = blocks.take<float2>((int64_t)p.tiles_m * rows * 8);
-    p.at = blocks.take<float>(rows * (int64_t)4);
-    if (!each) per_row = blocks.take<float>(rows * (int64_t)4);
     WF2_TRY(blocks.rc);
     XentSplit s{};
     s.x = x; s.w = w; s.labels = labels;
@@ -570,22 +1010,21 @@ WF2_API int wf2hip_linear_cross_entropy_f32(long rows, long dim, long vocab, con
     s.col_blocks = p.w.col_blocks;
     s.wblocks = (uint32_t)p.w.row_blocks;
     s.exponent = exponent;
+    s.total = total;
     WF2_TRY(split_operands<true>(s, st));
     p.exponent = exponent;
     p.x_exponents = (int64_t)p.w.row_blocks * 32;
     p.labels = labels;
-    p.rows = rows;
-    p.vocab = vocab;
+    p.rows = rows; p.vocab = vocab;
+    p.part = part; p.at = at;
     xent_tile_loss<<<p.tiles_m * p.tiles_n, kBlock, 0, st>>>(p);
     WF2_TRY(after_launch("xent_tile_loss"));
-    xent_fold<<<(uint32_t)ceil_div(rows, kWave), kFoldBlock, 0, st>>>(rows, vocab, p.tiles_m, p.part, p.at, labels, per_row, lse);
-    WF2_TRY(after_launch("xent_fold"));
   }
-  if (!each) {
-    xent_reduce<<<1, kBlock, 0, st>>>(rows, per_row, labels, reduction == WF2HIP_REDUCE_MEAN, loss);
-    WF2_TRY(after_launch("xent_reduce"));
-  }
-  return 0;
+  if (rows <= kFoldRows)
+    xent_fold<false><<<folds, kBlock, 0, st>>>(rows, vocab, (uint32_t)tiles_v, part, at, labels, reduction, loss, lse, total, share);
+  else
+    xent_fold<true><<<folds, 1024, 0, st>>>(rows, vocab, (uint32_t)tiles_v, part, at, labels, reduction, loss, lse, total, share);
+  return after_launch("xent_fold");
 }
 
 WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long vocab, const float* x, const float* w,
@@ -603,6 +1042,9 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
       return fail(WF2HIP_EOVERLAP, "%s: a gradient overlaps an input", name);
   if (meets(dx, nx, dw, nw)) return fail(WF2HIP_EOVERLAP, "%s: the gradients overlap", name);
   if (rows == 0) return wf2hip_fill_f32(dw, (size_t)nw, 0.0f);
+  const XentRoute route = xent_route(rows, dim, vocab, true);
+  if (route != kPairs)
+    return xent_backward_direct(route, rows, dim, vocab, x, w, labels, lse, reduction, dloss, scale, dx, dw);
   hipStream_t st = rt().stream;
   const int64_t words = xent_words(rows, vocab);
   const int64_t padded = ceil_div(rows, kTileN) * kTileN;

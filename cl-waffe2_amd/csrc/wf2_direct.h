@@ -1,0 +1,363 @@
+// wf2_direct.h -- binary32 matrix products on the 16-bit matrix cores, straight from binary32 storage.
+//
+// A binary32 number is three bfloat16 numbers: the 8 leading bits of its significand, the next 8, the last 8 (each part is
+// cut off, not rounded, so the rest is exact), with binary32's own range of exponents: no scale has to be known.  Of the
+// nine products of two such numbers the six largest are formed,
+//   a b = a1 b1 + a1 b2 + a2 b1 + a2 b2 + a1 b3 + a3 b1   (left out: at most 2^-22 |a b|),
+// on v_mfma_f32_32x32x16_bf16 with binary32 accumulators.  Twice the matrix instructions of the pairs of wf2_pairs.h, but
+// nothing is written before the product begins: for few rows against a long table, where the table's one read is the
+// time, and for products so small that launches are.
+#pragma once
+
+#include <type_traits>
+
+#include "wf2_common.h"
+
+namespace wf2 {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // unaligned 16-byte accesses are one instruction here
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+constexpr int kDirectStep = 32;                     // K goes by 32
+constexpr int kDirectPart = 32 * 16 * 2;            // bytes of one part of a 32 x 16 piece, in the order of the lanes
+constexpr int kDirectPiece = 3 * kDirectPart;
+constexpr int kDirectHalf = kDirectStep / 16 * kDirectPiece;   // 32 rows of an operand, a K step long
+
+// A barrier for LDS alone: loads from memory stay in flight (__syncthreads waits for them).
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// An operand: element (i, k) at base[i * ld + k] (k runs along the storage), or base[k * ld + i].
+struct DirectMatrix {
+  const float* base;
+  int64_t ld, rows;            // rows: extent of i
+  const int32_t* live;         // rows of the storage with live < 0 count as zeros (k along the rows only), or null
+};
+
+// Four consecutive k of row i (of 32), the g-th four of the step, as three parts into LDS: [part][k / 8 % 2][row][k % 8].
+__device__ __forceinline__ void put_parts(char* half, int i, int g, float a, float b, float c, float d) {
+  const float x[4] = {a, b, c, d};
+  uint32_t one[4], two[4], three[4];
+#pragma unroll
+  for (int n = 0; n < 4; n++) {
+    one[n] = __builtin_bit_cast(uint32_t, x[n]) & 0xffff0000u;
+    const float r = x[n] - __builtin_bit_cast(float, one[n]);
+    two[n] = __builtin_bit_cast(uint32_t, r) & 0xffff0000u;
+    three[n] = __builtin_bit_cast(uint32_t, r - __builtin_bit_cast(float, two[n]));
+  }
+  char* q = half + (g >> 2) * kDirectPiece + ((g >> 1) & 1) * 512 + i * 16 + (g & 1) * 8;
+  auto pack = [](uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); };   // upper halves
+  *reinterpret_cast<u2*>(q) = u2{pack(one[0], one[1]), pack(one[2], one[3])};
+  *reinterpret_cast<u2*>(q + kDirectPart) = u2{pack(two[0], two[1]), pack(two[2], two[3])};
+  *reinterpret_cast<u2*>(q + 2 * kDirectPart) = u2{pack(three[0], three[1]), pack(three[2], three[3])};
+}
+// ---- a long operand against a short one ----------------------------------------------------------------------
+//
+// A 128 x 32 NB tile of C[m][n] = sum_k A(m, k) B(n, k): a wavefront has 32 rows of A and all of the tile's columns.  No other
+// wavefront needs its rows, so they go from memory into the matrix instruction's operand registers (lane l: row l % 32,
+// k = 8 (l / 32) ... + 7 of 16) and are taken apart there, two steps ahead; only B's rows, which all four wavefronts read,
+// pass through LDS, taken apart once, a step ahead.  Vector instructions and matrix instructions share a SIMD's time
+// here, so what counts is how few of the former there are: per 32 x 32 x 32 products 88 / NB for A's parts and 22 for B's.
+constexpr int kSkinnyRows = 128;
+template <int NB>
+constexpr int kSkinnyLds = 2 * NB * kDirectHalf;
+
+__device__ __forceinline__ void three_parts(const float (&x)[8], b8 (&out)[3]) {
+  uint32_t one[8], two[8], three[8];
+#pragma unroll
+  for (int n = 0; n < 8; n++) {
+    one[n] = __builtin_bit_cast(uint32_t, x[n]) & 0xffff0000u;
+    const float r = x[n] - __builtin_bit_cast(float, one[n]);
+    two[n] = __builtin_bit_cast(uint32_t, r) & 0xffff0000u;
+    three[n] = __builtin_bit_cast(uint32_t, r - __builtin_bit_cast(float, two[n]));
+  }
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  auto pack = [](const uint32_t(&a)[8]) {
+    u4 v;
+#pragma unroll
+    for (int n = 0; n < 4; n++) v[n] = __builtin_amdgcn_perm(a[2 * n + 1], a[2 * n], 0x07060302u);
+    return __builtin_bit_cast(b8, v);
+  };
+  out[0] = pack(one);
+  out[1] = pack(two);
+  out[2] = pack(three);
+}
+
+template <int NB, bool BT>
+__device__ __forceinline__ void skinny_product(const DirectMatrix& A, const DirectMatrix& B, int64_t m0, int64_t n0, int64_t K,
+                                               char* smem, f16v (&acc)[NB]) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  // A: this lane's row
+  int64_t i = m0 + wave * 32 + (lane & 31);
+  i = i < A.rows ? i : A.rows - 1;   // rows behind the matrix feed outputs nobody keeps
+  const float* a = A.base + i * A.ld + (lane >> 5) * 8;
+  // B: this thread's units.  K contiguous: four k of NB rows; otherwise four rows of the operand at four k, the first 64 NB
+  // threads.
+  constexpr int kUnits = BT ? 4 : NB;
+  const int q = threadIdx.x;
+  const bool busy = !BT || q < 64 * NB;
+  const int bk = BT ? q / (8 * NB) * 4 : (q & 7) * 4;            // first of its four k
+  const int bi = BT ? q % (8 * NB) * 4 : q >> 3;                 // first row (of the tile)
+  const float* b[kUnits];
+  int inside = 4;                                                // BT: how many of the four rows lie inside
+#pragma unroll
+  for (int u = 0; u < kUnits; u++) {
+    if (BT) {
+      const int64_t n = n0 + bi;
+      inside = n + 4 <= B.rows ? 4 : n < B.rows ? (int)(B.rows - n) : 0;
+      b[u] = B.base + (int64_t)(busy ? bk + u : 0) * B.ld + (inside ? n : 0);
+    } else {
+      int64_t n = n0 + bi + u * 32;
+      n = n < B.rows ? n : B.rows - 1;
+      b[u] = B.base + n * B.ld + bk;
+    }
+  }
+  const int64_t bstep = BT ? kDirectStep * B.ld : kDirectStep;
+  const int32_t* live = BT && B.live ? B.live + bk : nullptr;
+  const bool columns = !BT || n0 + 32 * NB <= B.rows;            // uniform
+  f4 av[2][4], bv[kUnits];
+  auto fetch_a = [&](auto set, auto whole, int64_t left) {
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int k = (u >> 1) * 16 + (u & 1) * 4;
+      if constexpr (decltype(whole)::value) {
+        av[decltype(set)::value][u] = *reinterpret_cast<const f4u*>(a + k);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++) av[decltype(set)::value][u][c] = k + c + (lane >> 5) * 8 < left ? a[k + c] : 0.0f;
+      }
+    }
+    a += kDirectStep;
+  };
+  auto fetch_b = [&](auto whole, int64_t left) {
+    if (!busy) return;
+#pragma unroll
+    for (int u = 0; u < kUnits; u++) {
+      if constexpr (decltype(whole)::value) {
+        bv[u] = *reinterpret_cast<const f4u*>(b[u]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++) bv[u][c] = (BT ? bk + u < left && c < inside : bk + c < left) ? b[u][c] : 0.0f;
+      }
+      b[u] += bstep;
+    }
+    if (BT && live) {
+#pragma unroll
+      for (int u = 0; u < kUnits; u++)
+        if (bk + u < left && live[u] < 0) bv[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      live += kDirectStep;
+    }
+  };
+  auto store_b = [&](int buffer) {
+    if (!busy) return;
+    char* at = smem + buffer * NB * kDirectHalf;
+    if (BT) {
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        put_parts(at + (bi >> 5) * kDirectHalf, (bi & 31) + c, bk >> 2, bv[0][c], bv[BT ? 1 : 0][c], bv[BT ? 2 : 0][c], bv[BT ? 3 : 0][c]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnits; u++)
+        put_parts(at + u * kDirectHalf, bi, bk >> 2, bv[u][0], bv[u][1], bv[u][2], bv[u][3]);
+    }
+  };
+  auto products = [&](auto set, int buffer) {
+    const char* at = smem + buffer * NB * kDirectHalf + lane * 16;
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      float x[8];
+#pragma unroll
+      for (int c = 0; c < 8; c++) x[c] = av[decltype(set)::value][s * 2 + (c >> 2)][c & 3];
+      b8 p[3];
+      three_parts(x, p);
+#pragma unroll
+      for (int j = 0; j < NB; j++) {
+        b8 y[3];
+#pragma unroll
+        for (int t = 0; t < 3; t++) y[t] = *reinterpret_cast<const b8*>(at + j * kDirectHalf + s * kDirectPiece + t * kDirectPart);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[2], y[0], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[0], y[2], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[1], y[1], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[1], y[0], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[0], y[1], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[0], y[0], acc[j], 0, 0, 0);
+      }
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < NB; j++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[j][r] = 0.0f;
+  const int steps = (int)((K + kDirectStep - 1) / kDirectStep), full = (int)(K / kDirectStep);
+  const std::integral_constant<int, 0> even;
+  const std::integral_constant<int, 1> odd;
+  const std::true_type all;
+  const std::false_type some;
+  auto left = [&](int s) { return K - (int64_t)s * kDirectStep; };
+  fetch_b(some, K);
+  fetch_a(even, some, K);
+  if (steps > 1) fetch_a(odd, some, left(1));
+  store_b(0);
+  if (steps > 1) fetch_b(some, left(1));
+  lds_barrier();
+  int s = 0;
+  // B's step s is in buffer s % 2, A's steps s and s + 1 and B's step s + 1 are in registers or on their way
+  for (; s + 3 < (columns ? full : 0); s += 2) {
+    products(even, 0);
+    fetch_a(even, all, 0);
+    store_b(1);
+    fetch_b(all, left(s + 2));
+    lds_barrier();
+    products(odd, 1);
+    fetch_a(odd, all, 0);
+    store_b(0);
+    fetch_b(all, left(s + 3));
+    lds_barrier();
+  }
+  for (; s < steps; s += 2) {
+    products(even, 0);
+    if (s + 1 == steps) break;
+    if (s + 2 < steps) fetch_a(even, some, left(s + 2));
+    store_b(1);
+    if (s + 2 < steps) fetch_b(some, left(s + 2));
+    lds_barrier();
+    products(odd, 1);
+    if (s + 2 == steps) break;
+    if (s + 3 < steps) fetch_a(odd, some, left(s + 3));
+    store_b(0);
+    if (s + 3 < steps) fetch_b(some, left(s + 3));
+    lds_barrier();
+  }
+}
+
+// ---- both operands small ---------------------------------------------------------------------------------------
+//
+// A 32 x 32 NB tile: the four wavefronts of a workgroup share out K -- step s goes to wavefront s % 4 -- and bring their
+// operands from memory straight into operand registers: no LDS and no barrier until the four sums meet at the end.  As
+// many workgroups as the outputs allow and a quarter of the steps: what counts for small products is the length of the chain
+// of loads.  AT / BT: element (i, k) at base[k * ld + i].  After the meeting wavefront w has the rows 8 w + 4 h + 0 ... 3
+// of every 32 x 32 block (h = lane / 32), lane l the column l % 32.
+template <int NB>
+constexpr int kSmallLds = 4 * NB * 16 * kWave * 4;
+
+template <bool T>
+struct SmallStream {
+  const float* at;
+  int64_t ld;
+  const int32_t* live;
+  bool inside;         // T: this lane's row exists
+
+  __device__ __forceinline__ void start(const DirectMatrix& m, int64_t i, int64_t k0, int lane) {
+    inside = i < m.rows;
+    i = inside ? i : m.rows - 1;
+    k0 += (lane >> 5) * 8;
+    ld = m.ld;
+    at = T ? m.base + k0 * ld + i : m.base + i * ld + k0;
+    live = T && m.live ? m.live + k0 : nullptr;
+  }
+  // this lane's 16 numbers of the step that begins `skip` behind the start; `left`: how much of K is left there
+  __device__ __forceinline__ void fetch(int64_t skip, int64_t left, int lane, float (&v)[16]) const {
+    const int64_t mine = left - (lane >> 5) * 8;
+    const float* q = at + (T ? skip * ld : skip);
+    if (left >= kDirectStep) {
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int k = (u >> 1) * 16 + (u & 1) * 4;
+        if (T) {
+#pragma unroll
+          for (int c = 0; c < 4; c++) v[u * 4 + c] = q[(k + c) * ld];
+        } else {
+          const f4 x = *reinterpret_cast<const f4u*>(q + k);
+#pragma unroll
+          for (int c = 0; c < 4; c++) v[u * 4 + c] = x[c];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 16; n++) {
+        const int k = (n >> 3) * 16 + (n & 7);
+        v[n] = k < mine ? q[T ? k * ld : k] : 0.0f;
+      }
+    }
+    if (T && live) {
+#pragma unroll
+      for (int n = 0; n < 16; n++) {
+        const int k = (n >> 3) * 16 + (n & 7);
+        if (k < mine && live[skip + k] < 0) v[n] = 0.0f;
+      }
+    }
+  }
+};
+
+template <int NB, bool AT, bool BT>
+__device__ __forceinline__ void small_product(const DirectMatrix& A, const DirectMatrix& B, int64_t m0, int64_t n0, int64_t k0,
+                                              int64_t k1, char* smem, float (&out)[NB][4]) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  SmallStream<AT> a;
+  SmallStream<BT> b[NB];
+  a.start(A, m0 + (lane & 31), k0, lane);
+#pragma unroll
+  for (int j = 0; j < NB; j++) b[j].start(B, n0 + j * 32 + (lane & 31), k0, lane);
+  f16v acc[NB];
+#pragma unroll
+  for (int j = 0; j < NB; j++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[j][r] = 0.0f;
+  float av[16], bv[NB][16];
+  auto fetch = [&](int64_t skip) {
+    const int64_t left = k1 - k0 - skip;
+    if (left <= 0) return;
+    a.fetch(skip, left, lane, av);
+#pragma unroll
+    for (int j = 0; j < NB; j++) b[j].fetch(skip, left, lane, bv[j]);
+  };
+  fetch((int64_t)wave * kDirectStep);
+  for (int64_t skip = (int64_t)wave * kDirectStep; skip < k1 - k0; skip += 4 * kDirectStep) {
+    b8 x[2][3], y[NB][2][3];
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      three_parts(reinterpret_cast<const float(&)[8]>(av[s * 8]), x[s]);
+#pragma unroll
+      for (int j = 0; j < NB; j++) three_parts(reinterpret_cast<const float(&)[8]>(bv[j][s * 8]), y[j][s]);
+    }
+    fetch(skip + 4 * kDirectStep);
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int j = 0; j < NB; j++) {
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[s][2], y[j][s][0], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[s][0], y[j][s][2], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[s][1], y[j][s][1], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[s][1], y[j][s][0], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[s][0], y[j][s][1], acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[s][0], y[j][s][0], acc[j], 0, 0, 0);
+      }
+  }
+  // [wavefront][block][four registers][lane][4]
+  f4* meet = reinterpret_cast<f4*>(smem);
+#pragma unroll
+  for (int j = 0; j < NB; j++)
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+      meet[((wave * NB + j) * 4 + q) * kWave + lane] = f4{acc[j][q * 4], acc[j][q * 4 + 1], acc[j][q * 4 + 2], acc[j][q * 4 + 3]};
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < NB; j++) {
+    f4 sum = meet[(j * 4 + wave) * kWave + lane];
+#pragma unroll
+    for (int w = 1; w < 4; w++) sum += meet[((w * NB + j) * 4 + wave) * kWave + lane];
+#pragma unroll
+    for (int c = 0; c < 4; c++) out[j][c] = sum[c];
+  }
+  __syncthreads();   // LDS is free
+}
+
+}  // namespace wf2

@@ -131,7 +131,9 @@ def test_truth_gradients_by_differences():
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,dim,vocab", SHAPES)
 @pytest.mark.parametrize("reduction", ["mean", None])
-def test_against_float64(gpu, rows, dim, vocab, reduction):
+@pytest.mark.parametrize("route", ["0", "1", "2"])
+def test_against_float64(gpu, rows, dim, vocab, reduction, route, monkeypatch):
+    monkeypatch.setenv("WF2HIP_XENT_ROUTE", route)
     x, w, labels = inputs(rows, dim, vocab, left_out=0.2 if rows > 2 else 0.0)
     dy = np.random.default_rng(rows).uniform(0.1, 2.0, rows).astype(f32) if reduction is None else None
     check(gpu, x, w, labels, reduction, dy)
@@ -152,10 +154,12 @@ def test_sum_and_upstream_number(gpu):
         assert np.array_equal(p.numpy(), q.numpy())
 
 
+@pytest.mark.parametrize("route", ["0", "1", "2"])
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,dim,vocab", [(40, 64, 300), (300, 130, 1111)])
-def test_rows_left_out_hold_anything(gpu, rows, dim, vocab):
+def test_rows_left_out_hold_anything(gpu, rows, dim, vocab, route, monkeypatch):
     """NaN, infinities and the largest numbers in rows without a label change nothing elsewhere."""
+    monkeypatch.setenv("WF2HIP_XENT_ROUTE", route)
     W = gpu
     x, w, labels = inputs(rows, dim, vocab, left_out=0.3)
     clean = check(W, x, w, labels, "mean")
@@ -172,8 +176,10 @@ def test_rows_left_out_hold_anything(gpu, rows, dim, vocab):
         assert np.array_equal(a.numpy(), b.numpy())
 
 
+@pytest.mark.parametrize("route", ["0", "1", "2"])
 @pytest.mark.gpu
-def test_all_rows_left_out_and_no_rows(gpu):
+def test_all_rows_left_out_and_no_rows(gpu, route, monkeypatch):
+    monkeypatch.setenv("WF2HIP_XENT_ROUTE", route)
     W = gpu
     F, nn = W.functional, W.nn
     x, w, _ = inputs(9, 20, 50)
@@ -191,8 +197,10 @@ def test_all_rows_left_out_and_no_rows(gpu):
         assert not dw.numpy().any() and dx.shape == [0, 20]
 
 
+@pytest.mark.parametrize("route", ["0", "1", "2"])
 @pytest.mark.gpu
-def test_label_behind_the_vocabulary_is_nan(gpu):
+def test_label_behind_the_vocabulary_is_nan(gpu, route, monkeypatch):
+    monkeypatch.setenv("WF2HIP_XENT_ROUTE", route)
     W = gpu
     F, nn = W.functional, W.nn
     x, w, labels = inputs(40, 24, 100)
@@ -215,9 +223,11 @@ def test_sizes_of_numbers(gpu, scale_x, scale_w):
     check(gpu, (x * scale_x).astype(f32), (w * scale_w).astype(f32), labels, "mean")
 
 
+@pytest.mark.parametrize("route", ["0", "1", "2"])
 @pytest.mark.gpu
-def test_confident_and_spread_rows(gpu):
+def test_confident_and_spread_rows(gpu, route, monkeypatch):
     """Logits far apart: probabilities that underflow, losses near zero and very large ones."""
+    monkeypatch.setenv("WF2HIP_XENT_ROUTE", route)
     x, w, labels = inputs(60, 32, 400, sharp=1.0)
     x[:20] *= 30
     x[20:30] = 0
