@@ -213,8 +213,7 @@ def positional_embedding_backward(ctx: HIPTensor, dout: HIPTensor, dwte: HIPTens
     """The gradient of :func:`positional_embedding`, added into the tables' gradients in one launch:
     ``dwte[id] += dout``, ``dwpe[position] +=`` its sum over the sentences.  A token's rows are added up in
     their order, so the result is the same in every run.  Returns ``(dwte, dwpe)``."""
-    from . import nodes
-    return nodes.forward("GPT2PositionalEmbedding-backward", F.to_contiguous(dout), F.to_contiguous(ctx), dwte, dwpe)
+    return F.nodes.forward("GPT2PositionalEmbedding-backward", F.to_contiguous(dout), F.to_contiguous(ctx), dwte, dwpe)
 
 
 def model_forward(tokens: HIPTensor, model: dict, cfg: dict = CONFIG, mode: str = "fused") -> HIPTensor:

@@ -184,10 +184,9 @@ def linear_cross_entropy(x: HIPTensor, w: HIPTensor, labels: HIPTensor, reductio
     id leaves its position out (loss 0, no gradient).  ``reduction``: None (one loss per position), 'sum' or
     'mean' (over the positions that count).  Returns ``(loss, lse)``; ``lse``, one number per position, is what
     :func:`linear_cross_entropy_backward` needs.  Given ``loss`` / ``lse`` tensors are written."""
-    x2, labels1 = F.reshape(x, -1, x.shape[-1]), F.reshape(labels, -1)
-    rows = x2.shape[0]
+    x2, labels1 = _matrix(x), _run(labels)
     if lse is None:
-        lse = HIPTensor([rows], initial_element=None)
+        lse = HIPTensor([labels1.size], initial_element=None)
     if loss is None:
         loss = HIPTensor(list(labels.shape) if reduction is None else [1], initial_element=None)
     nodes.forward("HIP-Linear-Cross-Entropy-Node", x2, F.to_contiguous(w), labels1, _as_rows(loss, "loss"),
@@ -200,17 +199,27 @@ def linear_cross_entropy_backward(dy, x: HIPTensor, w: HIPTensor, labels: HIPTen
                                   dw: HIPTensor | None = None):
     """``(dx, dw)`` of :func:`linear_cross_entropy` from its inputs and its ``lse``.  ``dy``: the gradient of the
     loss, a tensor of the loss's shape or a number.  Given ``dx`` / ``dw`` tensors are overwritten."""
-    x2, labels1 = F.reshape(x, -1, x.shape[-1]), F.reshape(labels, -1)
+    x2, labels1 = _matrix(x), _run(labels)
     if dx is None:
         dx = HIPTensor(list(x.shape), initial_element=None)
     if dw is None:
         dw = HIPTensor(list(w.shape), initial_element=None)
-    if not dx.is_contiguous() or list(dx.shape) != list(x.shape):
+    if not dx.is_contiguous() or dx.shape != x.shape:
         raise ValueError(f"linear_cross_entropy_backward: dx must be a contiguous tensor of shape {x.shape}")
-    dout = F.reshape(dy, -1) if isinstance(dy, HIPTensor) else None
+    dout = _run(dy) if isinstance(dy, HIPTensor) else None
     nodes.forward("HIP-Linear-Cross-Entropy-Node-backward", x2, F.to_contiguous(w), labels1, _as_rows(lse, "lse"), dout,
-                  HIPTensor(list(x2.shape), vec=dx.vec), dw, reduction, 1.0 if dout is not None else float(dy))
+                  _matrix(dx), dw, reduction, 1.0 if dout is not None else float(dy))
     return dx, dw
+
+
+def _matrix(x: HIPTensor) -> HIPTensor:
+    """x[~ dim] as a contiguous matrix; x itself where it is one."""
+    return x if x.ndim == 2 and x.is_contiguous() else F.reshape(x, -1, x.shape[-1])
+
+
+def _run(x: HIPTensor) -> HIPTensor:
+    """x as one contiguous axis; x itself where it is one."""
+    return x if x.ndim == 1 and x.is_contiguous() else F.reshape(x, -1)
 
 
 def _as_rows(t: HIPTensor, what: str) -> HIPTensor:

@@ -621,21 +621,28 @@ def _softmax_cross_entropy_backward_node(dout: HIPTensor, z: HIPTensor, labels: 
 _REDUCTIONS = {None: _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
 
 
-def _require_labels(name: str, x: HIPTensor, w: HIPTensor, labels: HIPTensor, lse: HIPTensor, reduction) -> int:
-    """Checks what both directions of HIP-Linear-Cross-Entropy-Node read; returns the number of rows."""
+def _check(name: str, what: str, t: HIPTensor, shape: tuple) -> None:
+    """_require_rows with its questions asked in the order that costs an ordinary call least."""
+    if t.dtype != "float" or not t.is_contiguous() or t._geom()[0] != shape:
+        _require_rows(f"{name}: {what}", t, shape)
+
+
+def _require_labels(name: str, x: HIPTensor, w: HIPTensor, labels: HIPTensor, lse: HIPTensor, reduction):
+    """Checks what both directions of HIP-Linear-Cross-Entropy-Node read; returns (rows, dim, vocab)."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"{name}: reduction must be None, 'sum' or 'mean', got {reduction!r}")
-    if len(x.shape) != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1]:
+    sx, sw = x._geom()[0], w._geom()[0]
+    if len(sx) != 2 or len(sw) != 2 or sx[1] != sw[1]:
         raise ValueError(f"{name}: x[rows dim] and w[vocab dim] expected, got {x.shape} and {w.shape}")
-    rows = x.shape[0]
-    _require_rows(f"{name}: x", x)
-    _require_rows(f"{name}: w", w)
-    _require_rows(f"{name}: lse", lse, [rows])
+    rows, dim = sx
+    _check(name, "x", x, sx)
+    _check(name, "w", w, sw)
+    _check(name, "lse", lse, (rows,))
     if labels.dtype != "int32":
         raise ValueError(f"{name}: labels must be :int32 token ids, got :{labels.dtype}")
-    if not labels.is_contiguous() or list(labels.shape) != [rows]:
+    if not labels.is_contiguous() or labels._geom()[0] != (rows,):
         raise ValueError(f"{name}: labels must be {rows} contiguous token ids, got shape {labels.shape}")
-    return rows
+    return rows, dim, sw[0]
 
 
 @define_impl("HIP-Linear-Cross-Entropy-Node", HIPTensor, _only_float)
@@ -644,12 +651,10 @@ def _linear_cross_entropy_node(x: HIPTensor, w: HIPTensor, labels: HIPTensor, lo
     """``X[rows dim] W[vocab dim] Labels[rows] LOSS LSE[rows] -> LOSS``: softmax cross entropy of the logits
     x . w^T against token ids, without the logits.  LOSS has one element per row (reduction None) or one."""
     name = "HIP-Linear-Cross-Entropy-Node"
-    rows = _require_labels(name, x, w, labels, lse, reduction)
-    _require_rows(f"{name}: loss", loss, [rows] if reduction is None else [1])
-    _lib.check(_lib.get().wf2hip_linear_cross_entropy_f32(rows, x.shape[1], w.shape[0], C.c_void_p(x.ptr),
-                                                         C.c_void_p(w.ptr), C.c_void_p(labels.ptr),
-                                                         _REDUCTIONS[reduction], C.c_void_p(loss.ptr),
-                                                         C.c_void_p(lse.ptr)))
+    rows, dim, vocab = _require_labels(name, x, w, labels, lse, reduction)
+    _check(name, "loss", loss, (rows,) if reduction is None else (1,))
+    _lib.check(_lib.get().wf2hip_linear_cross_entropy_f32(rows, dim, vocab, x.ptr, w.ptr, labels.ptr,
+                                                         _REDUCTIONS[reduction], loss.ptr, lse.ptr))
     return loss
 
 
@@ -660,15 +665,14 @@ def _linear_cross_entropy_backward_node(x: HIPTensor, w: HIPTensor, labels: HIPT
     """``X W Labels LSE DOUT DX[rows dim] DW[vocab dim] -> DX DW``.  DOUT: the gradient of the loss, of its shape,
     or None for ones; both times ``scale``."""
     name = "HIP-Linear-Cross-Entropy-Node-backward"
-    rows = _require_labels(name, x, w, labels, lse, reduction)
-    _require_rows(f"{name}: dx", dx, x.shape)
-    _require_rows(f"{name}: dw", dw, w.shape)
+    rows, dim, vocab = _require_labels(name, x, w, labels, lse, reduction)
+    _check(name, "dx", dx, (rows, dim))
+    _check(name, "dw", dw, (vocab, dim))
     if dout is not None:
-        _require_rows(f"{name}: dout", dout, [rows] if reduction is None else [1])
+        _check(name, "dout", dout, (rows,) if reduction is None else (1,))
     _lib.check(_lib.get().wf2hip_linear_cross_entropy_backward_f32(
-        rows, x.shape[1], w.shape[0], C.c_void_p(x.ptr), C.c_void_p(w.ptr), C.c_void_p(labels.ptr),
-        C.c_void_p(lse.ptr), _REDUCTIONS[reduction], None if dout is None else C.c_void_p(dout.ptr), float(scale),
-        C.c_void_p(dx.ptr), C.c_void_p(dw.ptr)))
+        rows, dim, vocab, x.ptr, w.ptr, labels.ptr, lse.ptr, _REDUCTIONS[reduction], None if dout is None else dout.ptr,
+        scale, dx.ptr, dw.ptr))
     return dx, dw
 
 
@@ -791,14 +795,14 @@ def _gpt2_positional_embedding_backward(dout: HIPTensor, ctx: HIPTensor, dwte: H
     """``dout[N sentence-length embedding-size] ctx[N sentence-length] dwte[vocab-size embedding-size]
     dwpe[n-ctx embedding-size] -> dwte dwpe``: the node's gradient, added into those of its tables."""
     name = "GPT2PositionalEmbedding-backward"
-    if len(ctx.shape) != 2 or len(dwte.shape) != 2 or len(dwpe.shape) != 2:
+    sc, sw, sp = ctx._geom()[0], dwte._geom()[0], dwpe._geom()[0]
+    if len(sc) != 2 or len(sw) != 2 or len(sp) != 2:
         raise ValueError(f"{name}: ctx, dwte, dwpe must be matrices")
-    n, t = ctx.shape
-    vocab, dim = dwte.shape
-    _require_rows(f"{name}: ctx", ctx)
-    _require_rows(f"{name}: dout", dout, [n, t, dim])
-    _require_rows(f"{name}: dwte", dwte)
-    _require_rows(f"{name}: dwpe", dwpe, [dwpe.shape[0], dim])
-    _lib.check(_lib.get().wf2hip_embedding_gradient_f32(n * t, t, dim, C.c_void_p(ctx.ptr), C.c_void_p(dout.ptr),
-                                                       C.c_void_p(dwte.ptr), vocab, C.c_void_p(dwpe.ptr), dwpe.shape[0]))
+    n, t = sc
+    vocab, dim = sw
+    _check(name, "ctx", ctx, sc)
+    _check(name, "dout", dout, (n, t, dim))
+    _check(name, "dwte", dwte, sw)
+    _check(name, "dwpe", dwpe, (sp[0], dim))
+    _lib.check(_lib.get().wf2hip_embedding_gradient_f32(n * t, t, dim, ctx.ptr, dout.ptr, dwte.ptr, vocab, dwpe.ptr, sp[0]))
     return dwte, dwpe

@@ -153,7 +153,11 @@ class AdamW:
             self._states[name] = given
         b1, b2 = self.beta1, self.beta2
         self._steps = HIPTensor.from_numpy(np.array([b1 ** done, b2 ** done, done, 0.0]), dtype="double")
+        self._bytes = [4 * n for n in sizes]
         self._table = (_lib.AdamWTensor * len(sizes))()
+        # the table's column of gradient addresses, for one assignment per step
+        self._grads = np.frombuffer(self._table, np.uint64)[_lib.AdamWTensor.grad.offset // 8::C.sizeof(_lib.AdamWTensor) // 8] \
+            if sizes else np.zeros(0, np.uint64)
         scales = [self._states[k] if k in self._states else [None] * len(sizes) for k in ("m_scale", "r_scale")]
         second = self._states["v" if state_bits == 32 else "r"]
         for row, p, n, d, m, v, ms, rs in zip(self._table, self.params, sizes, decays, self._states["m"], second, *scales):
@@ -179,10 +183,11 @@ class AdamW:
         grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"AdamW: {len(grads)} gradients for {len(self.params)} parameters")
-        for row, g in zip(self._table, grads):
-            if g.dtype != "float" or g.size != row.n or not g.is_contiguous():
+        for g, nbytes in zip(grads, self._bytes):
+            # a contiguous tensor owns all of its storage, so that the storage's size is the tensor's
+            if g.dtype != "float" or g.vec.nbytes != nbytes or not g.is_contiguous():
                 raise ValueError("AdamW: a gradient must be a contiguous :float tensor of its parameter's size")
-            row.grad = g.ptr
+        self._grads[:] = [g.vec.ptr for g in grads]
         d = _lib.AdamWDesc(beta1=self.beta1, beta2=self.beta2, eps=self.eps, state_bits=self.state_bits)
         if isinstance(self.lr, HIPTensor):
             if self._own("lr", self.lr) != 1:
