@@ -68,8 +68,8 @@ __global__ __launch_bounds__(kBlock) void xent_largest(long rows, long dim, long
   if (b < kLargestW) {
     const int64_t n = (int64_t)vocab * dim, stride = (int64_t)kLargestW * kBlock;
     int64_t i = (int64_t)b * kBlock + threadIdx.x;
-    if ((uintptr_t)w % 16 == 0) {
-      const f4* w4 = reinterpret_cast<const f4*>(w);
+    {
+      const f4u* w4 = reinterpret_cast<const f4u*>(w);
       const int64_t n4 = n / 4;
       int64_t j = i;
       for (; j + 3 * stride < n4; j += 4 * stride) {
@@ -133,7 +133,9 @@ struct XentSplit {
   XentSum* total;         // PER_ROW
 };
 
-template <bool PER_ROW, bool VEC>
+// HELD: turns of 64 columns that a row's eight threads hold in registers, so that finding the row's largest element and
+// writing its pairs read the row once; 0: any length, read twice.
+template <bool PER_ROW, int HELD>
 __global__ __launch_bounds__(kBlock) void xent_split(XentSplit p) {
   __shared__ float part[kWavesPerBlock];
   const bool of_x = blockIdx.x >= p.wblocks;
@@ -145,19 +147,52 @@ __global__ __launch_bounds__(kBlock) void xent_split(XentSplit p) {
   const float* r = src + row * p.dim;
   const bool inside = row < nrows;
   bool live = inside;
+  if (!PER_ROW && of_x && inside) {
+    const int32_t label = p.labels[row];
+    live = label >= 0;
+    if (c8 == 0)
+      p.g[row] = label < 0 ? 0.0f
+                 : label >= p.vocab ? NAN
+                 : p.dloss && p.per_row_gradient ? __builtin_ldexpf(p.dloss[row], -p.head->eg) : 1.0f;
+  }
+  auto fetch = [&](int c, float(&a)[8]) {   // the eight columns from 8 c on
+    const long col = (long)c * 8;
+    if (live && col + 8 <= p.dim) {
+      const f4 t = *reinterpret_cast<const f4u*>(r + col), u = *reinterpret_cast<const f4u*>(r + col + 4);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        a[k] = t[k];
+        a[4 + k] = u[k];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; k++) a[k] = live && col + k < p.dim ? r[col + k] : 0.0f;
+    }
+  };
+  auto largest = [&](const float(&a)[8]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) m = fmaxf(m, finite_size(a[k]));
+    return m;
+  };
+  const int chunks = p.col_blocks * 2;
+  float held[HELD ? HELD : 1][8];
+#pragma unroll
+  for (int t = 0; t < HELD; t++)
+    if (t * 8 < chunks) fetch(t * 8 + c8, held[t]);
   int e;
   if (PER_ROW) {
     if (blockIdx.x == 0 && threadIdx.x == 0) p.total->arrived = 0u;
     float m = 0.0f;
-    if (inside) {
-      if (VEC) {
-        for (long c = c8 * 4; c < p.dim; c += 32) {
-          const f4 a = *reinterpret_cast<const f4*>(r + c);
+    if (HELD) {
 #pragma unroll
-          for (int k = 0; k < 4; k++) m = fmaxf(m, finite_size(a[k]));
-        }
-      } else {
-        for (long c = c8; c < p.dim; c += 8) m = fmaxf(m, finite_size(r[c]));
+      for (int t = 0; t < HELD; t++)
+        if (t * 8 < chunks) m = fmaxf(m, largest(held[t]));
+    } else {
+      for (int c = c8; c < chunks; c += 8) {
+        float a[8];
+        fetch(c, a);
+        m = fmaxf(m, largest(a));
       }
     }
 #pragma unroll
@@ -177,31 +212,10 @@ __global__ __launch_bounds__(kBlock) void xent_split(XentSplit p) {
         p.head->alpha = p.scale * p.head->weight * (p.dloss && !p.per_row_gradient ? p.dloss[0] : 1.0f);
       }
     }
-    if (of_x && inside) {
-      const int32_t label = p.labels[row];
-      live = label >= 0;
-      if (c8 == 0)
-        p.g[row] = label < 0 ? 0.0f
-                   : label >= p.vocab ? NAN
-                   : p.dloss && p.per_row_gradient ? __builtin_ldexpf(p.dloss[row], -p.head->eg) : 1.0f;
-    }
   }
   char* out = (of_x ? p.px : p.pw) + block * p.col_blocks * (int64_t)kPiece + rr * 16;
   const float up = __builtin_ldexpf(1.0f, e);
-  for (int c = c8; c < p.col_blocks * 2; c += 8) {   // eight columns each
-    float a[8];
-#pragma unroll
-    for (int k = 0; k < 8; k += 4) {
-      const long col = (long)c * 8 + k;
-      if (VEC) {
-        const f4 t = live && col < p.dim ? *reinterpret_cast<const f4*>(r + col) : f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < 4; i++) a[k + i] = t[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) a[k + i] = live && col + i < p.dim ? r[col + i] : 0.0f;
-      }
-    }
+  auto write = [&](int c, const float(&a)[8]) {
     h8 hi, lo;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
@@ -213,6 +227,17 @@ __global__ __launch_bounds__(kBlock) void xent_split(XentSplit p) {
     char* q = out + (int64_t)(c >> 1) * kPiece + (c & 1) * 512;
     *reinterpret_cast<h8*>(q) = hi;
     *reinterpret_cast<h8*>(q + kPiece / 2) = lo;
+  };
+  if (HELD) {
+#pragma unroll
+    for (int t = 0; t < HELD; t++)
+      if (t * 8 + c8 < chunks) write(t * 8 + c8, held[t]);
+  } else {
+    for (int c = c8; c < chunks; c += 8) {
+      float a[8];
+      fetch(c, a);
+      write(c, a);
+    }
   }
 }
 
@@ -229,15 +254,20 @@ struct XentLoss {
   float* at;               // [row] the label's logit
 };
 
+// Folds a maximum and a sum of exponentials into another.
+__device__ __forceinline__ void fold_in(float& top, float& sum, float2 a) {
+  const float both = fmaxf(top, a.x);
+  const float safe = both == -INFINITY ? 0.0f : both;
+  sum = sum * __builtin_amdgcn_exp2f((top - safe) * kLog2eF) + a.y * __builtin_amdgcn_exp2f((a.x - safe) * kLog2eF);
+  top = both;
+}
+
 // A tile of 128 words x 256 rows of x: a lane of the accumulators holds 32 words of one row of x, so that maxima and sums
 // run along registers.
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_loss(XentLoss p) {
-  __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
-  uint32_t tm, tn;
-  pair_tile(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
-  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
-  f16v acc[2][4];
-  pair_product<false, false, false>(p.w, p.x, m0, n0, 0, p.w.col_blocks, smem, acc);
+template <int NB>
+__device__ __forceinline__ void tile_loss(const XentLoss& p, uint32_t tm, int64_t m0, int64_t n0, char* smem) {
+  f16v acc[2][NB];
+  pair_product<false, false, false, NB>(p.w, p.x, m0, n0, 0, p.w.col_blocks, smem, acc);
   __syncthreads();   // the stages are free
   float2* fold = reinterpret_cast<float2*>(smem);            // [wave / 2][256 rows]
   int* ew = reinterpret_cast<int*>(smem + 2 * kTileN * sizeof(float2));
@@ -247,11 +277,11 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
     ew[threadIdx.x] = v < p.vocab ? p.exponent[v] : 0;
   }
   __syncthreads();
-  const int wm = (wave >> 1) * 64;
+  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 32 * NB;
   const bool ragged = m0 + kTileM > p.vocab;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int64_t n = n0 + (wave & 1) * 128 + j * 32 + (lane & 31);
+  for (int j = 0; j < NB; j++) {
+    const int64_t n = n0 + wn + j * 32 + (lane & 31);
     const bool inside = n < p.rows;
     const int ex = inside ? p.exponent[p.x_exponents + n] : 0;
     const int64_t label = inside ? p.labels[n] : -1;
@@ -286,29 +316,29 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
 #pragma unroll
       for (int r = 0; r < 16; r++)
         sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2eF, -base));
-    const float top2 = __shfl_xor(top, 32), sum2 = __shfl_xor(sum, 32);
-    const float both = fmaxf(top, top2);
-    const float safe = both == -INFINITY ? 0.0f : both;
-    sum = sum * __builtin_amdgcn_exp2f((top - safe) * kLog2eF) + sum2 * __builtin_amdgcn_exp2f((top2 - safe) * kLog2eF);
-    if (h == 0) fold[(wave >> 1) * kTileN + (wave & 1) * 128 + j * 32 + lane] = float2{both, sum};
+    fold_in(top, sum, float2{__shfl_xor(top, 32), __shfl_xor(sum, 32)});
+    if (h == 0) fold[(wave >> 1) * kTileN + wn + j * 32 + lane] = float2{top, sum};
   }
   __syncthreads();
   const int64_t n = n0 + threadIdx.x;
-  if (n < p.rows) {
-    const float2 a = fold[threadIdx.x], b = fold[kTileN + threadIdx.x];
-    const float both = fmaxf(a.x, b.x);
-    const float safe = both == -INFINITY ? 0.0f : both;
-    const float sum = a.y * __builtin_amdgcn_exp2f((a.x - safe) * kLog2eF) + b.y * __builtin_amdgcn_exp2f((b.x - safe) * kLog2eF);
-    p.part[(int64_t)tm * p.rows + n] = float2{both, sum};
+  if (threadIdx.x < 64 * NB && n < p.rows) {
+    float top = fold[threadIdx.x].x, sum = fold[threadIdx.x].y;
+    fold_in(top, sum, fold[kTileN + threadIdx.x]);
+    p.part[(int64_t)tm * p.rows + n] = float2{top, sum};
   }
 }
 
-// Folds a maximum and a sum of exponentials into another.
-__device__ __forceinline__ void fold_in(float& top, float& sum, float2 a) {
-  const float both = fmaxf(top, a.x);
-  const float safe = both == -INFINITY ? 0.0f : both;
-  sum = sum * __builtin_amdgcn_exp2f((top - safe) * kLog2eF) + a.y * __builtin_amdgcn_exp2f((a.x - safe) * kLog2eF);
-  top = both;
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_loss(XentLoss p) {
+  __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
+  uint32_t tm, tn;
+  pair_tile(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
+  if (p.rows - n0 > 128)
+    tile_loss<4>(p, tm, m0, n0, smem);
+  else if (p.rows - n0 > 64)
+    tile_loss<2>(p, tm, m0, n0, smem);
+  else
+    tile_loss<1>(p, tm, m0, n0, smem);
 }
 
 // The tiles' maxima and sums of a row.  MANY rows: 64 to a workgroup, a lane each, sixteen wavefronts taking every sixteenth
@@ -385,28 +415,28 @@ struct XentGradient {
   const float *lse, *g;
   long rows, dim;
   long first, words;       // the piece
-  uint32_t tiles_m, tiles_n;
-  int split, steps;        // dx: K steps per share of the piece, in all
-  float* out;              // dw (the piece's rows) or dx's planes
+  uint32_t tiles_m, tiles_n;           // of ds
+  uint32_t tiles_w, tiles_x, tiles_d;  // of 128 words, 128 rows of x, 256 columns
+  uint32_t shares;                     // dx: shares of the piece's K, of `split` K steps
+  int split, steps_dx, steps_dw;
+  bool dw_first;
+  float *planes, *dw;                  // dx's planes from this piece's first on, the piece's rows of dw
 };
 
 constexpr float kLoud = 32768.0f;   // ds is held times 2^15: at most 1 before
 
-// ds of a tile of 128 words x 256 rows of x; also of the tiles' rows and words behind the matrix, as zeros.
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_ds(XentGradient p) {
-  __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
-  uint32_t tm, tn;
-  pair_tile(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
-  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
-  f16v acc[2][4];
-  pair_product<false, false, false>(p.w, p.x, m0, n0, 0, p.w.col_blocks, smem, acc);
+// ds of a tile of 128 words x 64 NB rows of x; also of the tiles' rows and words behind the matrix, as zeros.
+template <int NB>
+__device__ __forceinline__ void tile_ds(const XentGradient& p, int64_t m0, int64_t n0, char* smem) {
+  f16v acc[2][NB];
+  pair_product<false, false, false, NB>(p.w, p.x, m0, n0, 0, p.w.col_blocks, smem, acc);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
-  const int wm = (wave >> 1) * 64;
+  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 32 * NB;
   const int down = -(p.head->ex + p.head->ew);
   const bool ragged = m0 + kTileM > p.words;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int64_t n = n0 + (wave & 1) * 128 + j * 32 + (lane & 31);
+  for (int j = 0; j < NB; j++) {
+    const int64_t n = n0 + wn + j * 32 + (lane & 31);
     const bool inside = n < p.rows;
     const float g = inside ? p.g[n] * kLoud : 0.0f;
     const float base = inside ? p.lse[n] * kLog2eF : 0.0f;
@@ -436,22 +466,31 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   }
 }
 
-// A share of K of dx: plane `share` of p.out, (rows, dim), unscaled.
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_dx(XentGradient p) {
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_ds(XentGradient p) {
   __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
-  const uint32_t tiles = p.tiles_m * p.tiles_n, share = blockIdx.x / tiles;
   uint32_t tm, tn;
-  pair_tile(blockIdx.x - share * tiles, p.tiles_m, p.tiles_n, &tm, &tn);
+  pair_tile(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
   const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
+  if (p.rows - n0 > 128)
+    tile_ds<4>(p, m0, n0, smem);
+  else if (p.rows - n0 > 64)
+    tile_ds<2>(p, m0, n0, smem);
+  else
+    tile_ds<1>(p, m0, n0, smem);
+}
+
+// A share of K of dx: plane `share` of p.planes, (rows, dim), unscaled.
+template <int NB>
+__device__ __forceinline__ void tile_dx(const XentGradient& p, uint32_t share, int64_t m0, int64_t n0, char* smem) {
   const int64_t s0 = (int64_t)share * p.split;
-  const int steps = p.steps - s0 < p.split ? (int)(p.steps - s0) : p.split;
-  f16v acc[2][4];
-  pair_product<false, true, true>(p.ds, p.w, m0, n0, s0 * 16, steps, smem, acc);
+  const int steps = p.steps_dx - s0 < p.split ? (int)(p.steps_dx - s0) : p.split;
+  f16v acc[2][NB];
+  pair_product<false, true, true, NB>(p.ds, p.w, m0, n0, s0 * 16, steps, smem, acc);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
-  float* out = p.out + (int64_t)share * p.rows * p.dim;
+  float* out = p.planes + (int64_t)share * p.rows * p.dim;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int64_t d = n0 + (wave & 1) * 128 + j * 32 + (lane & 31);
+  for (int j = 0; j < NB; j++) {
+    const int64_t d = n0 + (wave & 1) * 32 * NB + j * 32 + (lane & 31);
     if (d < p.dim) {
 #pragma unroll
       for (int i = 0; i < 2; i++)
@@ -464,32 +503,17 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   }
 }
 
-// dx <- the planes' sum, scaled; rows without a label are zero whatever the common factor is
-__global__ __launch_bounds__(kBlock) void xent_fold_dx(long rows, long dim, int planes, const float* __restrict__ part,
-                                                       const float* __restrict__ g, const XentHead* __restrict__ head,
-                                                       float* __restrict__ dx) {
-  const int64_t n = (int64_t)rows * dim, i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (i >= n) return;
-  float sum = part[i];
-  for (int s = 1; s < planes; s++) sum += part[s * n + i];
-  const float v = __builtin_ldexpf(sum, head->eg - 15 - head->ew) * head->alpha;
-  dx[i] = g[i / dim] == 0.0f ? 0.0f : v;
-}
-
 // The piece's rows of dw.
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_dw(XentGradient p) {
-  __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
-  uint32_t tm, tn;
-  pair_tile(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
-  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
-  f16v acc[2][4];
-  pair_product<true, true, true>(p.ds, p.x, m0, n0, 0, p.steps, smem, acc);
+template <int NB>
+__device__ __forceinline__ void tile_dw(const XentGradient& p, int64_t m0, int64_t n0, char* smem) {
+  f16v acc[2][NB];
+  pair_product<true, true, true, NB>(p.ds, p.x, m0, n0, 0, p.steps_dw, smem, acc);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
   const int down = p.head->eg - 15 - p.head->ex;
   const float alpha = p.head->alpha;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int64_t d = n0 + (wave & 1) * 128 + j * 32 + (lane & 31);
+  for (int j = 0; j < NB; j++) {
+    const int64_t d = n0 + (wave & 1) * 32 * NB + j * 32 + (lane & 31);
     if (d < p.dim) {
 #pragma unroll
       for (int i = 0; i < 2; i++)
@@ -497,10 +521,68 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
         for (int r = 0; r < 16; r++) {
           const int64_t v = m0 + (wave >> 1) * 64 + i * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
           const float a = __builtin_ldexpf(acc[i][j][r], down);
-          if (v < p.words) p.out[v * p.dim + d] = a == 0.0f ? 0.0f : a * alpha;
+          if (v < p.words) p.dw[v * p.dim + d] = a == 0.0f ? 0.0f : a * alpha;
         }
     }
   }
+}
+
+// Both products of a piece in one launch, so that neither has a last round of its own: the tiles with the longer K first
+// (dw's K are the rows of x, dx's a share of the words).  A tile that overhangs the columns by more than half runs as a
+// narrower one.
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_gradients(XentGradient p) {
+  __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
+  const uint32_t dw_tiles = p.tiles_w * p.tiles_d, dx_tiles = p.tiles_x * p.tiles_d;
+  uint32_t id = blockIdx.x;
+  // the second kind begins at a multiple of 8 workgroups, where the XCDs' round robin begins anew
+  const uint32_t first = p.dw_first ? dw_tiles : dx_tiles * p.shares, behind = (first + 7) & ~7u;
+  const bool of_first = id < behind;
+  if (of_first && id >= first) return;
+  if (!of_first) id -= behind;
+  const bool dw = of_first == p.dw_first;
+  uint32_t tm, tn, share = 0;
+  if (!dw) {
+    share = id / dx_tiles;
+    id -= share * dx_tiles;
+  }
+  pair_tile(id, dw ? p.tiles_w : p.tiles_x, p.tiles_d, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
+  const int64_t rest = p.dim - n0;
+  if (dw) {
+    if (rest > 128)
+      tile_dw<4>(p, m0, n0, smem);
+    else if (rest > 64)
+      tile_dw<2>(p, m0, n0, smem);
+    else
+      tile_dw<1>(p, m0, n0, smem);
+  } else {
+    if (rest > 128)
+      tile_dx<4>(p, share, m0, n0, smem);
+    else if (rest > 64)
+      tile_dx<2>(p, share, m0, n0, smem);
+    else
+      tile_dx<1>(p, share, m0, n0, smem);
+  }
+}
+
+// dx <- the planes' sum, scaled; rows without a label are zero whatever the common factor is
+template <bool VEC>
+__global__ __launch_bounds__(kBlock) void xent_fold_dx(int64_t n, long dim, int planes, const float* __restrict__ part,
+                                                       const float* __restrict__ g, const XentHead* __restrict__ head,
+                                                       float* __restrict__ dx) {
+  typedef float fv __attribute__((ext_vector_type(VEC ? 4 : 1)));
+  constexpr int V = VEC ? 4 : 1;
+  const int64_t i = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * V;
+  if (i >= n) return;
+  fv sum = *reinterpret_cast<const fv*>(part + i);
+#pragma unroll 4
+  for (int s = 1; s < planes; s++) sum += *reinterpret_cast<const fv*>(part + s * n + i);
+  const int down = head->eg - 15 - head->ew;
+  const float alpha = head->alpha;
+  const bool none = g[i / dim] == 0.0f;   // a vector lies within a row
+#pragma unroll
+  for (int c = 0; c < V; c++) sum[c] = none ? 0.0f : __builtin_ldexpf(sum[c], down) * alpha;
+  *reinterpret_cast<fv*>(dx + i) = sum;
 }
 
 // ---- straight from binary32: few rows, small products -----------------------------------------------------------
@@ -937,10 +1019,15 @@ static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int6
 template <bool PER_ROW>
 static int split_operands(const XentSplit& p, hipStream_t st) {
   const uint32_t blocks = p.wblocks + (uint32_t)ceil_div(p.rows, 32);
-  if (p.dim % 4 == 0 && ((uintptr_t)p.x | (uintptr_t)p.w) % 16 == 0)
-    xent_split<PER_ROW, true><<<blocks, kBlock, 0, st>>>(p);
+  // rows read twice without a register copy: 100 us for the (50257, 768) table where one read takes 64
+  if (PER_ROW && p.dim <= 256)
+    xent_split<PER_ROW, 4><<<blocks, kBlock, 0, st>>>(p);
+  else if (PER_ROW && p.dim <= 512)
+    xent_split<PER_ROW, 8><<<blocks, kBlock, 0, st>>>(p);
+  else if (PER_ROW && p.dim <= 832)
+    xent_split<PER_ROW, 13><<<blocks, kBlock, 0, st>>>(p);
   else
-    xent_split<PER_ROW, false><<<blocks, kBlock, 0, st>>>(p);
+    xent_split<PER_ROW, 0><<<blocks, kBlock, 0, st>>>(p);
   return after_launch("xent_split");
 }
 
@@ -1048,18 +1135,20 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
   hipStream_t st = rt().stream;
   const int64_t words = xent_words(rows, vocab);
   const int64_t padded = ceil_div(rows, kTileN) * kTileN;
-  const int64_t tiles_d = ceil_div(dim, kTileN);
-  // dx has few tiles and a long K: shares of K that fill the device twice, of at least 16 K steps, in even numbers (a
-  // share starts at a whole row block of w)
-  const int64_t dx_tiles = ceil_div(rows, kTileM) * tiles_d, all_steps = ceil_div(words < vocab ? words : vocab, 16);
-  int64_t shares = ceil_div(4 * rt().num_cus, dx_tiles);
-  if (shares > all_steps / 16) shares = all_steps / 16;
-  if (shares < 1) shares = 1;
-  const int64_t split = ceil_div(ceil_div(all_steps, shares), 2) * 2;
+  const int64_t tiles_d = ceil_div(dim, kTileN), tiles_x = ceil_div(rows, kTileM);
+  // dx has few tiles and a long K: shares of it of about a quarter of what a workgroup slot (two to a compute unit) gets to
+  // do in all, so that the last ones fill the gaps; half of it where dw's tiles are short enough for that.  At least 16 K
+  // steps, an even number (a share starts at a whole row block of w).
+  const int64_t steps_dx = ceil_div(words < vocab ? words : vocab, 16), steps_dw = ceil_div(rows, 16);
+  const int64_t slot = tiles_d * (words / kTileM * steps_dw + tiles_x * steps_dx) / (2 * rt().num_cus);
+  int64_t split = steps_dw <= slot / 2 ? slot / 2 : slot / 4;
+  if (split > steps_dx) split = steps_dx;
+  if (split < 16) split = 16;
+  split = ceil_div(ceil_div(steps_dx, ceil_div(steps_dx, split)), 2) * 2;
   int64_t planes = 0;
   for (int64_t c = 0; c < vocab; c += words) planes += ceil_div(ceil_div(words < vocab - c ? words : vocab - c, 16), split);
-  const int64_t most = ((int64_t)1 << 31) - 1;
-  if (words / kTileM * (padded / kTileN) > most || dx_tiles * shares > most || words / kTileM * tiles_d > most ||
+  const int64_t most = ((int64_t)1 << 31) - 16;
+  if (words / kTileM * (padded / kTileN) > most || tiles_d * (words / kTileM + tiles_x * ceil_div(steps_dx, split)) > most ||
       ceil_div(nx, kBlock) > most)
     return fail(WF2HIP_EUNSUPPORTED, "%s: too many tiles for one launch", name);
 
@@ -1113,24 +1202,25 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
     xent_tile_ds<<<p.tiles_m * p.tiles_n, kBlock, 0, st>>>(p);
     WF2_TRY(after_launch("xent_tile_ds"));
 
-    XentGradient q = p;
-    q.tiles_m = (uint32_t)ceil_div(rows, kTileM);
-    q.tiles_n = (uint32_t)tiles_d;
-    q.steps = (int)ceil_div(p.words, 16);
-    q.split = (int)split;
-    const int64_t here = ceil_div(q.steps, split);
-    q.out = part + plane * nx;
-    xent_tile_dx<<<(uint32_t)(dx_tiles * here), kBlock, 0, st>>>(q);
-    WF2_TRY(after_launch("xent_tile_dx"));
-    plane += here;
-
-    q = p;
-    q.tiles_n = (uint32_t)tiles_d;
-    q.steps = (int)ceil_div(rows, 16);
-    q.out = dw + c * dim;
-    xent_tile_dw<<<(uint32_t)(q.tiles_m * tiles_d), kBlock, 0, st>>>(q);
-    WF2_TRY(after_launch("xent_tile_dw"));
+    p.tiles_w = p.tiles_m;
+    p.tiles_x = (uint32_t)tiles_x;
+    p.tiles_d = (uint32_t)tiles_d;
+    p.steps_dx = (int)ceil_div(p.words, 16);
+    p.steps_dw = (int)steps_dw;
+    p.split = (int)split;
+    p.shares = (uint32_t)ceil_div(p.steps_dx, split);
+    p.dw_first = steps_dw >= split;
+    p.planes = part + plane * nx;
+    p.dw = dw + c * dim;
+    plane += p.shares;
+    const uint32_t dw_tiles = p.tiles_w * p.tiles_d, dx_units = p.tiles_x * p.tiles_d * p.shares;
+    const uint32_t front = p.dw_first ? dw_tiles : dx_units;
+    xent_tile_gradients<<<((front + 7) & ~7u) + (p.dw_first ? dx_units : dw_tiles), kBlock, 0, st>>>(p);
+    WF2_TRY(after_launch("xent_tile_gradients"));
   }
-  xent_fold_dx<<<(uint32_t)ceil_div(nx, kBlock), kBlock, 0, st>>>(rows, dim, (int)planes, part, g, head, dx);
+  if (dim % 4 == 0 && (uintptr_t)dx % 16 == 0)
+    xent_fold_dx<true><<<(uint32_t)ceil_div(nx / 4, kBlock), kBlock, 0, st>>>(nx, dim, (int)planes, part, g, head, dx);
+  else
+    xent_fold_dx<false><<<(uint32_t)ceil_div(nx, kBlock), kBlock, 0, st>>>(nx, dim, (int)planes, part, g, head, dx);
   return after_launch("xent_fold_dx");
 }

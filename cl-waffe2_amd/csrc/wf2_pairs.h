@@ -36,15 +36,15 @@ struct PairMatrix {
   __host__ __device__ int64_t pitch() const { return (int64_t)col_blocks * kPiece; }
 };
 
-// One workgroup's 128 x 256 tile of C[m][n] = sum_k A(m, k) B(n, k): four wavefronts, each 64 x 128 as 2 x 4
-// blocks of 32 x 32; two workgroups to a compute unit, so that one's prologue and epilogue run under the
+// One workgroup's 128 x 64 NB tile of C[m][n] = sum_k A(m, k) B(n, k), NB = 4 (2 and 1 at the end of a matrix that leaves most of
+// a tile empty): four wavefronts, each 64 x 32 NB as 2 x NB blocks of 32 x 32; two workgroups to a compute unit, so that one's prologue and epilogue run under the
 // other's products.  K steps of 16 arrive by DMA in a ring of three stages of 24 KB, two steps ahead.
 // AT / BT: k runs along the rows of that operand's storage instead of its columns.
 // LOUD: the lo parts of A are stored 2^11 times too large (numbers of a wide range: dozens of octaves below the
 // largest still keep 22 bits); their partner is scaled down in registers, exactly unless it is 2^18 times below its
 // largest.
 constexpr int kTileM = 128, kTileN = 256;
-constexpr int kStageA = kTileM / 32 * kPiece, kStageB = kTileN / 32 * kPiece, kStage = kStageA + kStageB;
+constexpr int kStageA = kTileM / 32 * kPiece, kStage = kStageA + kTileN / 32 * kPiece;
 constexpr int kRing = 3;
 
 template <bool T>
@@ -94,24 +94,24 @@ struct PairStream {
   }
 };
 
-template <bool AT, bool BT, bool LOUD>
+template <bool AT, bool BT, bool LOUD, int NB>
 __device__ __forceinline__ void pair_product(const PairMatrix& A, const PairMatrix& B, int64_t m0, int64_t n0,
-                                             int64_t k0, int steps, char* smem, f16v (&acc)[2][4]) {
+                                             int64_t k0, int steps, char* smem, f16v (&acc)[2][NB]) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
 
   PairStream<AT> sa[2];
-  PairStream<BT> sb[4];
+  PairStream<BT> sb[NB];
 #pragma unroll
   for (int j = 0; j < 2; j++) sa[j].start(A, m0, wave * 2 + j, k0);
 #pragma unroll
-  for (int j = 0; j < 4; j++) sb[j].start(B, n0, wave * 4 + j, k0);
+  for (int j = 0; j < NB; j++) sb[j].start(B, n0, wave * NB + j, k0);
   uint32_t oa[2], ob[2];
 #pragma unroll
   for (int j = 0; j < 2; j++) {
     oa[j] = PairStream<AT>::lane_offset(lane, j);
-    ob[j] = PairStream<BT>::lane_offset(lane, j);
+    ob[j] = PairStream<BT>::lane_offset(lane, (wave * NB + j) & 1);
   }
   int fetched = 0;
   uint32_t into = 0;
@@ -123,8 +123,8 @@ __device__ __forceinline__ void pair_product(const PairMatrix& A, const PairMatr
       sa[j].next(fetched & 1);
     }
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      dma16(to + kStageA + (wave * 4 + j) * 1024, ob[BT ? (j & 1) : 0], reinterpret_cast<const float*>(sb[j].at));
+    for (int j = 0; j < NB; j++) {
+      dma16(to + kStageA + (wave * NB + j) * 1024, ob[BT ? (j & 1) : 0], reinterpret_cast<const float*>(sb[j].at));
       sb[j].next(fetched & 1);
     }
     fetched++;
@@ -134,55 +134,55 @@ __device__ __forceinline__ void pair_product(const PairMatrix& A, const PairMatr
 #pragma unroll
   for (int i = 0; i < 2; i++)
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+    for (int j = 0; j < NB; j++)
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
 
   const uint32_t ra = PairStream<AT>::read_offset(lane) + (wave >> 1) * 2 * kPiece;
-  const uint32_t rb = PairStream<BT>::read_offset(lane) + kStageA + (wave & 1) * 4 * kPiece;
+  const uint32_t rb = PairStream<BT>::read_offset(lane) + kStageA + (wave & 1) * NB * kPiece;
 
   fetch();
   if (steps > 1) fetch();
   uint32_t from = 0;
   for (int s = 0; s < steps; s++) {
-    // this wavefront's part of the stage has landed when at most the next stage's six loads are in flight; its own
+    // this wavefront's part of the stage has landed when at most the next stage's 2 + NB loads are in flight; its own
     // reads of the stage before have ended
     if (s + 1 < steps)
-      asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 + NB) : "memory");
     else
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     // everybody is past the products of the step before: its stage is free
     if (s + 2 < steps) fetch();
-    h8 ah[2], al[2], bh[4], bl[4];
+    h8 ah[2], al[2], bh[NB], bl[NB];
     const char* st = smem + from;
 #pragma unroll
     for (int i = 0; i < 2; i++) ah[i] = PairStream<AT>::read(st, ra + i * kPiece, 0);
 #pragma unroll
-    for (int j = 0; j < 4; j++) bh[j] = PairStream<BT>::read(st, rb + j * kPiece, 0);
+    for (int j = 0; j < NB; j++) bh[j] = PairStream<BT>::read(st, rb + j * kPiece, 0);
 #pragma unroll
-    for (int j = 0; j < 4; j++) bl[j] = PairStream<BT>::read(st, rb + j * kPiece, 1);
+    for (int j = 0; j < NB; j++) bl[j] = PairStream<BT>::read(st, rb + j * kPiece, 1);
 #pragma unroll
     for (int i = 0; i < 2; i++) al[i] = PairStream<AT>::read(st, ra + i * kPiece, 1);
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int j = 0; j < 4; j++)
+      for (int j = 0; j < NB; j++)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int j = 0; j < 4; j++)
+      for (int j = 0; j < NB; j++)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
     if (LOUD) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) bh[j] = bh[j] * (_Float16)0.00048828125f;   // 2^-11
+      for (int j = 0; j < NB; j++) bh[j] = bh[j] * (_Float16)0.00048828125f;   // 2^-11
     }
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int j = 0; j < 4; j++)
+      for (int j = 0; j < NB; j++)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
     from = from == (kRing - 1) * kStage ? 0 : from + kStage;
   }
