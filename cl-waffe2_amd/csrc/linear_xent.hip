@@ -604,7 +604,7 @@ struct XentDirect {
   int64_t pitch;
   uint32_t tiles_dw;           // dw: columns of x
   uint32_t tiles_dx, tiles_nx; // dx: columns, rows of x
-  uint32_t dw_units;           // workgroups of dw; those of dx follow
+  uint32_t dw_units, dx_units; // workgroups of either
   int64_t share;               // words of a share of dx's K
   float *dx, *dw;              // dx: a plane per share
 };
@@ -612,12 +612,12 @@ struct XentDirect {
 // A tile of 128 words x 32 NB rows of x.
 template <int NB>
 __global__ __launch_bounds__(kBlock) void xent_direct_loss(XentDirect p) {
-  __shared__ __attribute__((aligned(16))) char smem[kSkinnyLds<NB>];
+  __shared__ __attribute__((aligned(16))) char smem[kSkinnyLds<NB, false>];
   if (blockIdx.x == 0 && threadIdx.x == 0) p.total->arrived = 0u;
   const uint32_t tn = blockIdx.x % p.tiles_n, tv = blockIdx.x / p.tiles_n;
   const int64_t m0 = (int64_t)tv * kSkinnyRows, n0 = (int64_t)tn * 32 * NB;
   f16v acc[NB];
-  skinny_product<NB, false>(DirectMatrix{p.w, p.dim, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.rows, nullptr}, m0, n0, p.dim,
+  skinny_product<NB, false, false>(DirectMatrix{p.w, p.dim, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.rows, nullptr}, m0, n0, p.dim,
                             smem, acc);
   lds_barrier();   // the stages are free
   float2* fold = reinterpret_cast<float2*>(smem);   // [wavefront][row of x]
@@ -668,12 +668,12 @@ __device__ __forceinline__ float xent_weight(const XentDirect& p) {
 // the storage.
 template <int NB>
 __global__ __launch_bounds__(kBlock) void xent_direct_ds(XentDirect p) {
-  __shared__ __attribute__((aligned(16))) char smem[kSkinnyLds<NB>];
+  __shared__ __attribute__((aligned(16))) char smem[kSkinnyLds<NB, false>];
   const uint32_t tn = blockIdx.x % p.tiles_n, tv = blockIdx.x / p.tiles_n;
   const int64_t m0 = (int64_t)tv * kSkinnyRows, n0 = (int64_t)tn * 32 * NB;
   const float weight = xent_weight(p);
   f16v acc[NB];
-  skinny_product<NB, false>(DirectMatrix{p.w, p.dim, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.rows, nullptr}, m0, n0, p.dim,
+  skinny_product<NB, false, false>(DirectMatrix{p.w, p.dim, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.rows, nullptr}, m0, n0, p.dim,
                             smem, acc);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
 #pragma unroll
@@ -808,40 +808,22 @@ __global__ __launch_bounds__(kBlock) void xent_small_ds(XentDirect p) {
   }
 }
 
-// Tiles of dw -- NBW 0: 32 words x 32 columns; otherwise 128 words x 32 NBW columns; K the rows of x -- and, behind them, of
-// dx (32 columns x 32 NBX rows of x, K a share of the words).
-template <int NBW, int NBX>
-__global__ __launch_bounds__(kBlock) void xent_direct_gradients(XentDirect p) {
-  constexpr int kLdsW = NBW ? kSkinnyLds<NBW> : kSmallLds<1>, kLdsX = kSmallLds<NBX>;
-  __shared__ __attribute__((aligned(16))) char smem[kLdsW > kLdsX ? kLdsW : kLdsX];
+// Tiles of dw (32 words x 32 columns, K the rows of x) and, behind them, of dx (32 columns x 32 NBX rows of x, K a share of the
+// words).
+template <int NBX>
+__global__ __launch_bounds__(kBlock) void xent_small_gradients(XentDirect p) {
+  __shared__ __attribute__((aligned(16))) char smem[kSmallLds<NBX>];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
   if (blockIdx.x < p.dw_units) {
     const uint32_t td = blockIdx.x % p.tiles_dw, tv = blockIdx.x / p.tiles_dw;
-    const DirectMatrix ds{p.ds, p.pitch, p.vocab, nullptr}, x{p.x, p.dim, p.dim, p.labels};
-    if constexpr (NBW == 0) {
-      const int64_t m0 = (int64_t)tv * 32, d = (int64_t)td * 32 + (lane & 31);
-      float s[1][4];
-      small_product<1, false, true>(ds, x, m0, (int64_t)td * 32, 0, p.rows, smem, s);
+    const int64_t m0 = (int64_t)tv * 32, d = (int64_t)td * 32 + (lane & 31);
+    float s[1][4];
+    small_product<1, false, true>(DirectMatrix{p.ds, p.pitch, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.dim, p.labels}, m0,
+                                  (int64_t)td * 32, 0, p.rows, smem, s);
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        const int64_t v = m0 + wave * 8 + h * 4 + c;
-        if (v < p.vocab && d < p.dim) p.dw[v * p.dim + d] = s[0][c];
-      }
-    } else {
-      const int64_t m0 = (int64_t)tv * kSkinnyRows, d0 = (int64_t)td * 32 * NBW;
-      f16v acc[NBW ? NBW : 1];
-      skinny_product<NBW ? NBW : 1, true>(ds, x, m0, d0, p.rows, smem, acc);
-#pragma unroll
-      for (int j = 0; j < NBW; j++) {
-        const int64_t d = d0 + j * 32 + (lane & 31);
-        if (d < p.dim) {
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const int64_t v = m0 + wave * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
-            if (v < p.vocab) p.dw[v * p.dim + d] = acc[j][r];
-          }
-        }
-      }
+    for (int c = 0; c < 4; c++) {
+      const int64_t v = m0 + wave * 8 + h * 4 + c;
+      if (v < p.vocab && d < p.dim) p.dw[v * p.dim + d] = s[0][c];
     }
     return;
   }
@@ -862,6 +844,53 @@ __global__ __launch_bounds__(kBlock) void xent_direct_gradients(XentDirect p) {
       for (int c = 0; c < 4; c++) {
         const int64_t d = d0 + wave * 8 + h * 4 + c;
         if (d < p.dim) out[n * p.dim + d] = s[j][c];
+      }
+    }
+  }
+}
+
+// The same in tiles of 128: dw 128 words x 32 NBW columns, dx 128 columns x 32 NBX rows of x.  dx first: its K is the longer.
+template <int NBW, int NBX>
+__global__ __launch_bounds__(kBlock) void xent_direct_gradients(XentDirect p) {
+  constexpr int kLdsW = kSkinnyLds<NBW, false>, kLdsX = kSkinnyLds<NBX, true>;
+  __shared__ __attribute__((aligned(16))) char smem[kLdsW > kLdsX ? kLdsW : kLdsX];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
+  if (blockIdx.x >= p.dx_units) {
+    const uint32_t unit = blockIdx.x - p.dx_units;
+    const uint32_t td = unit % p.tiles_dw, tv = unit / p.tiles_dw;
+    const int64_t m0 = (int64_t)tv * kSkinnyRows, d0 = (int64_t)td * 32 * NBW;
+    f16v acc[NBW];
+    skinny_product<NBW, false, true>(DirectMatrix{p.ds, p.pitch, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.dim, p.labels}, m0, d0,
+                                     p.rows, smem, acc);
+#pragma unroll
+    for (int j = 0; j < NBW; j++) {
+      const int64_t d = d0 + j * 32 + (lane & 31);
+      if (d < p.dim) {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int64_t v = m0 + wave * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
+          if (v < p.vocab) p.dw[v * p.dim + d] = acc[j][r];
+        }
+      }
+    }
+    return;
+  }
+  const uint32_t td = blockIdx.x % p.tiles_dx, rest = blockIdx.x / p.tiles_dx;
+  const uint32_t tn = rest % p.tiles_nx, share = rest / p.tiles_nx;
+  const int64_t d0 = (int64_t)td * kSkinnyRows, n0 = (int64_t)tn * 32 * NBX;
+  const int64_t k0 = share * p.share, K = (k0 + p.share < p.vocab ? k0 + p.share : p.vocab) - k0;
+  f16v acc[NBX];
+  skinny_product<NBX, true, true>(DirectMatrix{p.w + k0 * p.dim, p.dim, p.dim, nullptr},
+                                  DirectMatrix{p.ds + k0 * p.pitch, p.pitch, p.rows, nullptr}, d0, n0, K, smem, acc);
+  float* out = p.dx + (int64_t)share * p.rows * p.dim;
+#pragma unroll
+  for (int j = 0; j < NBX; j++) {
+    const int64_t n = n0 + j * 32 + (lane & 31);
+    if (n < p.rows) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int64_t d = d0 + wave * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
+        if (d < p.dim) out[n * p.dim + d] = acc[j][r];
       }
     }
   }
@@ -950,19 +979,29 @@ static XentRoute xent_route(int64_t rows, int64_t dim, int64_t vocab, bool backw
 // Width of a tile in blocks of 32: no wider than the operand, `most` where that is longer.
 static int xent_blocks(int64_t extent, int most) { return extent <= 32 ? 1 : extent <= 64 || most == 2 ? 2 : 4; }
 
+// Whether the gradients' tiles are 128 wide (a wavefront each for 32 of them) or 32 (a quarter of K each).
+static bool xent_wide_gradients(XentRoute route, int64_t rows, int64_t dim, int64_t vocab) {
+  if (const char* env = getenv("WF2HIP_XENT_ROUTE"))
+    if (env[0] == '1' || env[0] == '2') return env[0] == '1';
+  return route == kSkinny || ceil_div(vocab, kSkinnyRows) * ceil_div(dim, 128) >= 128;
+}
+
 static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int64_t vocab, const float* x, const float* w,
                                 const int32_t* labels, const float* lse, int reduction, const float* dloss, float scale,
                                 float* dx, float* dw) {
   hipStream_t st = rt().stream;
   const bool small = route == kSmall;
-  const int nb = xent_blocks(rows, small ? 2 : 4), nbw = small ? 0 : xent_blocks(dim, 4), nbx = xent_blocks(rows, 2);
+  const int nb = xent_blocks(rows, small ? 2 : 4);
+  // the gradients have tiles of their own: 128 wide where those fill the device
+  const bool wide = xent_wide_gradients(route, rows, dim, vocab);
+  const int nbw = wide ? xent_blocks(dim, 4) : 1, nbx = xent_blocks(rows, wide ? 4 : 2);
   XentDirect p{};
   p.x = x; p.w = w; p.labels = labels;
   p.rows = rows; p.dim = dim; p.vocab = vocab;
   p.tiles_v = (uint32_t)ceil_div(vocab, small ? 32 : kSkinnyRows);
   p.tiles_n = (uint32_t)ceil_div(rows, 32 * nb);
-  p.tiles_dw = (uint32_t)ceil_div(dim, small ? 32 : 32 * nbw);
-  p.tiles_dx = (uint32_t)ceil_div(dim, 32);
+  p.tiles_dw = (uint32_t)ceil_div(dim, 32 * nbw);
+  p.tiles_dx = (uint32_t)ceil_div(dim, wide ? kSkinnyRows : 32);
   p.tiles_nx = (uint32_t)ceil_div(rows, 32 * nbx);
   p.lse = lse; p.dloss = dloss;
   p.per_row = reduction == WF2HIP_REDUCE_NONE;
@@ -976,10 +1015,11 @@ static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int6
   if (shares < 1) shares = 1;
   p.share = ceil_div(all_steps, shares) * kDirectStep;
   shares = ceil_div(vocab, p.share);
-  const int64_t dw_units = (int64_t)p.tiles_v * p.tiles_dw, most = ((int64_t)1 << 31) - 1;
+  const int64_t dw_units = ceil_div(vocab, wide ? kSkinnyRows : 32) * p.tiles_dw, most = ((int64_t)1 << 31) - 1;
   if (dw_units + dx_tiles * shares > most || (int64_t)p.tiles_v * p.tiles_n > most)
     return fail(WF2HIP_EUNSUPPORTED, "linear cross entropy backward: too many tiles for one launch");
   p.dw_units = (uint32_t)dw_units;
+  p.dx_units = (uint32_t)(dx_tiles * shares);
   Blocks blocks;
   p.ds = blocks.take<float>(vocab * p.pitch * 4);
   p.dx = shares > 1 ? blocks.take<float>(shares * rows * dim * 4) : dx;
@@ -993,23 +1033,21 @@ static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int6
   else
     nb == 1 ? xent_direct_ds<1><<<tiles, kBlock, 0, st>>>(p) : xent_direct_ds<2><<<tiles, kBlock, 0, st>>>(p);
   WF2_TRY(after_launch("xent ds"));
-  auto gradients = [&](auto wide, auto rows_wide) {
-    xent_direct_gradients<decltype(wide)::value, decltype(rows_wide)::value><<<units, kBlock, 0, st>>>(p);
-  };
-  auto with_rows = [&](auto wide) {
-    if (nbx == 1)
-      gradients(wide, std::integral_constant<int, 1>());
+  if (!wide) {
+    nbx == 1 ? xent_small_gradients<1><<<units, kBlock, 0, st>>>(p) : xent_small_gradients<2><<<units, kBlock, 0, st>>>(p);
+  } else {
+    auto with = [&](auto w_blocks) {
+      constexpr int NBW = decltype(w_blocks)::value;
+      if (nbx == 4)
+        xent_direct_gradients<NBW, 4><<<units, kBlock, 0, st>>>(p);
+      else
+        nbx == 1 ? xent_direct_gradients<NBW, 1><<<units, kBlock, 0, st>>>(p) : xent_direct_gradients<NBW, 2><<<units, kBlock, 0, st>>>(p);
+    };
+    if (nbw == 4)
+      with(std::integral_constant<int, 4>());
     else
-      gradients(wide, std::integral_constant<int, 2>());
-  };
-  if (nbw == 0)
-    with_rows(std::integral_constant<int, 0>());
-  else if (nbw == 1)
-    with_rows(std::integral_constant<int, 1>());
-  else if (nbw == 2)
-    with_rows(std::integral_constant<int, 2>());
-  else
-    with_rows(std::integral_constant<int, 4>());
+      nbw == 1 ? with(std::integral_constant<int, 1>()) : with(std::integral_constant<int, 2>());
+  }
   WF2_TRY(after_launch("xent_direct_gradients"));
   if (shares == 1) return 0;
   xent_direct_fold<<<(uint32_t)ceil_div(rows * dim, kBlock), kBlock, 0, st>>>(rows * dim, (int)shares, p.dx, dx);

@@ -20,6 +20,7 @@ typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // unaligne
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kDirectStep = 32;                     // K goes by 32
 constexpr int kDirectPart = 32 * 16 * 2;            // bytes of one part of a 32 x 16 piece, in the order of the lanes
@@ -65,8 +66,11 @@ __device__ __forceinline__ void put_parts(char* half, int i, int g, float a, flo
 // pass through LDS, taken apart once, a step ahead.  Vector instructions and matrix instructions share a SIMD's time
 // here, so what counts is how few of the former there are: per 32 x 32 x 32 products 88 / NB for A's parts and 22 for B's.
 constexpr int kSkinnyRows = 128;
-template <int NB>
-constexpr int kSkinnyLds = 2 * NB * kDirectHalf;
+// AT: k runs along the rows of A's storage.  A wavefront then turns its 32 x 32 numbers of a step over on their way: the
+// parts are written to LDS of its own as they come, four columns at a time, and read back by the transposing LDS
+// read; within a wavefront LDS keeps the order of the program, so no barrier is needed.
+template <int NB, bool AT>
+constexpr int kSkinnyLds = 2 * NB * kDirectHalf + (AT ? 4 * kDirectHalf : 0);
 
 __device__ __forceinline__ void three_parts(const float (&x)[8], b8 (&out)[3]) {
   uint32_t one[8], two[8], three[8];
@@ -77,7 +81,6 @@ __device__ __forceinline__ void three_parts(const float (&x)[8], b8 (&out)[3]) {
     two[n] = __builtin_bit_cast(uint32_t, r) & 0xffff0000u;
     three[n] = __builtin_bit_cast(uint32_t, r - __builtin_bit_cast(float, two[n]));
   }
-  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
   auto pack = [](const uint32_t(&a)[8]) {
     u4 v;
 #pragma unroll
@@ -89,15 +92,28 @@ __device__ __forceinline__ void three_parts(const float (&x)[8], b8 (&out)[3]) {
   out[2] = pack(three);
 }
 
-template <int NB, bool BT>
+typedef __fp16 fp4 __attribute__((ext_vector_type(4)));
+
+template <int NB, bool AT, bool BT>
 __device__ __forceinline__ void skinny_product(const DirectMatrix& A, const DirectMatrix& B, int64_t m0, int64_t n0, int64_t K,
                                                char* smem, f16v (&acc)[NB]) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  // A: this lane's row
-  int64_t i = m0 + wave * 32 + (lane & 31);
-  i = i < A.rows ? i : A.rows - 1;   // rows behind the matrix feed outputs nobody keeps
-  const float* a = A.base + i * A.ld + (lane >> 5) * 8;
+  // A: this lane's row, or (AT) its four columns of the k rows l / 8 + 0, 8, 16, 24
+  const int64_t i0 = m0 + wave * 32;
+  const float* a;
+  int a_inside = 4;                  // AT: how many of the four columns lie inside
+  if (AT) {
+    const int64_t i = i0 + (lane & 7) * 4;
+    a_inside = i + 4 <= A.rows ? 4 : i < A.rows ? (int)(A.rows - i) : 0;
+    a = A.base + (int64_t)(lane >> 3) * A.ld + (a_inside ? i : 0);
+  } else {
+    int64_t i = i0 + (lane & 31);
+    i = i < A.rows ? i : A.rows - 1;   // rows behind the matrix feed outputs nobody keeps
+    a = A.base + i * A.ld + (lane >> 5) * 8;
+  }
+  const int64_t a_step = AT ? kDirectStep * A.ld : kDirectStep;
+  char* mine = smem + 2 * NB * kDirectHalf + wave * kDirectHalf;   // AT: [part][k row][32 columns]
   // B: this thread's units.  K contiguous: four k of NB rows; otherwise four rows of the operand at four k, the first 64 NB
   // threads.
   constexpr int kUnits = BT ? 4 : NB;
@@ -127,14 +143,41 @@ __device__ __forceinline__ void skinny_product(const DirectMatrix& A, const Dire
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       const int k = (u >> 1) * 16 + (u & 1) * 4;
+      const float* q = AT ? a + (int64_t)u * 8 * A.ld : a + k;
       if constexpr (decltype(whole)::value) {
-        av[decltype(set)::value][u] = *reinterpret_cast<const f4u*>(a + k);
+        av[decltype(set)::value][u] = *reinterpret_cast<const f4u*>(q);
       } else {
 #pragma unroll
-        for (int c = 0; c < 4; c++) av[decltype(set)::value][u][c] = k + c + (lane >> 5) * 8 < left ? a[k + c] : 0.0f;
+        for (int c = 0; c < 4; c++)
+          av[decltype(set)::value][u][c] =
+              (AT ? (lane >> 3) + u * 8 < left && c < a_inside : k + c + (lane >> 5) * 8 < left) ? q[c] : 0.0f;
       }
     }
-    a += kDirectStep;
+    a += a_step;
+  };
+  // AT: the step's numbers in parts, in the order of the storage
+  auto turn = [&](auto set) {
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const f4 x = av[decltype(set)::value][u];
+      float two4[8] = {x[0], x[1], x[2], x[3], 0.0f, 0.0f, 0.0f, 0.0f};
+      b8 p[3];
+      three_parts(two4, p);
+#pragma unroll
+      for (int t = 0; t < 3; t++)
+        *reinterpret_cast<u2*>(mine + t * 2048 + ((lane >> 3) + u * 8) * 64 + (lane & 7) * 8) =
+            __builtin_shufflevector(__builtin_bit_cast(u4, p[t]), __builtin_bit_cast(u4, p[t]), 0, 1);
+    }
+  };
+  auto turned = [&](int s, int t) {   // part t of this lane's operand of the half step s
+    const int g = lane >> 4, l16 = lane & 15;
+    const char* q = mine + t * 2048 + (s * 16 + (g >> 1) * 8 + (l16 >> 2)) * 64 + (g & 1) * 32 + (l16 & 3) * 8;
+    auto read = [](const char* r) {
+      return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                                        (__attribute__((address_space(3))) fp4*)(__attribute__((address_space(3))) char*)r));
+    };
+    const u2 lo = read(q), hi = read(q + 4 * 64);
+    return __builtin_bit_cast(b8, u4{lo[0], lo[1], hi[0], hi[1]});
   };
   auto fetch_b = [&](auto whole, int64_t left) {
     if (!busy) return;
@@ -170,13 +213,19 @@ __device__ __forceinline__ void skinny_product(const DirectMatrix& A, const Dire
   };
   auto products = [&](auto set, int buffer) {
     const char* at = smem + buffer * NB * kDirectHalf + lane * 16;
+    if (AT) turn(set);
 #pragma unroll
     for (int s = 0; s < 2; s++) {
-      float x[8];
-#pragma unroll
-      for (int c = 0; c < 8; c++) x[c] = av[decltype(set)::value][s * 2 + (c >> 2)][c & 3];
       b8 p[3];
-      three_parts(x, p);
+      if (AT) {
+#pragma unroll
+        for (int t = 0; t < 3; t++) p[t] = turned(s, t);
+      } else {
+        float x[8];
+#pragma unroll
+        for (int c = 0; c < 8; c++) x[c] = av[decltype(set)::value][s * 2 + (c >> 2)][c & 3];
+        three_parts(x, p);
+      }
 #pragma unroll
       for (int j = 0; j < NB; j++) {
         b8 y[3];
@@ -209,7 +258,7 @@ __device__ __forceinline__ void skinny_product(const DirectMatrix& A, const Dire
   lds_barrier();
   int s = 0;
   // B's step s is in buffer s % 2, A's steps s and s + 1 and B's step s + 1 are in registers or on their way
-  for (; s + 3 < (columns ? full : 0); s += 2) {
+  for (; s + 3 < (columns && (!AT || i0 + 32 <= A.rows) ? full : 0); s += 2) {   // as many barriers on either loop
     products(even, 0);
     fetch_a(even, all, 0);
     store_b(1);
