@@ -44,7 +44,8 @@ struct AdamwArgs {
   float decay[kTensors];
   double* steps;                    // b1^(t-1), b2^(t-1), t - 1, arrivals
   const float* lr_at;               // learning rate on the device, or null
-  float lr, beta1, beta2, eps;
+  double lr, beta1, beta2;
+  float eps;
   int32_t count;
   int32_t last;                     // the step's last launch counts it
 };
@@ -94,13 +95,16 @@ __device__ __forceinline__ uint32_t encode4(const float (&a)[4], float* scale) {
 #pragma unroll
   for (int c = 0; c < 4; c++) top = fmaxf(top, finite_or_zero(__builtin_fabsf(a[c])));
   top = dpp_max(top);
-  const float s = fmaxf(top / 448.0f, 1.17549435e-38f);
+  const float s = fmaxf(top * (1.0f / 448.0f), 1.17549435e-38f);
   *scale = s;
+  // a / s to the last bit for three operations: next to the border of two codes another rounding of the quotient is another
+  // code, which the following steps carry on
   const float up = 1.0f / s;
   float y[4];
 #pragma unroll
   for (int c = 0; c < 4; c++) {
-    y[c] = a[c] * up;
+    const float q = a[c] * up;
+    y[c] = __builtin_fmaf(__builtin_fmaf(-q, s, a[c]), up, q);
     y[c] = __builtin_fabsf(y[c]) < 512.0f ? y[c] : NAN;
   }
   int code = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
@@ -253,13 +257,13 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamwArgs<BITS> a) {
     at += __builtin_popcountll(__ballot(t + lane < a.count && a.first[t + lane < a.count ? t + lane : 0] <= blockIdx.x));
   at = __builtin_amdgcn_readfirstlane(at);
   AdamwTensor t{a.p[at], a.g[at], a.m[at], a.v[at], a.m_scale[BITS == 8 ? at : 0], a.r_scale[BITS == 8 ? at : 0], a.n[at], (blockIdx.x - a.first[at]) * (uint32_t)kAdamwChunk};
-  const float lr = a.lr_at ? a.lr_at[0] : a.lr;
+  const double lr = a.lr_at ? (double)a.lr_at[0] : a.lr;
   const float weight_decay = a.decay[at];
   // What the step's number gives, in binary64: b^t from the product that the states carry along.  The last workgroup to
   // have read it counts the step.
   if (threadIdx.x == 0) {
-    const double p1 = a.steps[0] * (double)a.beta1, p2 = a.steps[1] * (double)a.beta2;
-    numbers[0] = (float)((double)lr / (1.0 - p1));
+    const double p1 = a.steps[0] * a.beta1, p2 = a.steps[1] * a.beta2;
+    numbers[0] = (float)(lr / (1.0 - p1));
     numbers[1] = (float)(1.0 / __builtin_sqrt(1.0 - p2));
     if (a.last) {
       const double done = a.steps[2];
@@ -275,7 +279,7 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamwArgs<BITS> a) {
   }
   auto step = [&]() {
     __syncthreads();
-    return AdamwStep{1.0f - a.beta1, 1.0f - a.beta2, numbers[0], numbers[1], a.eps, lr * weight_decay};
+    return AdamwStep{(float)(1.0 - a.beta1), (float)(1.0 - a.beta2), numbers[0], numbers[1], a.eps, (float)lr * weight_decay};
   };
   // whole vectors of every stream, and a whole chunk
   const bool aligned = (((uintptr_t)t.p | (uintptr_t)t.g) & 15) == 0 &&
@@ -318,7 +322,7 @@ static int adamw_launches(const wf2hip_adamw_desc& d, long count, const wf2hip_a
     a.lr = d.lr;
     a.beta1 = d.beta1;
     a.beta2 = d.beta2;
-    a.eps = d.eps;
+    a.eps = (float)d.eps;
     a.last = i == count;
     adamw_kernel<BITS, NT><<<(uint32_t)blocks, kBlock, 0, rt().stream>>>(a);
     WF2_TRY(after_launch("adamw_kernel"));
@@ -335,7 +339,7 @@ WF2_API int wf2hip_adamw_step(const wf2hip_adamw_desc* d, long count, const wf2h
   WF2_TRY(require_init());
   if (!d || count < 0 || (count && !tensors) || !steps) return fail(WF2HIP_EINVAL, "%s: null pointer or negative count", name);
   if (d->state_bits != 8 && d->state_bits != 32) return fail(WF2HIP_EINVAL, "%s: states have 8 or 32 bits, not %d", name, d->state_bits);
-  if (!(d->beta1 >= 0.0f && d->beta1 < 1.0f && d->beta2 >= 0.0f && d->beta2 < 1.0f))
+  if (!(d->beta1 >= 0.0 && d->beta1 < 1.0 && d->beta2 >= 0.0 && d->beta2 < 1.0))
     return fail(WF2HIP_EINVAL, "%s: decay rates must be in [0, 1)", name);
   const bool bytes8 = d->state_bits == 8;
   try {

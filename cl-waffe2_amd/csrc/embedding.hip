@@ -52,10 +52,10 @@ __device__ __forceinline__ int32_t token_of(float id, int32_t vocab) {
 // The token table's part: the tokens are dealt out to `classes` classes by their low bits, and a workgroup of sixteen
 // wavefronts owns a class, hence every element it adds to.  It reads all ids (they stay in L2), keeps the rows of its
 // class in LDS in their order, sorts them by token (stable) and deals the sorted list out in equal runs to its
-// wavefronts, 64 vectors of the columns to each: a wavefront reads its rows eight at a time and touches the table once per token,
+// wavefronts, 64 vectors of the columns to each: a wavefront reads its rows eight or sixteen at a time and touches the table once per token,
 // however often that occurs; a token whose rows span several runs is put together from the wavefronts' parts in LDS.
-// (A text's most frequent word is a few per cent of it, a padded batch's padding most of it.)  The position table's part runs in
-// the same launch, a thread per vector.  Bound by HBM: dout once, and the rows of dwte it meets twice; short calls by
+// (A text's most frequent word is a few per cent of it, a padded batch's padding most of it.)  The position table's part is
+// dealt out to the same workgroups.  Bound by HBM: dout once, and the rows of dwte it meets twice; short calls by
 // the length of the chain ids -> rows -> table.
 constexpr int kGradBlock = 1024, kGradWaves = kGradBlock / kWave;
 constexpr int kGatherStep = 4 * kGradBlock;   // ids that a workgroup looks at at a time
@@ -70,6 +70,7 @@ struct EmbeddingGradient {
   int32_t vocab;
   uint32_t classes;       // a power of two
   int token_bits;         // bits of a token above those of its class
+  int shares;             // threads to a vector of the positions' part
 };
 
 struct GatherLds {
@@ -83,22 +84,24 @@ struct GatherLds {
 __device__ __forceinline__ void gather_sort(GatherLds& s, int count, uint32_t classes, int token_bits) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   if (count <= kRankMost) {
+    // four threads to an entry
+    static_assert(kRankMost * 4 == kGradBlock, "a thread for every quarter of an entry's comparisons");
     int rank = 0, row = 0, t = 0;
-    const int i = threadIdx.x;
+    const int i = threadIdx.x >> 2;
     if (i < count) {
       t = s.token[i];
       row = s.row[i];
-      int j = 0;
 #pragma unroll 4
-      for (; j + 3 < count; j += 4) {
-        const int4 u = *reinterpret_cast<const int4*>(s.token + j);
-        rank += (u.x < t || (u.x == t && j < i)) + (u.y < t || (u.y == t && j + 1 < i)) +
-                (u.z < t || (u.z == t && j + 2 < i)) + (u.w < t || (u.w == t && j + 3 < i));
+      for (int j = (threadIdx.x & 3) * 4; j < count; j += 16) {
+        const int4 u = *reinterpret_cast<const int4*>(s.token + j);   // what lies behind the list is not counted
+        rank += (u.x < t || (u.x == t && j < i)) + (j + 1 < count && (u.y < t || (u.y == t && j + 1 < i))) +
+                (j + 2 < count && (u.z < t || (u.z == t && j + 2 < i))) + (j + 3 < count && (u.w < t || (u.w == t && j + 3 < i)));
       }
-      for (; j < count; j++) rank += s.token[j] < t || (s.token[j] == t && j < i);
     }
+    rank += __shfl_xor(rank, 1);
+    rank += __shfl_xor(rank, 2);
     __syncthreads();
-    if (i < count) {
+    if (i < count && (threadIdx.x & 3) == 0) {
       s.row[rank] = row;
       s.token[rank] = t;
     }
@@ -155,21 +158,8 @@ template <bool VEC>
 __global__ __launch_bounds__(kGradBlock) void embedding_gradient_kernel(EmbeddingGradient p) {
   typedef float fv __attribute__((ext_vector_type(VEC ? 4 : 1)));
   constexpr int V = VEC ? 4 : 1;
-  constexpr int kBatch = 8;
+  constexpr int kBatch = 8, kDeep = 16;
   const int64_t per_row = p.dim / V;   // vectors of a row
-  if (blockIdx.x >= p.classes) {
-    // positions: vector i of dwpe's first seq rows
-    const int64_t i = (int64_t)(blockIdx.x - p.classes) * kGradBlock + threadIdx.x;
-    if (i >= p.seq * per_row) return;
-    const int64_t step = p.seq * p.dim;
-    const float* q = p.dout + i * V;
-    fv sum = *reinterpret_cast<const fv*>(q);
-#pragma unroll 4
-    for (int64_t n = step; n < p.rows * p.dim; n += step) sum += *reinterpret_cast<const fv*>(q + n);
-    fv* out = reinterpret_cast<fv*>(p.dwpe + i * V);
-    *out = *out + sum;
-    return;
-  }
   __shared__ GatherLds s;
   __shared__ fv part[kGradWaves][2][kWave];   // sums of tokens whose rows began before a wavefront's run, or go on behind it
   const uint32_t mine = blockIdx.x;
@@ -189,6 +179,30 @@ __global__ __launch_bounds__(kGradBlock) void embedding_gradient_kernel(Embeddin
   };
   int64_t next = 0;   // rows looked at so far
   fetch(0);
+  // This workgroup's share of the positions: vectors of dwpe's first seq rows, `shares` threads to a vector (many short
+  // sentences), whose sums meet in LDS.
+  fv* meet = &part[0][0][0];
+  const int vecs = kGradBlock / p.shares, mine_of = threadIdx.x / vecs;
+  for (int64_t first = (int64_t)blockIdx.x * vecs; first < p.seq * per_row; first += (int64_t)p.classes * vecs) {
+    const int64_t i = first + threadIdx.x % vecs;
+    const int64_t step = p.seq * p.dim;
+    fv sum = {};
+    if (i < p.seq * per_row) {
+      const float* q = p.dout + i * V;
+#pragma unroll 8
+      for (int64_t n = mine_of * step; n < p.rows * p.dim; n += p.shares * step) sum += *reinterpret_cast<const fv*>(q + n);
+    }
+    if (p.shares > 1) {
+      meet[threadIdx.x] = sum;
+      __syncthreads();
+      for (int w = 1; w < p.shares && mine_of == 0; w++) sum += meet[w * vecs + threadIdx.x];
+      __syncthreads();
+    }
+    if (mine_of == 0 && i < p.seq * per_row) {
+      fv* out = reinterpret_cast<fv*>(p.dwpe + i * V);
+      *out = *out + sum;
+    }
+  }
   while (next < p.rows) {
     // keep rows of this class while another step's fit
     int count = 0;
@@ -239,18 +253,28 @@ __global__ __launch_bounds__(kGradBlock) void embedding_gradient_kernel(Embeddin
         bool lead = same(e0);   // the run's first token began before it
         fv sum = {}, table = {};
         int32_t of = 0;
-        // Eight rows, and the table's rows they go to, at a time: the loads carry no test (rows behind the run are its
-        // last one again), so that all of them are in flight before the first addition.
-        for (int e = e0; e < e1; e += kBatch) {
-          const int at = e + (lane & (kBatch - 1));
-          const int at8 = at < e1 ? at : e1 - 1;
-          const int32_t rows8 = s.row[at8], tokens8 = s.token[at8];
-          const uint64_t heads = __ballot(at < e1 && (at8 == e0 || s.token[at8 ? at8 - 1 : 0] != tokens8));
+        // The loads carry no test (rows behind the run are its last one again), so that all of a batch are in flight before
+        // its first addition: sixteen rows of one token, or eight rows and the table's rows they go to.
+        for (int e = e0; e < e1;) {
+          const int at = e + (lane & (kDeep - 1));
+          const int clamped = at < e1 ? at : e1 - 1;
+          const int32_t rows = s.row[clamped], tokens = s.token[clamped];
+          const uint64_t heads = __ballot(at < e1 && (clamped == e0 || s.token[clamped ? clamped - 1 : 0] != tokens));
+          if ((heads & ((1u << kDeep) - 1)) == 0 && e + kDeep <= e1) {
+            fv r[kDeep];
+#pragma unroll
+            for (int u = 0; u < kDeep; u++)
+              r[u] = *reinterpret_cast<const fv*>(p.dout + (int64_t)__builtin_amdgcn_readlane(rows, u) * p.dim + c);
+#pragma unroll
+            for (int u = 0; u < kDeep; u++) sum += r[u];
+            e += kDeep;
+            continue;
+          }
           fv r[kBatch], t[kBatch];
 #pragma unroll
           for (int u = 0; u < kBatch; u++) {
-            r[u] = *reinterpret_cast<const fv*>(p.dout + (int64_t)__builtin_amdgcn_readlane(rows8, u) * p.dim + c);
-            t[u] = *reinterpret_cast<const fv*>(p.dwte + (int64_t)__builtin_amdgcn_readlane(tokens8, u) * p.dim + c);
+            r[u] = *reinterpret_cast<const fv*>(p.dout + (int64_t)__builtin_amdgcn_readlane(rows, u) * p.dim + c);
+            t[u] = *reinterpret_cast<const fv*>(p.dwte + (int64_t)__builtin_amdgcn_readlane(tokens, u) * p.dim + c);
           }
 #pragma unroll
           for (int u = 0; u < kBatch; u++) {
@@ -267,10 +291,11 @@ __global__ __launch_bounds__(kGradBlock) void embedding_gradient_kernel(Embeddin
               } else {
                 sum += r[u];
               }
-              of = __builtin_amdgcn_readlane(tokens8, u);
+              of = __builtin_amdgcn_readlane(tokens, u);
               table = t[u];
             }
           }
+          e += kBatch;
         }
         if (lead)
           part[wave][0][lane] = sum;
@@ -347,16 +372,14 @@ WF2_API int wf2hip_embedding_gradient_f32(long rows, long seq, long dim, const f
       if (meet(o, i)) return fail(WF2HIP_EOVERLAP, "%s: a table's gradient overlaps an input", name);
   if (meet(out[0], out[1])) return fail(WF2HIP_EOVERLAP, "%s: the tables' gradients overlap", name);
   const bool vec = dim % 4 == 0 && ((uintptr_t)dout | (uintptr_t)dwte | (uintptr_t)dwpe) % 16 == 0;
-  const int64_t per_row = vec ? dim / 4 : dim;
-  EmbeddingGradient p{ctx, dout, dwte, dwpe, rows, seq, dim, (int32_t)vocab, 1, 0};
+  EmbeddingGradient p{ctx, dout, dwte, dwpe, rows, seq, dim, (int32_t)vocab, 1, 0, 1};
   // about sixteen rows to a class, at most a class per compute unit: every workgroup reads all the ids
   while (p.classes < 256 && (int64_t)p.classes * 16 < rows) p.classes *= 2;
   while (((int64_t)p.classes << p.token_bits) < vocab) p.token_bits++;
-  const int64_t positions = ceil_div((int64_t)seq * per_row, kGradBlock), blocks = (int64_t)p.classes + positions;
-  if (blocks >= ((int64_t)1 << 31)) return fail(WF2HIP_EUNSUPPORTED, "%s: too many elements for one launch", name);
+  while (p.shares < 16 && (int64_t)p.shares * 16 * seq < rows) p.shares *= 2;   // at most sixteen sentences to a thread
   if (vec)
-    embedding_gradient_kernel<true><<<(uint32_t)blocks, kGradBlock, 0, rt().stream>>>(p);
+    embedding_gradient_kernel<true><<<p.classes, kGradBlock, 0, rt().stream>>>(p);
   else
-    embedding_gradient_kernel<false><<<(uint32_t)blocks, kGradBlock, 0, rt().stream>>>(p);
+    embedding_gradient_kernel<false><<<p.classes, kGradBlock, 0, rt().stream>>>(p);
   return after_launch("embedding_gradient_kernel");
 }

@@ -250,6 +250,7 @@ struct XentLoss {
   const int32_t* labels;
   long rows, vocab;
   uint32_t tiles_m, tiles_n;
+  int width;               // rows of x in a tile: 256, or less where that leaves the device empty
   float2* part;            // [tile of the vocabulary][row]: maximum, sum of exp(s - maximum)
   float* at;               // [row] the label's logit
 };
@@ -262,7 +263,7 @@ __device__ __forceinline__ void fold_in(float& top, float& sum, float2 a) {
   top = both;
 }
 
-// A tile of 128 words x 256 rows of x: a lane of the accumulators holds 32 words of one row of x, so that maxima and sums
+// A tile of 128 words x 64 NB rows of x: a lane of the accumulators holds 32 words of one row of x, so that maxima and sums
 // run along registers.
 template <int NB>
 __device__ __forceinline__ void tile_loss(const XentLoss& p, uint32_t tm, int64_t m0, int64_t n0, char* smem) {
@@ -332,17 +333,18 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
   uint32_t tm, tn;
   pair_tile(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
-  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
-  if (p.rows - n0 > 128)
+  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * p.width;
+  const int64_t rest = p.rows - n0 < p.width ? p.rows - n0 : p.width;
+  if (rest > 128)
     tile_loss<4>(p, tm, m0, n0, smem);
-  else if (p.rows - n0 > 64)
+  else if (rest > 64)
     tile_loss<2>(p, tm, m0, n0, smem);
   else
     tile_loss<1>(p, tm, m0, n0, smem);
 }
 
 // The tiles' maxima and sums of a row.  MANY rows: 64 to a workgroup, a lane each, sixteen wavefronts taking every sixteenth
-// tile and meeting in LDS; few rows: a workgroup to each, a thread to every 256th tile (rows 61, 786 tiles: 20 -> FOLD us).
+// tile and meeting in LDS; few rows: a workgroup to each, a thread to every 256th tile (61 rows, 786 tiles: 20 -> 4.5 us).
 // With a reduction the workgroup that arrives last adds up the workgroups' shares in their order.
 constexpr int kFoldRows = 2048;   // up to here a workgroup per row
 template <bool MANY>
@@ -416,11 +418,13 @@ struct XentGradient {
   long rows, dim;
   long first, words;       // the piece
   uint32_t tiles_m, tiles_n;           // of ds
+  int width;                           // as XentLoss
   uint32_t tiles_w, tiles_x, tiles_d;  // of 128 words, 128 rows of x, 256 columns
-  uint32_t shares;                     // dx: shares of the piece's K, of `split` K steps
-  int split, steps_dx, steps_dw;
+  uint32_t shares_x, shares_w;         // of the products' K, of split_x / split_w K steps
+  int split_x, split_w, steps_x, steps_w;
   bool dw_first;
-  float *planes, *dw;                  // dx's planes from this piece's first on, the piece's rows of dw
+  float *planes;                       // dx's planes from this piece's first on
+  float *dw;                           // the piece's rows of dw, or (several shares) its planes
 };
 
 constexpr float kLoud = 32768.0f;   // ds is held times 2^15: at most 1 before
@@ -470,10 +474,11 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
   uint32_t tm, tn;
   pair_tile(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
-  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
-  if (p.rows - n0 > 128)
+  const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * p.width;
+  const int64_t rest = p.rows - n0 < p.width ? p.rows - n0 : p.width;
+  if (rest > 128)
     tile_ds<4>(p, m0, n0, smem);
-  else if (p.rows - n0 > 64)
+  else if (rest > 64)
     tile_ds<2>(p, m0, n0, smem);
   else
     tile_ds<1>(p, m0, n0, smem);
@@ -482,8 +487,8 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
 // A share of K of dx: plane `share` of p.planes, (rows, dim), unscaled.
 template <int NB>
 __device__ __forceinline__ void tile_dx(const XentGradient& p, uint32_t share, int64_t m0, int64_t n0, char* smem) {
-  const int64_t s0 = (int64_t)share * p.split;
-  const int steps = p.steps_dx - s0 < p.split ? (int)(p.steps_dx - s0) : p.split;
+  const int64_t s0 = (int64_t)share * p.split_x;
+  const int steps = p.steps_x - s0 < p.split_x ? (int)(p.steps_x - s0) : p.split_x;
   f16v acc[2][NB];
   pair_product<false, true, true, NB>(p.ds, p.w, m0, n0, s0 * 16, steps, smem, acc);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
@@ -503,14 +508,18 @@ __device__ __forceinline__ void tile_dx(const XentGradient& p, uint32_t share, i
   }
 }
 
-// The piece's rows of dw.
+// The piece's rows of dw; with several shares of K a plane of them each, unscaled.
 template <int NB>
-__device__ __forceinline__ void tile_dw(const XentGradient& p, int64_t m0, int64_t n0, char* smem) {
+__device__ __forceinline__ void tile_dw(const XentGradient& p, uint32_t share, int64_t m0, int64_t n0, char* smem) {
+  const int64_t s0 = (int64_t)share * p.split_w;
+  const int steps = p.steps_w - s0 < p.split_w ? (int)(p.steps_w - s0) : p.split_w;
   f16v acc[2][NB];
-  pair_product<true, true, true, NB>(p.ds, p.x, m0, n0, 0, p.steps_dw, smem, acc);
+  pair_product<true, true, true, NB>(p.ds, p.x, m0, n0, s0 * 16, steps, smem, acc);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
-  const int down = p.head->eg - 15 - p.head->ex;
-  const float alpha = p.head->alpha;
+  const bool plane = p.shares_w > 1;
+  const int down = plane ? 0 : p.head->eg - 15 - p.head->ex;
+  const float alpha = plane ? 1.0f : p.head->alpha;
+  float* out = p.dw + (int64_t)share * p.words * p.dim;
 #pragma unroll
   for (int j = 0; j < NB; j++) {
     const int64_t d = n0 + (wave & 1) * 32 * NB + j * 32 + (lane & 31);
@@ -521,40 +530,38 @@ __device__ __forceinline__ void tile_dw(const XentGradient& p, int64_t m0, int64
         for (int r = 0; r < 16; r++) {
           const int64_t v = m0 + (wave >> 1) * 64 + i * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
           const float a = __builtin_ldexpf(acc[i][j][r], down);
-          if (v < p.words) p.dw[v * p.dim + d] = a == 0.0f ? 0.0f : a * alpha;
+          if (v < p.words) out[v * p.dim + d] = a == 0.0f ? 0.0f : a * alpha;
         }
     }
   }
 }
 
 // Both products of a piece in one launch, so that neither has a last round of its own: the tiles with the longer K first
-// (dw's K are the rows of x, dx's a share of the words).  A tile that overhangs the columns by more than half runs as a
+// (dw's K are the rows of x, dx's the words; either in shares where there are few tiles).  A tile that overhangs the columns by more than half runs as a
 // narrower one.
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_gradients(XentGradient p) {
   __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
   const uint32_t dw_tiles = p.tiles_w * p.tiles_d, dx_tiles = p.tiles_x * p.tiles_d;
   uint32_t id = blockIdx.x;
   // the second kind begins at a multiple of 8 workgroups, where the XCDs' round robin begins anew
-  const uint32_t first = p.dw_first ? dw_tiles : dx_tiles * p.shares, behind = (first + 7) & ~7u;
+  const uint32_t first = p.dw_first ? dw_tiles * p.shares_w : dx_tiles * p.shares_x, behind = (first + 7) & ~7u;
   const bool of_first = id < behind;
   if (of_first && id >= first) return;
   if (!of_first) id -= behind;
   const bool dw = of_first == p.dw_first;
-  uint32_t tm, tn, share = 0;
-  if (!dw) {
-    share = id / dx_tiles;
-    id -= share * dx_tiles;
-  }
+  uint32_t tm, tn;
+  const uint32_t tiles = dw ? dw_tiles : dx_tiles, share = id / tiles;
+  id -= share * tiles;
   pair_tile(id, dw ? p.tiles_w : p.tiles_x, p.tiles_d, &tm, &tn);
   const int64_t m0 = (int64_t)tm * kTileM, n0 = (int64_t)tn * kTileN;
   const int64_t rest = p.dim - n0;
   if (dw) {
     if (rest > 128)
-      tile_dw<4>(p, m0, n0, smem);
+      tile_dw<4>(p, share, m0, n0, smem);
     else if (rest > 64)
-      tile_dw<2>(p, m0, n0, smem);
+      tile_dw<2>(p, share, m0, n0, smem);
     else
-      tile_dw<1>(p, m0, n0, smem);
+      tile_dw<1>(p, share, m0, n0, smem);
   } else {
     if (rest > 128)
       tile_dx<4>(p, share, m0, n0, smem);
@@ -565,24 +572,39 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   }
 }
 
-// dx <- the planes' sum, scaled; rows without a label are zero whatever the common factor is
+// dx and, where it is in planes too, dw of a piece: the planes' sums, scaled.  Rows of dx without a label are zero whatever the
+// common factor is.
+struct XentPlanes {
+  int64_t n;            // elements of a plane
+  int planes;
+  const float* part;
+  float* out;
+};
 template <bool VEC>
-__global__ __launch_bounds__(kBlock) void xent_fold_dx(int64_t n, long dim, int planes, const float* __restrict__ part,
-                                                       const float* __restrict__ g, const XentHead* __restrict__ head,
-                                                       float* __restrict__ dx) {
+__global__ __launch_bounds__(kBlock) void xent_fold_gradients(XentPlanes x, XentPlanes w, uint32_t x_groups, long dim,
+                                                              const float* __restrict__ g, const XentHead* __restrict__ head) {
   typedef float fv __attribute__((ext_vector_type(VEC ? 4 : 1)));
   constexpr int V = VEC ? 4 : 1;
-  const int64_t i = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * V;
+  const bool of_x = blockIdx.x < x_groups;
+  const int64_t n = of_x ? x.n : w.n;
+  const int planes = of_x ? x.planes : w.planes;
+  const float* part = of_x ? x.part : w.part;
+  const int64_t i = ((int64_t)(of_x ? blockIdx.x : blockIdx.x - x_groups) * kBlock + threadIdx.x) * V;
   if (i >= n) return;
   fv sum = *reinterpret_cast<const fv*>(part + i);
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 1; s < planes; s++) sum += *reinterpret_cast<const fv*>(part + s * n + i);
-  const int down = head->eg - 15 - head->ew;
-  const float alpha = head->alpha;
-  const bool none = g[i / dim] == 0.0f;   // a vector lies within a row
+  if (head) {
+    const int down = head->eg - 15 - (of_x ? head->ew : head->ex);
+    const float alpha = head->alpha;
+    const bool none = of_x && g[i / dim] == 0.0f;   // a vector lies within a row
 #pragma unroll
-  for (int c = 0; c < V; c++) sum[c] = none ? 0.0f : __builtin_ldexpf(sum[c], down) * alpha;
-  *reinterpret_cast<fv*>(dx + i) = sum;
+    for (int c = 0; c < V; c++) {
+      const float a = __builtin_ldexpf(sum[c], down);
+      sum[c] = none || a == 0.0f ? 0.0f : a * alpha;
+    }
+  }
+  *reinterpret_cast<fv*>((of_x ? x.out : w.out) + i) = sum;
 }
 
 // ---- straight from binary32: few rows, small products -----------------------------------------------------------
@@ -602,11 +624,11 @@ struct XentDirect {
   float scale;
   float* ds;                   // (vocab, pitch)
   int64_t pitch;
-  uint32_t tiles_dw;           // dw: columns of x
+  uint32_t tiles_dw, tiles_vw; // dw: columns of x, words
   uint32_t tiles_dx, tiles_nx; // dx: columns, rows of x
   uint32_t dw_units, dx_units; // workgroups of either
-  int64_t share;               // words of a share of dx's K
-  float *dx, *dw;              // dx: a plane per share
+  int64_t share_x, share_w;    // words of a share of dx's K, rows of x of a share of dw's
+  float *dx, *dw;              // a plane per share
 };
 
 // A tile of 128 words x 32 NB rows of x.
@@ -815,15 +837,18 @@ __global__ __launch_bounds__(kBlock) void xent_small_gradients(XentDirect p) {
   __shared__ __attribute__((aligned(16))) char smem[kSmallLds<NBX>];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
   if (blockIdx.x < p.dw_units) {
-    const uint32_t td = blockIdx.x % p.tiles_dw, tv = blockIdx.x / p.tiles_dw;
+    const uint32_t td = blockIdx.x % p.tiles_dw, rest = blockIdx.x / p.tiles_dw;
+    const uint32_t tv = rest % p.tiles_vw, share = rest / p.tiles_vw;
     const int64_t m0 = (int64_t)tv * 32, d = (int64_t)td * 32 + (lane & 31);
+    const int64_t k0 = share * p.share_w, k1 = k0 + p.share_w < p.rows ? k0 + p.share_w : p.rows;
     float s[1][4];
     small_product<1, false, true>(DirectMatrix{p.ds, p.pitch, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.dim, p.labels}, m0,
-                                  (int64_t)td * 32, 0, p.rows, smem, s);
+                                  (int64_t)td * 32, k0, k1, smem, s);
+    float* out = p.dw + (int64_t)share * p.vocab * p.dim;
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       const int64_t v = m0 + wave * 8 + h * 4 + c;
-      if (v < p.vocab && d < p.dim) p.dw[v * p.dim + d] = s[0][c];
+      if (v < p.vocab && d < p.dim) out[v * p.dim + d] = s[0][c];
     }
     return;
   }
@@ -831,7 +856,7 @@ __global__ __launch_bounds__(kBlock) void xent_small_gradients(XentDirect p) {
   const uint32_t td = unit % p.tiles_dx, rest = unit / p.tiles_dx;
   const uint32_t tn = rest % p.tiles_nx, share = rest / p.tiles_nx;
   const int64_t d0 = (int64_t)td * 32, n0 = (int64_t)tn * 32 * NBX;
-  const int64_t k0 = share * p.share, k1 = k0 + p.share < p.vocab ? k0 + p.share : p.vocab;
+  const int64_t k0 = share * p.share_x, k1 = k0 + p.share_x < p.vocab ? k0 + p.share_x : p.vocab;
   float s[NBX][4];
   small_product<NBX, true, true>(DirectMatrix{p.w, p.dim, p.dim, nullptr}, DirectMatrix{p.ds, p.pitch, p.rows, nullptr}, d0, n0, k0, k1,
                                  smem, s);
@@ -857,11 +882,14 @@ __global__ __launch_bounds__(kBlock) void xent_direct_gradients(XentDirect p) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, h = lane >> 5;
   if (blockIdx.x >= p.dx_units) {
     const uint32_t unit = blockIdx.x - p.dx_units;
-    const uint32_t td = unit % p.tiles_dw, tv = unit / p.tiles_dw;
+    const uint32_t td = unit % p.tiles_dw, rest = unit / p.tiles_dw;
+    const uint32_t tv = rest % p.tiles_vw, share = rest / p.tiles_vw;
     const int64_t m0 = (int64_t)tv * kSkinnyRows, d0 = (int64_t)td * 32 * NBW;
+    const int64_t k0 = share * p.share_w, K = (k0 + p.share_w < p.rows ? k0 + p.share_w : p.rows) - k0;
     f16v acc[NBW];
-    skinny_product<NBW, false, true>(DirectMatrix{p.ds, p.pitch, p.vocab, nullptr}, DirectMatrix{p.x, p.dim, p.dim, p.labels}, m0, d0,
-                                     p.rows, smem, acc);
+    skinny_product<NBW, false, true>(DirectMatrix{p.ds + k0, p.pitch, p.vocab, nullptr},
+                                     DirectMatrix{p.x + k0 * p.dim, p.dim, p.dim, p.labels + k0}, m0, d0, K, smem, acc);
+    float* out = p.dw + (int64_t)share * p.vocab * p.dim;
 #pragma unroll
     for (int j = 0; j < NBW; j++) {
       const int64_t d = d0 + j * 32 + (lane & 31);
@@ -869,7 +897,7 @@ __global__ __launch_bounds__(kBlock) void xent_direct_gradients(XentDirect p) {
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           const int64_t v = m0 + wave * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
-          if (v < p.vocab) p.dw[v * p.dim + d] = acc[j][r];
+          if (v < p.vocab) out[v * p.dim + d] = acc[j][r];
         }
       }
     }
@@ -878,7 +906,7 @@ __global__ __launch_bounds__(kBlock) void xent_direct_gradients(XentDirect p) {
   const uint32_t td = blockIdx.x % p.tiles_dx, rest = blockIdx.x / p.tiles_dx;
   const uint32_t tn = rest % p.tiles_nx, share = rest / p.tiles_nx;
   const int64_t d0 = (int64_t)td * kSkinnyRows, n0 = (int64_t)tn * 32 * NBX;
-  const int64_t k0 = share * p.share, K = (k0 + p.share < p.vocab ? k0 + p.share : p.vocab) - k0;
+  const int64_t k0 = share * p.share_x, K = (k0 + p.share_x < p.vocab ? k0 + p.share_x : p.vocab) - k0;
   f16v acc[NBX];
   skinny_product<NBX, true, true>(DirectMatrix{p.w + k0 * p.dim, p.dim, p.dim, nullptr},
                                   DirectMatrix{p.ds + k0 * p.pitch, p.pitch, p.rows, nullptr}, d0, n0, K, smem, acc);
@@ -894,17 +922,6 @@ __global__ __launch_bounds__(kBlock) void xent_direct_gradients(XentDirect p) {
       }
     }
   }
-}
-
-// dx <- the planes' sum
-__global__ __launch_bounds__(kBlock) void xent_direct_fold(int64_t n, int planes, const float* __restrict__ part,
-                                                           float* __restrict__ dx) {
-  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (i >= n) return;
-  float sum = part[i];
-#pragma unroll 8
-  for (int s = 1; s < planes; s++) sum += part[s * n + i];
-  dx[i] = sum;
 }
 
 // Tiles times rows up to which the last workgroup finishes a small call.
@@ -951,6 +968,14 @@ static PairMatrix pair_matrix(const char* base, int64_t rows, int64_t cols) {
 }
 static int64_t pair_bytes(const PairMatrix& m) { return m.row_blocks * m.pitch(); }
 
+// Rows of x in a tile of logits: 256 where that gives every compute unit two tiles, else 128 or 64 (loss of 256 x 768 x 8192:
+// 54 -> 37 us).
+static int xent_width(int64_t tiles_m, int64_t rows) {
+  for (int width = kTileN; width > 64; width /= 2)
+    if (tiles_m * ceil_div(rows, width) >= 2 * rt().num_cus) return width;
+  return 64;
+}
+
 // Words of a piece of the backward: ds (4 bytes per row of x and word) takes at most 1 GiB, in pieces of equal size.
 static int64_t xent_words(int64_t rows, int64_t vocab) {
   const int64_t padded = ceil_div(rows, kTileN) * kTileN;
@@ -958,6 +983,19 @@ static int64_t xent_words(int64_t rows, int64_t vocab) {
   if (fit < 1) fit = 1;
   const int64_t tiles = ceil_div(vocab, kTileM), pieces = ceil_div(tiles, fit);
   return ceil_div(tiles, pieces) * kTileM;
+}
+
+// The planes' sums of both gradients in one launch; n 0: that one is not in planes.
+static int fold_gradients(const XentPlanes& x, const XentPlanes& w, int64_t dim, const float* g, const XentHead* head, hipStream_t st) {
+  const bool vec = dim % 4 == 0 && ((uintptr_t)x.out | (uintptr_t)w.out) % 16 == 0;
+  const int64_t per = vec ? 4 : 1, gx = ceil_div(x.n / per, kBlock), gw = ceil_div(w.n / per, kBlock);
+  if (gx + gw == 0) return 0;
+  if (gx + gw >= ((int64_t)1 << 31)) return fail(WF2HIP_EUNSUPPORTED, "linear cross entropy backward: too many elements for one launch");
+  if (vec)
+    xent_fold_gradients<true><<<(uint32_t)(gx + gw), kBlock, 0, st>>>(x, w, (uint32_t)gx, dim, g, head);
+  else
+    xent_fold_gradients<false><<<(uint32_t)(gx + gw), kBlock, 0, st>>>(x, w, (uint32_t)gx, dim, g, head);
+  return after_launch("xent_fold_gradients");
 }
 
 // Which route a call takes.
@@ -972,8 +1010,15 @@ static XentRoute xent_route(int64_t rows, int64_t dim, int64_t vocab, bool backw
   if (!fits) return kPairs;
   if (const char* env = getenv("WF2HIP_XENT_ROUTE"))
     if (env[0] >= '0' && env[0] <= '2') return (XentRoute)(env[0] - '0');
-  if (rows > 256 && rows * dim * vocab > ((int64_t)1 << 30)) return kPairs;
-  return ceil_div(vocab, kSkinnyRows) * ceil_div(rows, 128) >= rt().num_cus ? kSkinny : kSmall;
+  // Measured (us, kPairs / kSkinny / kSmall; rows x dim x vocab):
+  //   forward   256 x 768 x 1000  48 / 46 / 17    1000 x 400 x 2000 24 / 34 / 25    256 x 768 x 8192  37 / 50 / 46
+  //             16 x 1600 x 20000 98 / 56 / 37    61 x 768 x 50257  88 / 53 / 73    128 x 768 x 50257 102 / 85 / 129
+  //             256 x 768 x 50257 123 / 143 / 213
+  //   backward  256 x 768 x 1000  92 / 83 / 53    400 x 200 x 3000  78 / 94 / 75    1000 x 400 x 2000 86 / 105 / 154
+  //             16 x 1600 x 20000 198 / 149 / 263 61 x 768 x 50257  240 / 208 / 676 64 x 768 x 8192   61 / 70 / 117
+  const int64_t work = rows * dim * vocab;
+  if (work <= (backward ? (int64_t)1 << 28 : (int64_t)3 << 28)) return kSmall;
+  return backward ? (rows <= 64 && vocab * dim >= ((int64_t)1 << 24) ? kSkinny : kPairs) : rows <= 160 ? kSkinny : kPairs;
 }
 
 // Width of a tile in blocks of 32: no wider than the operand, `most` where that is longer.
@@ -983,7 +1028,7 @@ static int xent_blocks(int64_t extent, int most) { return extent <= 32 ? 1 : ext
 static bool xent_wide_gradients(XentRoute route, int64_t rows, int64_t dim, int64_t vocab) {
   if (const char* env = getenv("WF2HIP_XENT_ROUTE"))
     if (env[0] == '1' || env[0] == '2') return env[0] == '1';
-  return route == kSkinny || ceil_div(vocab, kSkinnyRows) * ceil_div(dim, 128) >= 128;
+  return route == kSkinny;
 }
 
 static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int64_t vocab, const float* x, const float* w,
@@ -1008,24 +1053,29 @@ static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int6
   p.mean = reduction == WF2HIP_REDUCE_MEAN;
   p.scale = scale;
   p.pitch = ceil_div(rows, 32) * 32;
-  // shares of dx's K: enough workgroups to fill the device four times, of at least eight K steps
-  const int64_t dx_tiles = (int64_t)p.tiles_nx * p.tiles_dx, all_steps = ceil_div(vocab, kDirectStep);
-  int64_t shares = ceil_div(4 * rt().num_cus, dx_tiles);
-  if (shares > all_steps / 8) shares = all_steps / 8;
-  if (shares < 1) shares = 1;
-  p.share = ceil_div(all_steps, shares) * kDirectStep;
-  shares = ceil_div(vocab, p.share);
-  const int64_t dw_units = ceil_div(vocab, wide ? kSkinnyRows : 32) * p.tiles_dw, most = ((int64_t)1 << 31) - 1;
-  if (dw_units + dx_tiles * shares > most || (int64_t)p.tiles_v * p.tiles_n > most)
+  p.tiles_vw = (uint32_t)ceil_div(vocab, wide ? kSkinnyRows : 32);
+  // shares of either product's K: enough workgroups to fill the device four times, of at least eight K steps
+  auto share_of = [&](int64_t tiles, int64_t K) {
+    const int64_t steps = ceil_div(K, kDirectStep);
+    int64_t shares = ceil_div(4 * rt().num_cus, tiles);
+    if (shares > steps / 8) shares = steps / 8;
+    return ceil_div(steps, shares < 1 ? 1 : shares) * kDirectStep;
+  };
+  const int64_t dx_tiles = (int64_t)p.tiles_nx * p.tiles_dx, dw_tiles = (int64_t)p.tiles_vw * p.tiles_dw;
+  p.share_x = share_of(dx_tiles, vocab);
+  p.share_w = share_of(dw_tiles, rows);
+  const int64_t shares_x = ceil_div(vocab, p.share_x), shares_w = ceil_div(rows, p.share_w), most = ((int64_t)1 << 31) - 1;
+  if (dw_tiles * shares_w + dx_tiles * shares_x > most || (int64_t)p.tiles_v * p.tiles_n > most)
     return fail(WF2HIP_EUNSUPPORTED, "linear cross entropy backward: too many tiles for one launch");
-  p.dw_units = (uint32_t)dw_units;
-  p.dx_units = (uint32_t)(dx_tiles * shares);
+  p.dw_units = (uint32_t)(dw_tiles * shares_w);
+  p.dx_units = (uint32_t)(dx_tiles * shares_x);
   Blocks blocks;
+  const int64_t nx = rows * dim, nw = vocab * dim;
   p.ds = blocks.take<float>(vocab * p.pitch * 4);
-  p.dx = shares > 1 ? blocks.take<float>(shares * rows * dim * 4) : dx;
-  p.dw = dw;
+  p.dx = shares_x > 1 ? blocks.take<float>(shares_x * nx * 4) : dx;
+  p.dw = shares_w > 1 ? blocks.take<float>(shares_w * nw * 4) : dw;
   WF2_TRY(blocks.rc);
-  const uint32_t tiles = p.tiles_v * p.tiles_n, units = (uint32_t)(dw_units + dx_tiles * shares);
+  const uint32_t tiles = p.tiles_v * p.tiles_n, units = p.dw_units + p.dx_units;
   if (small)
     nb == 1 ? xent_small_ds<1><<<tiles, kBlock, 0, st>>>(p) : xent_small_ds<2><<<tiles, kBlock, 0, st>>>(p);
   else if (nb == 4)
@@ -1049,9 +1099,8 @@ static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int6
       nbw == 1 ? with(std::integral_constant<int, 1>()) : with(std::integral_constant<int, 2>());
   }
   WF2_TRY(after_launch("xent_direct_gradients"));
-  if (shares == 1) return 0;
-  xent_direct_fold<<<(uint32_t)ceil_div(rows * dim, kBlock), kBlock, 0, st>>>(rows * dim, (int)shares, p.dx, dx);
-  return after_launch("xent_direct_fold");
+  return fold_gradients(XentPlanes{shares_x > 1 ? nx : 0, (int)shares_x, p.dx, dx}, XentPlanes{shares_w > 1 ? nw : 0, (int)shares_w, p.dw, dw},
+                        dim, nullptr, nullptr, st);
 }
 
 template <bool PER_ROW>
@@ -1089,9 +1138,10 @@ WF2_API int wf2hip_linear_cross_entropy_f32(long rows, long dim, long vocab, con
   if (rows == 0) return each ? 0 : wf2hip_fill_f32(loss, 1, reduction == WF2HIP_REDUCE_MEAN ? NAN : 0.0f);
   Blocks blocks;
   const XentRoute route = xent_route(rows, dim, vocab, false);
-  const int nb = route == kPairs ? kTileN / 32 : xent_blocks(rows, route == kSmall ? 2 : 4);
   static_assert(kTileM == kSkinnyRows, "one height of tiles on both routes");
-  const int64_t tiles_v = ceil_div(vocab, route == kSmall ? 32 : kTileM), tiles_n = ceil_div(rows, 32 * nb);
+  const int64_t tiles_v = ceil_div(vocab, route == kSmall ? 32 : kTileM);
+  const int nb = route == kPairs ? xent_width(tiles_v, rows) / 32 : xent_blocks(rows, route == kSmall ? 2 : 4);
+  const int64_t tiles_n = ceil_div(rows, 32 * nb);
   if (tiles_v * tiles_n >= ((int64_t)1 << 31)) return fail(WF2HIP_EUNSUPPORTED, "%s: too many tiles for one launch", name);
   const uint32_t folds = (uint32_t)(rows <= kFoldRows ? rows : ceil_div(rows, kWave));
   const bool one_launch = route == kSmall && tiles_v * rows <= kLastMost;
@@ -1141,6 +1191,7 @@ WF2_API int wf2hip_linear_cross_entropy_f32(long rows, long dim, long vocab, con
     p.x_exponents = (int64_t)p.w.row_blocks * 32;
     p.labels = labels;
     p.rows = rows; p.vocab = vocab;
+    p.width = 32 * nb;
     p.part = part; p.at = at;
     xent_tile_loss<<<p.tiles_m * p.tiles_n, kBlock, 0, st>>>(p);
     WF2_TRY(after_launch("xent_tile_loss"));
@@ -1174,20 +1225,24 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
   const int64_t words = xent_words(rows, vocab);
   const int64_t padded = ceil_div(rows, kTileN) * kTileN;
   const int64_t tiles_d = ceil_div(dim, kTileN), tiles_x = ceil_div(rows, kTileM);
-  // dx has few tiles and a long K: shares of it of about a quarter of what a workgroup slot (two to a compute unit) gets to
-  // do in all, so that the last ones fill the gaps; half of it where dw's tiles are short enough for that.  At least 16 K
-  // steps, an even number (a share starts at a whole row block of w).
-  const int64_t steps_dx = ceil_div(words < vocab ? words : vocab, 16), steps_dw = ceil_div(rows, 16);
-  const int64_t slot = tiles_d * (words / kTileM * steps_dw + tiles_x * steps_dx) / (2 * rt().num_cus);
-  int64_t split = steps_dw <= slot / 2 ? slot / 2 : slot / 4;
-  if (split > steps_dx) split = steps_dx;
-  if (split < 16) split = 16;
-  split = ceil_div(ceil_div(steps_dx, ceil_div(steps_dx, split)), 2) * 2;
+  // Either product's K goes in shares of about a quarter of what a workgroup slot (two to a compute unit) gets to do in all,
+  // so that the last ones fill the gaps -- half of it for dx where dw's tiles are short enough for that -- but dw's only
+  // where its tiles are few (a plane of dw is as large as the table).  At least 32 K steps, an even number (a share starts
+  // at a whole row block).
+  const int64_t steps_x = ceil_div(words < vocab ? words : vocab, 16), steps_w = ceil_div(rows, 16);
+  const int64_t dw_tiles = tiles_d * (words / kTileM), dx_tiles = tiles_d * tiles_x;
+  const int64_t slots = 2 * rt().num_cus, slot = (dw_tiles * steps_w + dx_tiles * steps_x) / slots;
+  auto split_of = [](int64_t steps, int64_t target) {
+    if (target < 32) target = 32;
+    return ceil_div(ceil_div(steps, ceil_div(steps, target < steps ? target : steps)), 2) * 2;
+  };
+  const int64_t split_x = split_of(steps_x, steps_w <= slot / 2 ? slot / 2 : slot / 4);
+  const int64_t split_w = words >= vocab && dw_tiles < slots ? split_of(steps_w, slot / 2) : steps_w;
+  const int64_t shares_w = ceil_div(steps_w, split_w);
   int64_t planes = 0;
-  for (int64_t c = 0; c < vocab; c += words) planes += ceil_div(ceil_div(words < vocab - c ? words : vocab - c, 16), split);
+  for (int64_t c = 0; c < vocab; c += words) planes += ceil_div(ceil_div(words < vocab - c ? words : vocab - c, 16), split_x);
   const int64_t most = ((int64_t)1 << 31) - 16;
-  if (words / kTileM * (padded / kTileN) > most || tiles_d * (words / kTileM + tiles_x * ceil_div(steps_dx, split)) > most ||
-      ceil_div(nx, kBlock) > most)
+  if (words / kTileM * ceil_div(rows, 64) > most || dw_tiles * shares_w + dx_tiles * ceil_div(steps_x, split_x) > most)
     return fail(WF2HIP_EUNSUPPORTED, "%s: too many tiles for one launch", name);
 
   Blocks blocks;
@@ -1197,6 +1252,7 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
   px.base = blocks.take<char>(pair_bytes(px));
   ds.base = blocks.take<char>(pair_bytes(ds));
   float* part = blocks.take<float>(planes * nx * 4);
+  float* part_w = shares_w > 1 ? blocks.take<float>(shares_w * nw * 4) : nullptr;
   float* g = blocks.take<float>(rows * (int64_t)4);
   float* largest = blocks.take<float>((kLargestW + kLargestX) * 4);
   XentHead* head = blocks.take<XentHead>(sizeof(XentHead));
@@ -1236,29 +1292,28 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
     p.rows = rows;
     p.dim = dim;
     p.tiles_m = (uint32_t)ceil_div(p.words, kTileM);
-    p.tiles_n = (uint32_t)(padded / kTileN);
+    p.width = xent_width(p.tiles_m, rows);
+    p.tiles_n = (uint32_t)ceil_div(rows, p.width);
     xent_tile_ds<<<p.tiles_m * p.tiles_n, kBlock, 0, st>>>(p);
     WF2_TRY(after_launch("xent_tile_ds"));
 
     p.tiles_w = p.tiles_m;
     p.tiles_x = (uint32_t)tiles_x;
     p.tiles_d = (uint32_t)tiles_d;
-    p.steps_dx = (int)ceil_div(p.words, 16);
-    p.steps_dw = (int)steps_dw;
-    p.split = (int)split;
-    p.shares = (uint32_t)ceil_div(p.steps_dx, split);
-    p.dw_first = steps_dw >= split;
+    p.steps_x = (int)ceil_div(p.words, 16);
+    p.steps_w = (int)steps_w;
+    p.split_x = (int)split_x;
+    p.split_w = (int)split_w;
+    p.shares_x = (uint32_t)ceil_div(p.steps_x, split_x);
+    p.shares_w = (uint32_t)shares_w;
+    p.dw_first = split_w >= split_x;
     p.planes = part + plane * nx;
-    p.dw = dw + c * dim;
-    plane += p.shares;
-    const uint32_t dw_tiles = p.tiles_w * p.tiles_d, dx_units = p.tiles_x * p.tiles_d * p.shares;
-    const uint32_t front = p.dw_first ? dw_tiles : dx_units;
-    xent_tile_gradients<<<((front + 7) & ~7u) + (p.dw_first ? dx_units : dw_tiles), kBlock, 0, st>>>(p);
+    p.dw = part_w ? part_w : dw + c * dim;
+    plane += p.shares_x;
+    const uint32_t dw_units = p.tiles_w * p.tiles_d * p.shares_w, dx_units = p.tiles_x * p.tiles_d * p.shares_x;
+    const uint32_t front = p.dw_first ? dw_units : dx_units;
+    xent_tile_gradients<<<((front + 7) & ~7u) + (p.dw_first ? dx_units : dw_units), kBlock, 0, st>>>(p);
     WF2_TRY(after_launch("xent_tile_gradients"));
   }
-  if (dim % 4 == 0 && (uintptr_t)dx % 16 == 0)
-    xent_fold_dx<true><<<(uint32_t)ceil_div(nx / 4, kBlock), kBlock, 0, st>>>(nx, dim, (int)planes, part, g, head, dx);
-  else
-    xent_fold_dx<false><<<(uint32_t)ceil_div(nx, kBlock), kBlock, 0, st>>>(nx, dim, (int)planes, part, g, head, dx);
-  return after_launch("xent_fold_dx");
+  return fold_gradients(XentPlanes{nx, (int)planes, part, dx}, XentPlanes{part_w ? nw : 0, (int)shares_w, part_w, dw}, dim, g, head, st);
 }

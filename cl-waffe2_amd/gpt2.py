@@ -227,3 +227,56 @@ def model_forward(tokens: HIPTensor, model: dict, cfg: dict = CONFIG, mode: str 
     ln = F.layer_norm_fused if mode != "nodes" else F.layer_norm
     x = ln(x, model["ln_f_g"], model["ln_f_b"], cfg["eps"])
     return F.matmul(x, F.t(model["wte"]))
+
+
+BLOCK_PARAMETERS = ("w_qkv", "w_o", "w_fc", "w_proj", "b_qkv", "b_o", "b_fc", "b_proj", "ln1_g", "ln1_b", "ln2_g", "ln2_b")
+
+
+def model_parameters(model: dict) -> list:
+    """Every tensor of `model` in the order :func:`model_gradients` returns their gradients."""
+    return [model["wte"], model["wpe"]] + [layer[k] for layer in model["layers"] for k in BLOCK_PARAMETERS] + \
+        [model["ln_f_g"], model["ln_f_b"]]
+
+
+def model_loss(tokens: HIPTensor, labels: HIPTensor, model: dict, cfg: dict = CONFIG, reduction: str | None = "mean",
+               saved: dict | None = None) -> HIPTensor:
+    """The language model's loss: the mean over the positions that count of the softmax cross entropy of
+    :func:`model_forward`'s logits against ``labels`` (N, T) :int32 (the tokens one position on; a negative id leaves its
+    position out), without the logits.  `saved`, when given, receives what :func:`model_gradients` needs."""
+    from . import nn
+    x = positional_embedding(tokens, model["wte"], model["wpe"])
+    layers = []
+    for layer in model["layers"]:
+        kept = {} if saved is not None else None
+        x = block_forward(x, layer, cfg=cfg, saved=kept)
+        layers.append(kept)
+    h = F.layer_norm_fused(x, model["ln_f_g"], model["ln_f_b"], cfg["eps"])
+    loss, lse = nn.linear_cross_entropy(h, model["wte"], labels, reduction=reduction)
+    if saved is not None:
+        saved.update(tokens=tokens, labels=labels, layers=layers, last=x, hidden=h, lse=lse, reduction=reduction)
+    return loss
+
+
+def model_gradients(saved: dict, model: dict, cfg: dict = CONFIG, dy=1.0) -> list:
+    """The gradients of :func:`model_loss` from what it saved, one per tensor of :func:`model_parameters`.  The token
+    table has two: the loss's (it is the head's matrix) and the embedding's, which is added to it."""
+    from . import nn
+    dh, dwte = nn.linear_cross_entropy_backward(dy, saved["hidden"], model["wte"], saved["labels"], saved["lse"],
+                                                reduction=saved["reduction"])
+    dx, dg, db = F.layer_norm_backward(saved["last"], model["ln_f_g"], dh, cfg["eps"])
+    blocks = []
+    for layer, kept in zip(reversed(model["layers"]), reversed(saved["layers"])):
+        dx, grads = block_backward(dx, kept, layer, cfg)
+        blocks.append([grads[k] for k in BLOCK_PARAMETERS])
+    dwpe = HIPTensor(list(model["wpe"].shape))
+    positional_embedding_backward(saved["tokens"], dx, dwte, dwpe)
+    return [dwte, dwpe] + [g for grads in reversed(blocks) for g in grads] + [dg, db]
+
+
+def train_step(tokens: HIPTensor, labels: HIPTensor, model: dict, optimizer, cfg: dict = CONFIG) -> HIPTensor:
+    """One step of ``optimizer`` (an ``optimizers.AdamW`` over :func:`model_parameters`) on the mean loss of a batch;
+    returns that loss."""
+    saved = {}
+    loss = model_loss(tokens, labels, model, cfg, saved=saved)
+    optimizer.step(model_gradients(saved, model, cfg))
+    return loss

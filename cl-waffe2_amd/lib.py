@@ -120,7 +120,7 @@ class AdamWDesc(C.Structure):
     """``struct wf2hip_adamw_desc``"""
 
     _fields_ = [
-        ("lr_device", C.c_void_p), ("lr", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float),
+        ("lr_device", C.c_void_p), ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
         ("state_bits", C.c_int32), ("reserved", C.c_int32),
     ]
 

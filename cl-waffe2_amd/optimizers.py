@@ -130,7 +130,7 @@ class AdamW:
         if state_bits not in (8, 32):
             raise ValueError(f"AdamW: states have 8 or 32 bits, not {state_bits}")
         self.params, self.lr, self.state_bits = list(params), lr, state_bits
-        self.beta1, self.beta2, self.eps = float(np.float32(beta1)), float(np.float32(beta2)), float(eps)
+        self.beta1, self.beta2, self.eps = float(beta1), float(beta2), float(eps)
         sizes = [self._own("a parameter", p) for p in self.params]
         decays = [float(weight_decay)] * len(sizes) if isinstance(weight_decay, F.Number) else [float(d) for d in weight_decay]
         if len(decays) != len(sizes):

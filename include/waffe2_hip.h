@@ -792,7 +792,8 @@ int wf2hip_adam_step_f32(long n, float* param, const float* grad, float* m, floa
 /* One AdamW step over `count` tensors in one launch (one per 91 tensors, 67 with 8-bit states), the weights' decay apart from the gradient:
  *   m <- m + (g - m) (1 - beta1),   v <- v + (1 - beta2) (g g - v),
  *   param <- param - lr weight_decay param - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps),
- * t the number of this step.  The reference has Adam only (source/optimizers/impls/adam.lisp:45-117), a tensor
+ * t the number of this step, in binary32 but for what beta and t give: 1 - beta, lr / (1 - beta1^t) and
+ * 1 / sqrt(1 - beta2^t) are formed in binary64 and rounded once.  The reference has Adam only (source/optimizers/impls/adam.lisp:45-117), a tensor
  * at a time.  state_bits 32: m and v are floats.  state_bits 8: m holds codes of m and v codes of r = sqrt(v),
  * one byte per element, in blocks of 256 consecutive elements of a tensor: an e4m3 number (sign, 4 bits of
  * exponent under a bias of 7, 3 of mantissa) times the block's scale, max(largest |element| / 448, 2^-126),
@@ -817,7 +818,7 @@ typedef struct wf2hip_adamw_tensor {
 } wf2hip_adamw_tensor;
 typedef struct wf2hip_adamw_desc {
   const float* lr_device;
-  float lr, beta1, beta2, eps;
+  double lr, beta1, beta2, eps;
   int32_t state_bits; /* 8 or 32 */
   int32_t reserved;
 } wf2hip_adamw_desc;

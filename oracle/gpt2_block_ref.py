@@ -178,3 +178,50 @@ def model_forward(tokens, model, n_head, eps=1e-5):
         x = block_forward(x, layer, n_head, eps)
     x = layer_norm(x, model["ln_f_g"].astype(f8), model["ln_f_b"].astype(f8), eps)
     return x @ model["wte"].astype(f8).T
+
+
+def model_loss(tokens, labels, model, n_head, eps=1e-5):
+    """Mean over the positions with a label (label >= 0) of -log softmax(logits)[label], float64."""
+    logits = model_forward(tokens, model, n_head, eps).reshape(-1, model["wte"].shape[0])
+    labels = np.asarray(labels).reshape(-1)
+    top = logits.max(axis=1, keepdims=True)
+    lse = (top + np.log(np.exp(logits - top).sum(axis=1, keepdims=True)))[:, 0]
+    keep = labels >= 0
+    each = lse - logits[np.arange(len(labels)), np.maximum(labels, 0)]
+    return each[keep].mean()
+
+
+def model_gradients(tokens, labels, model, n_head, eps=1e-5):
+    """Gradients of model_loss in float64 and, per tensor, the magnitude its last product or sum adds up.  Returns two
+    dicts keyed 'wte', 'wpe', 'ln_f_g', 'ln_f_b' and (layer, parameter name)."""
+    f8 = np.float64
+    ids = np.rint(np.asarray(tokens)).astype(np.int64)
+    labels = np.asarray(labels).reshape(-1)
+    wte, wpe = model["wte"].astype(f8), model["wpe"].astype(f8)
+    xs = [wte[ids] + wpe[np.arange(ids.shape[1])][None]]
+    for layer in model["layers"]:
+        xs.append(block_forward(xs[-1], layer, n_head, eps))
+    g, b = model["ln_f_g"].astype(f8), model["ln_f_b"].astype(f8)
+    h = layer_norm(xs[-1], g, b, eps).reshape(len(labels), -1)
+    logits = h @ wte.T
+    p = np.exp(logits - logits.max(axis=1, keepdims=True))
+    p /= p.sum(axis=1, keepdims=True)
+    keep = labels >= 0
+    p[np.arange(len(labels)), np.maximum(labels, 0)] -= 1.0
+    ds = p * (keep / keep.sum())[:, None]
+    grads, scales = {}, {}
+    dh = (ds @ wte).reshape(xs[-1].shape)
+    grads["wte"], scales["wte"] = ds.T @ h, np.abs(ds).T @ np.abs(h)
+    dx, grads["ln_f_g"], grads["ln_f_b"], _, scales["ln_f_g"] = layer_norm_backward(xs[-1], g, dh, eps)
+    scales["ln_f_b"] = np.abs(dh).sum(axis=(0, 1))
+    for i in range(len(model["layers"]) - 1, -1, -1):
+        gr, sc = block_backward(xs[i], model["layers"][i], n_head, dx, eps)
+        dx = gr.pop("x")
+        sc.pop("x")
+        for k in gr:
+            grads[(i, k)], scales[(i, k)] = gr[k], sc[k]
+    np.add.at(grads["wte"], ids, dx)
+    np.add.at(scales["wte"], ids, np.abs(dx))
+    grads["wpe"], scales["wpe"] = np.zeros_like(wpe), np.zeros_like(wpe)
+    grads["wpe"][:ids.shape[1]], scales["wpe"][:ids.shape[1]] = dx.sum(axis=0), np.abs(dx).sum(axis=0)
+    return grads, scales

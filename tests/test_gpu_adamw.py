@@ -33,8 +33,7 @@ def decode(codes, scale):
 
 def reference(p, g, m, v, t, decay, hyper=HYPER):
     """One step in float64: p, m, v and their bounds for a binary32 implementation."""
-    b1, b2 = float(f32(hyper["beta1"])), float(f32(hyper["beta2"]))
-    lr, eps = float(f32(hyper["lr"])), float(f32(hyper["eps"]))
+    b1, b2, lr, eps = (hyper[k] for k in ("beta1", "beta2", "lr", "eps"))
     p, g, m, v = (a.astype(np.float64) for a in (p, g, m, v))
     m1 = m + (g - m) * (1 - b1)
     v1 = v + (1 - b2) * (g * g - v)
@@ -75,10 +74,10 @@ def test_reference_matches_a_spelt_out_step():
     t, d = 3, 0.1
     p1, m1, v1, *_ = reference(p, g, m, v, t, d)
     for i in range(5):
-        b1, b2 = float(f32(0.9)), float(f32(0.95))
+        b1, b2 = 0.9, 0.95
         mm = b1 * float(m[i]) + (1 - b1) * float(g[i])
         vv = b2 * float(v[i]) + (1 - b2) * float(g[i]) ** 2
-        want = float(p[i]) * (1 - float(f32(6e-3)) * float(f32(d))) - float(f32(6e-3)) * (mm / (1 - b1 ** t)) / (np.sqrt(vv / (1 - b2 ** t)) + float(f32(1e-8)))
+        want = float(p[i]) * (1 - 6e-3 * float(f32(d))) - 6e-3 * (mm / (1 - b1 ** t)) / (np.sqrt(vv / (1 - b2 ** t)) + 1e-8)
         assert abs(want - p1[i]) < 1e-15 and abs(mm - m1[i]) < 1e-18 and abs(vv - v1[i]) < 1e-18
 
 
@@ -160,7 +159,7 @@ def test_states_in_8_bits(gpu, t):
         v = decode(codes[i][1], codes[i][3]) ** 2
         p1, m1, v1, ep, em, ev = reference(d[0], d[1], m, v, t, 0.1)
         em, ev = em + 2 * U * np.abs(m), ev + 4 * U * v      # the decoded states are products, rounded
-        b1, b2 = float(f32(HYPER["beta1"])), float(f32(HYPER["beta2"]))
+        b1, b2 = HYPER["beta1"], HYPER["beta2"]
         root = np.sqrt(v1 / (1 - b2 ** t)) + 1e-8
         ep = ep + 6e-3 / (1 - b1 ** t) * (2 * U * np.abs(m) + np.abs(m1) * 2 * U * v / np.maximum(v1, 1e-300)) / root
         assert np.all(np.abs(p[i].numpy() - p1) <= ep), (SIZES[i], np.max(np.abs(p[i].numpy() - p1) / ep))
@@ -243,7 +242,7 @@ def test_replayed_steps_count_on(gpu):
         q, h = (tensors(W, [d[k] for d in data]) for k in (0, 1))
         rate = F.from_numpy(np.array([1e-3], f32))
         opt = O.AdamW(p, lr=rate, state_bits=bits)
-        ref = O.AdamW(q, lr=1e-3, state_bits=bits)
+        ref = O.AdamW(q, lr=float(f32(1e-3)), state_bits=bits)   # the number that the tensor on the device holds
         opt.step(g)
         ref.step(h)
         with W.lib.Graph() as graph:
@@ -252,7 +251,7 @@ def test_replayed_steps_count_on(gpu):
         for i in range(4):
             if i == 2:
                 F.move_(rate, F.from_numpy(np.array([5e-4], f32)))
-                ref.lr = 5e-4
+                ref.lr = float(f32(5e-4))
                 F.mul_(g[1], -2.0)
                 F.mul_(h[1], -2.0)
             graph.launch()

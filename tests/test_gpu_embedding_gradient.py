@@ -56,7 +56,8 @@ def check(W, *data):
 
 
 SHAPES = [(1, 1, 1, 1, 1), (1, 1, 5, 3, 4), (2, 7, 50, 16, 12), (2, 24, 300, 32, 64), (3, 33, 1000, 64, 70), (5, 51, 3, 51, 33),
-          (1, 257, 70000, 300, 20), (2, 100, 5000, 128, 768), (8, 1024, 50257, 1024, 96), (9, 200, 13, 200, 1025), (64, 17, 97, 17, 8)]
+          (1, 257, 70000, 300, 20), (2, 100, 5000, 128, 768), (8, 1024, 50257, 1024, 96), (9, 200, 13, 200, 1025), (64, 17, 97, 17, 8),
+          (700, 3, 40, 4, 36), (300, 1, 5000, 2, 1)]
 
 
 @pytest.mark.gpu
