@@ -15,6 +15,7 @@
 // operator beyond a few hundred rows.
 #include <stdlib.h>
 
+#include <algorithm>
 #include <utility>
 
 #include "wf2_direct.h"
@@ -572,23 +573,25 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   }
 }
 
-// dx and, where it is in planes too, dw of a piece: the planes' sums, scaled.  Rows of dx without a label are zero whatever the
-// common factor is.
+// The planes' sums of dx and of dw (or a piece of it), scaled where there is a `head`.  Rows of dx without a label are zero
+// whatever the common factor is.  `out` may be the first plane.
 struct XentPlanes {
-  int64_t n;            // elements of a plane
+  int64_t n;            // elements of a plane; 0: nothing to add up
   int planes;
   const float* part;
   float* out;
+  const XentHead* head;
 };
 template <bool VEC>
 __global__ __launch_bounds__(kBlock) void xent_fold_gradients(XentPlanes x, XentPlanes w, uint32_t x_groups, long dim,
-                                                              const float* __restrict__ g, const XentHead* __restrict__ head) {
+                                                              const float* __restrict__ g) {
   typedef float fv __attribute__((ext_vector_type(VEC ? 4 : 1)));
   constexpr int V = VEC ? 4 : 1;
   const bool of_x = blockIdx.x < x_groups;
   const int64_t n = of_x ? x.n : w.n;
   const int planes = of_x ? x.planes : w.planes;
   const float* part = of_x ? x.part : w.part;
+  const XentHead* head = of_x ? x.head : w.head;
   const int64_t i = ((int64_t)(of_x ? blockIdx.x : blockIdx.x - x_groups) * kBlock + threadIdx.x) * V;
   if (i >= n) return;
   fv sum = *reinterpret_cast<const fv*>(part + i);
@@ -985,16 +988,16 @@ static int64_t xent_words(int64_t rows, int64_t vocab) {
   return ceil_div(tiles, pieces) * kTileM;
 }
 
-// The planes' sums of both gradients in one launch; n 0: that one is not in planes.
-static int fold_gradients(const XentPlanes& x, const XentPlanes& w, int64_t dim, const float* g, const XentHead* head, hipStream_t st) {
+// The planes' sums of both gradients in one launch.
+static int fold_gradients(const XentPlanes& x, const XentPlanes& w, int64_t dim, const float* g, hipStream_t st) {
   const bool vec = dim % 4 == 0 && ((uintptr_t)x.out | (uintptr_t)w.out) % 16 == 0;
   const int64_t per = vec ? 4 : 1, gx = ceil_div(x.n / per, kBlock), gw = ceil_div(w.n / per, kBlock);
   if (gx + gw == 0) return 0;
   if (gx + gw >= ((int64_t)1 << 31)) return fail(WF2HIP_EUNSUPPORTED, "linear cross entropy backward: too many elements for one launch");
   if (vec)
-    xent_fold_gradients<true><<<(uint32_t)(gx + gw), kBlock, 0, st>>>(x, w, (uint32_t)gx, dim, g, head);
+    xent_fold_gradients<true><<<(uint32_t)(gx + gw), kBlock, 0, st>>>(x, w, (uint32_t)gx, dim, g);
   else
-    xent_fold_gradients<false><<<(uint32_t)(gx + gw), kBlock, 0, st>>>(x, w, (uint32_t)gx, dim, g, head);
+    xent_fold_gradients<false><<<(uint32_t)(gx + gw), kBlock, 0, st>>>(x, w, (uint32_t)gx, dim, g);
   return after_launch("xent_fold_gradients");
 }
 
@@ -1016,8 +1019,8 @@ static XentRoute xent_route(int64_t rows, int64_t dim, int64_t vocab, bool backw
   //             256 x 768 x 50257 123 / 143 / 213
   //   backward  256 x 768 x 1000  92 / 83 / 53    400 x 200 x 3000  78 / 94 / 75    1000 x 400 x 2000 86 / 105 / 154
   //             16 x 1600 x 20000 198 / 149 / 263 61 x 768 x 50257  240 / 208 / 676 64 x 768 x 8192   61 / 70 / 117
-  const int64_t work = rows * dim * vocab;
-  if (work <= (backward ? (int64_t)1 << 28 : (int64_t)3 << 28)) return kSmall;
+  const double work = (double)rows * (double)dim * (double)vocab;   // may pass 2^63
+  if (work <= (backward ? 0x1p28 : 0x3p28)) return kSmall;
   return backward ? (rows <= 64 && vocab * dim >= ((int64_t)1 << 24) ? kSkinny : kPairs) : rows <= 160 ? kSkinny : kPairs;
 }
 
@@ -1099,8 +1102,8 @@ static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int6
       nbw == 1 ? with(std::integral_constant<int, 1>()) : with(std::integral_constant<int, 2>());
   }
   WF2_TRY(after_launch("xent_direct_gradients"));
-  return fold_gradients(XentPlanes{shares_x > 1 ? nx : 0, (int)shares_x, p.dx, dx}, XentPlanes{shares_w > 1 ? nw : 0, (int)shares_w, p.dw, dw},
-                        dim, nullptr, nullptr, st);
+  return fold_gradients(XentPlanes{shares_x > 1 ? nx : 0, (int)shares_x, p.dx, dx, nullptr},
+                        XentPlanes{shares_w > 1 ? nw : 0, (int)shares_w, p.dw, dw, nullptr}, dim, nullptr, st);
 }
 
 template <bool PER_ROW>
@@ -1237,12 +1240,13 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
     return ceil_div(ceil_div(steps, ceil_div(steps, target < steps ? target : steps)), 2) * 2;
   };
   const int64_t split_x = split_of(steps_x, steps_w <= slot / 2 ? slot / 2 : slot / 4);
-  const int64_t split_w = words >= vocab && dw_tiles < slots ? split_of(steps_w, slot / 2) : steps_w;
-  const int64_t shares_w = ceil_div(steps_w, split_w);
-  int64_t planes = 0;
-  for (int64_t c = 0; c < vocab; c += words) planes += ceil_div(ceil_div(words < vocab - c ? words : vocab - c, 16), split_x);
+  const int64_t split_w = dw_tiles < slots ? split_of(steps_w, slot / 2) : steps_w;
+  const int64_t shares_w = ceil_div(steps_w, split_w), shares_x = ceil_div(steps_x, split_x);
+  // dx's planes: of all pieces as far as 1 GiB goes; where they fill it they are added up in the first one
+  int64_t planes = ceil_div(vocab, words) * shares_x;
+  if (planes > ((int64_t)1 << 28) / nx) planes = std::min(planes, std::max(((int64_t)1 << 28) / nx, shares_x + 1));
   const int64_t most = ((int64_t)1 << 31) - 16;
-  if (words / kTileM * ceil_div(rows, 64) > most || dw_tiles * shares_w + dx_tiles * ceil_div(steps_x, split_x) > most)
+  if (words / kTileM * ceil_div(rows, 64) > most || dw_tiles * shares_w + dx_tiles * shares_x > most)
     return fail(WF2HIP_EUNSUPPORTED, "%s: too many tiles for one launch", name);
 
   Blocks blocks;
@@ -1252,7 +1256,7 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
   px.base = blocks.take<char>(pair_bytes(px));
   ds.base = blocks.take<char>(pair_bytes(ds));
   float* part = blocks.take<float>(planes * nx * 4);
-  float* part_w = shares_w > 1 ? blocks.take<float>(shares_w * nw * 4) : nullptr;
+  float* part_w = shares_w > 1 ? blocks.take<float>(shares_w * std::min<int64_t>(words, vocab) * dim * 4) : nullptr;
   float* g = blocks.take<float>(rows * (int64_t)4);
   float* largest = blocks.take<float>((kLargestW + kLargestX) * 4);
   XentHead* head = blocks.take<XentHead>(sizeof(XentHead));
@@ -1314,6 +1318,10 @@ WF2_API int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long v
     const uint32_t front = p.dw_first ? dw_units : dx_units;
     xent_tile_gradients<<<((front + 7) & ~7u) + (p.dw_first ? dx_units : dw_units), kBlock, 0, st>>>(p);
     WF2_TRY(after_launch("xent_tile_gradients"));
+    const bool done = c + words >= vocab, full = !done && plane + shares_x > planes;
+    WF2_TRY(fold_gradients(XentPlanes{done || full ? nx : 0, (int)plane, part, done ? dx : part, done ? head : nullptr},
+                           XentPlanes{part_w ? p.words * dim : 0, (int)shares_w, part_w, dw + c * dim, head}, dim, g, st));
+    if (full) plane = 1;
   }
-  return fold_gradients(XentPlanes{nx, (int)planes, part, dx}, XentPlanes{part_w ? nw : 0, (int)shares_w, part_w, dw}, dim, g, head, st);
+  return 0;
 }

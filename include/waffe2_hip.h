@@ -886,7 +886,11 @@ int wf2hip_linear_cross_entropy_f32(long rows, long dim, long vocab, const float
 /* Its gradients from the same inputs and the forward's lse: with
  *   ds[n, v] = g[n] (exp(s[n, v] - lse[n]) - [v = labels[n]]),   dx = ds . w,   dw = ds^T . x
  * (both overwritten), g[n] = scale * dloss[n] (reduction none), scale * dloss[0] (sum), the same over the number
- * of rows with a label (mean); dloss NULL stands for ones. */
+ * of rows with a label (mean); dloss NULL stands for ones.  Beyond small products and few rows an element of x (rows with
+ * a label), w or ds is kept to 2^-22 of itself or 2^-39 of the largest of its matrix, whichever is more: hidden states and tables
+ * whose rows differ by less than a factor of 2^16 lose nothing that binary32 sums keep.  Scratch from the pool: about the
+ * size of x and w, up to 1 GiB for ds (512 bytes per row where that is more), and up to 1 GiB or two more copies of dx for
+ * sums in parts. */
 int wf2hip_linear_cross_entropy_backward_f32(long rows, long dim, long vocab, const float* x,
                                              const float* w, const int32_t* labels, const float* lse,
                                              int reduction, const float* dloss, float scale, float* dx,

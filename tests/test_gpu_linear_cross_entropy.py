@@ -295,6 +295,64 @@ def test_replayed_graph_equals_eager(gpu, rows, dim, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,vocab", [(16500, 24, 20003), (262000, 260, 3211)])
+def test_vocabulary_in_pieces(gpu, rows, dim, vocab):
+    """More than 2^28 elements of ds: the backward walks the vocabulary in pieces; in the second case dx's shares of all
+    pieces would pass 2^28 elements too and are added up on the way.  Held against float64 on every row's loss, a few
+    dozen rows of dx (the one of the largest gradient among them) and words of dw.  The logits' error bound over a whole
+    row takes sum |a||b| <= |a||b| in the Euclidean norm; otherwise the bounds are those of bounds()."""
+    import torch
+    F, nn = gpu.functional, gpu.nn
+    x, w, labels = inputs(rows, dim, vocab, left_out=0.1)
+    dy = np.random.default_rng(1).uniform(0.1, 2.0, rows).astype(f32)
+    d = [F.from_numpy(x), F.from_numpy(w), F.from_numpy(labels, dtype="int32")]
+    each, lse = nn.linear_cross_entropy(*d, reduction=None)
+    gx, gw = nn.linear_cross_entropy_backward(F.from_numpy(dy), *d, lse, reduction=None)
+    each, lse, gx, gw = (t.numpy() for t in (each, lse, gx, gw))
+    keep = labels >= 0
+    at = np.unique(np.append(np.linspace(0, rows - 1, 40).astype(int), np.argmax(dy * keep)))
+    words = np.unique(np.append(np.linspace(0, vocab - 1, 40).astype(int), labels[keep][:8]))
+    # the rows: all of their words
+    t = truth(x[at], w, labels[at], None, dy[at])
+    _, _, e_dx, _ = bounds(t)
+    assert np.all(np.abs(gx[at] - t["dx"]) <= e_dx), np.max(np.abs(gx[at] - t["dx"]) / e_dx)
+    assert not gx[~keep].any()
+    # the words, and every row's loss
+    W64, V64 = torch.from_numpy(w).double(), torch.from_numpy(w[words]).double()
+    top_x, top_w = float(np.abs(x[keep]).max()), float(np.abs(w).max())
+    norm_w, sum_w = float(W64.norm(dim=1).max()), float(W64.abs().sum(1).max())
+    dw = torch.zeros(len(words), dim, dtype=torch.float64)
+    total, e_dw = torch.zeros_like(dw), torch.zeros_like(dw)
+    for r in range(0, rows, 16384):
+        xs, ls = torch.from_numpy(x[r:r + 16384]).double(), torch.from_numpy(labels[r:r + 16384]).long()
+        s = xs @ W64.t()
+        l = torch.logsumexp(s, 1)
+        far = (s - l[:, None]).abs().amax(1)
+        at_label = s.gather(1, ls.clamp(min=0)[:, None])[:, 0]
+        row_s = (dim + 14) * U * xs.norm(dim=1) * norm_w + 2.0 ** -39 * (top_x * sum_w + top_w * xs.abs().sum(1))
+        err_lse = row_s + 4 * U * (l.abs() + 1) + 4 * U + far * U
+        got = torch.from_numpy(lse[r:r + 16384]).double()
+        assert bool(((got - l).abs() <= err_lse)[ls >= 0].all())
+        got = torch.from_numpy(each[r:r + 16384]).double()
+        want = torch.where(ls >= 0, l - at_label, 0.0)
+        assert bool(((got - want).abs() <= torch.where(ls >= 0, err_lse + row_s + 2 * U * s.abs().amax(1), 0.0)).all())
+        away = s[:, words] - l[:, None]
+        p, hot = away.exp(), (torch.from_numpy(words)[None] == ls[:, None]).double()
+        g = torch.where(ls >= 0, torch.from_numpy(dy[r:r + 16384]).double(), 0.0)[:, None]
+        ds = (p - hot) * g
+        small = 2.0 ** -39 * (top_x * V64.abs().sum(1) + top_w * xs.abs().sum(1)[:, None])
+        err_s = (dim + 14) * U * (xs.abs() @ V64.abs().t()) + small
+        err = g * (p * (err_s + err_lse[:, None] + (4 + away.abs()) * U) + 4 * U * (p + U)) + 4 * U * ds.abs()
+        dw += ds.t() @ xs
+        total += ds.abs().t() @ xs.abs()
+        e_dw += err.t() @ xs.abs() + 2.0 ** -39 * (float(dy.max()) * xs.abs().sum(0) + top_x * ds.abs().sum(0)[:, None])
+    e_dw = (e_dw + (rows + 14) * U * total).numpy() + 1e-37
+    off = np.abs(gw[words] - dw.numpy())
+    assert np.all(off <= e_dw), np.max(off / e_dw)
+    assert np.isfinite(gw).all() and np.isfinite(gx).all()
+
+
+@pytest.mark.gpu
 def test_argument_checks(gpu):
     W = gpu
     F, nn = W.functional, W.nn
