@@ -162,6 +162,18 @@
 (defcfun "wf2hip_adam_step_f32" :int
   (n :long) (param :pointer) (grad :pointer) (m :pointer) (v :pointer)
   (one-minus-beta1 :float) (one-minus-beta2 :float) (lr-t :float) (eps :float))
+;; one AdamW step over a model's tensors: desc a wf2hip_adamw_desc, tensors an array of wf2hip_adamw_tensor (adamw-step-hip
+;; in kernels.lisp writes both)
+(defcfun "wf2hip_adamw_step" :int (desc :pointer) (count :long) (tensors :pointer) (steps :pointer))
+
+;; softmax cross entropy over a vocabulary from hidden states and the token table, and its gradients
+(defcfun "wf2hip_linear_cross_entropy_f32" :int
+  (rows :long) (dim :long) (vocab :long) (x :pointer) (w :pointer) (labels :pointer) (reduction :int)
+  (loss :pointer) (lse :pointer))
+(defcfun "wf2hip_linear_cross_entropy_backward_f32" :int
+  (rows :long) (dim :long) (vocab :long) (x :pointer) (w :pointer) (labels :pointer) (lse :pointer) (reduction :int)
+  (dloss :pointer) (scale :float) (dx :pointer) (dw :pointer))
+(defconstant +reduce-none+ 0) (defconstant +reduce-sum+ 1) (defconstant +reduce-mean+ 2)
 
 ;; HIP graphs: record the launches of one compiled forward, replay them with one call.
 (defcfun "wf2hip_graph_begin" :int)

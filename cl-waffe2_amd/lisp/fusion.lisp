@@ -232,6 +232,58 @@ the reference's node."
       (call-composed 'cl-waffe2/nn:softmax-cross-entropy x labels :axis axis :delta delta
                                                               :avoid-overflow avoid-overflow :reduction reduction)))
 
+;; ---- softmax cross entropy over a vocabulary, without the logits --------------------------------
+(defun linear-cross-entropy-gradients (x w labels lse dout reduction)
+  "The gradients of HIP-Linear-Cross-Entropy-Node with respect to X and W from one library call."
+  (ensure-extension)
+  (let ((dout (eager-contiguous dout))
+        (dx (fresh-like x))
+        (dw (fresh-like w)))
+    (check (wf2hip-linear-cross-entropy-backward-f32 (first (shape x)) (second (shape x)) (first (shape w))
+                                                     (tensor-device-pointer x) (tensor-device-pointer w)
+                                                     (tensor-device-pointer labels) (tensor-device-pointer lse)
+                                                     reduction (tensor-device-pointer dout) 1.0
+                                                     (tensor-device-pointer dx) (tensor-device-pointer dw)))
+    (values dx dw)))
+
+(define-op (HIP-Linear-Cross-Entropy-Node (self reduction)
+            :slots ((reduction :initform 0 :accessor linear-cross-entropy-reduction))
+            :save-for-backward-names (x w labels lse)
+            :where (X[rows dim] W[vocab dim] Labels[rows] LSE[rows] OUT[losses] -> OUT[losses])
+            :documentation "OUT <- logsumexp(x . w^T) - x . w[label] per row, or their sum or mean (one element), without
+the logits: the lm-head of examples/gpt-2/model.lisp:137-196 and its criterion (source/nn/criterion.lisp:82-196) in one
+node.  Labels: :int32 token ids, a negative one leaves its row out.  LSE is what the backward needs."
+            :forward ((self x w labels lse out)
+                      (ensure-extension)
+                      (check (wf2hip-linear-cross-entropy-f32 (first (shape x)) (second (shape x)) (first (shape w))
+                                                              (tensor-device-pointer x) (tensor-device-pointer w)
+                                                              (tensor-device-pointer labels)
+                                                              (linear-cross-entropy-reduction self)
+                                                              (tensor-device-pointer out) (tensor-device-pointer lse)))
+                      (with-setting-save4bw ((x x) (w w) (labels labels) (lse lse)) out))
+            :backward ((self dout)
+                       (with-reading-save4bw ((x x) (w w) (labels labels) (lse lse))
+                         (multiple-value-bind (dx dw)
+                             (linear-cross-entropy-gradients x w labels lse dout (linear-cross-entropy-reduction self))
+                           (values dx dw nil nil nil)))))
+  (setf (linear-cross-entropy-reduction self) reduction))
+
+(defun !linear-cross-entropy-hip (x w labels &key (reduction :mean))
+  "Softmax cross entropy of the logits (!matmul x (!t w)) against the :int32 token ids LABELS[rows] as one node:
+X[rows dim] hidden states, W[vocab dim] the token table.  REDUCTION: :mean (over the rows whose label is not negative),
+:sum, or nil for a loss per row."
+  (assert (and (hip-float-tensor-p x) (hip-float-tensor-p w) (typep labels 'HIPTensor) (eql (dtype labels) :int32)) ()
+          "!linear-cross-entropy-hip: :float hidden states and table, :int32 labels, all HIPTensors")
+  (let ((rows (first (shape x)))
+        (code (ecase reduction
+                ((nil) +reduce-none+)
+                (:sum +reduce-sum+)
+                (:mean +reduce-mean+))))
+    (call (HIP-Linear-Cross-Entropy-Node code)
+          (->contiguous x) (->contiguous w) (->contiguous labels)
+          (make-input (list rows) nil :dtype :float :order (order x))
+          (make-input (list (if reduction 1 rows)) nil :dtype :float :order (order x)))))
+
 ;; ---- unfold ------------------------------------------------------------------------------------
 (defun unfold-out-size (size pad kernel stride)
   "conv-out-size (source/nn/pool.lisp:10-17) with dilation 1."

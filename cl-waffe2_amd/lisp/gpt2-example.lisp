@@ -36,3 +36,19 @@
                                                              (tensor-device-pointer wpe) (first (shape wpe))
                                                              (tensor-device-pointer ctx-out))))
                           ctx-out))
+
+(defcfun "wf2hip_embedding_gradient_f32" :int
+  (rows :long) (seq :long) (dim :long) (ctx :pointer) (dout :pointer) (dwte :pointer) (vocab :long) (dwpe :pointer)
+  (n-ctx :long))
+
+(defun positional-embedding-gradient (ctx dout dwte dwpe)
+  "The gradient of the node, added into the tables' gradients in one launch: dwte[round(ctx)] += dout,
+dwpe[position] += its sum over the sentences.  All contiguous :float HIPTensors."
+  (ensure-extension)
+  (let ((n (first (shape ctx)))
+        (seq (second (shape ctx))))
+    (check (wf2hip-embedding-gradient-f32 (* n seq) seq (second (shape dwte))
+                                          (tensor-device-pointer ctx) (tensor-device-pointer dout)
+                                          (tensor-device-pointer dwte) (first (shape dwte))
+                                          (tensor-device-pointer dwpe) (first (shape dwpe)))))
+  (values dwte dwpe))

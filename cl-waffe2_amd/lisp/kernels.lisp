@@ -374,3 +374,63 @@ extension has both, source/backends/cpu/mathematics.lisp:8-76)."
                   (cl-waffe2/optimizers::eps-of optimizer))))
         (call-next-method))))
 
+;; AdamW over all parameters of a model in one call (wf2hip_adamw_step): no counterpart in the reference, whose optimizers
+;; step a tensor at a time.
+(defun adamw-steps-hip (&key (done 0) (beta1 0.9d0) (beta2 0.999d0))
+  "The counter of adamw-step-hip after DONE steps: beta1^t, beta2^t, t and a zero, as a :double tensor."
+  (upload (make-array 4 :element-type 'double-float
+                        :initial-contents (list (expt beta1 done) (expt beta2 done) (coerce done 'double-float) 0.0d0))
+          :dtype :double))
+
+(defun adamw-step-hip (params grads m second steps
+                       &key (m-scale nil) (r-scale nil) (lr 1.0d-3) (beta1 0.9d0) (beta2 0.999d0) (eps 1.0d-8)
+                         (weight-decay 0.01))
+  "One AdamW step.  PARAMS, GRADS, M, SECOND: lists of contiguous HIPTensors, a :float parameter, its gradient and its two
+states each.  The states are :float tensors (m and v), or, with M-SCALE and R-SCALE, :uint8 codes of m and sqrt(v) under a
+:float scale per 256 elements.  STEPS: of adamw-steps-hip.  LR: a number, or a one-element :float tensor read on the device.
+WEIGHT-DECAY: a number, or one per parameter."
+  (ensure-extension)
+  (assert (every #'contiguous-device-tensor-p (append params grads m second m-scale r-scale)) ()
+          "adamw-step-hip: contiguous HIPTensors only")
+  (let* ((count (length params))
+         (codes (and m-scale t))
+         (scales (if codes count 0)))
+    (assert (and (= count (length grads)) (= count (length m)) (= count (length second))
+                 (= scales (length m-scale)) (= scales (length r-scale))) ()
+            "adamw-step-hip: a gradient and two states for every parameter, and two scales or none")
+    ;; the two structs as words of 8 bytes: six pointers, n, (weight_decay, reserved); lr_device, four doubles,
+    ;; (state_bits, reserved)
+    (with-foreign-objects ((table :int64 (max 1 (* 8 count))) (desc :int64 6))
+      (loop for i from 0 below count
+            for at = (* 8 i)
+            for param = (nth i params)
+            for grad = (nth i grads)
+            do (assert (and (= (apply #'* (shape param)) (apply #'* (shape grad)))
+                            (= (apply #'* (shape param)) (apply #'* (shape (nth i m))))
+                            (= (apply #'* (shape param)) (apply #'* (shape (nth i second))))) ()
+                       "adamw-step-hip: a gradient and states of the parameter's size")
+               (setf (mem-aref table :pointer at) (tensor-device-pointer param)
+                     (mem-aref table :pointer (+ at 1)) (tensor-device-pointer grad)
+                     (mem-aref table :pointer (+ at 2)) (tensor-device-pointer (nth i m))
+                     (mem-aref table :pointer (+ at 3)) (tensor-device-pointer (nth i second))
+                     (mem-aref table :int64 (+ at 4)) 0
+                     (mem-aref table :int64 (+ at 5)) 0
+                     (mem-aref table :int64 (+ at 6)) (apply #'* (shape param))
+                     (mem-aref table :float (+ (* 2 at) 14))
+                     (coerce (if (listp weight-decay) (nth i weight-decay) weight-decay) 'single-float)
+                     (mem-aref table :int32 (+ (* 2 at) 15)) 0)
+               (if codes
+                   (setf (mem-aref table :pointer (+ at 4)) (tensor-device-pointer (nth i m-scale))
+                         (mem-aref table :pointer (+ at 5)) (tensor-device-pointer (nth i r-scale)))))
+      (if (numberp lr)
+          (setf (mem-aref desc :int64 0) 0
+                (mem-aref desc :double 1) (coerce lr 'double-float))
+          (setf (mem-aref desc :pointer 0) (tensor-device-pointer lr)
+                (mem-aref desc :double 1) 0.0d0))
+      (setf (mem-aref desc :double 2) (coerce beta1 'double-float)
+            (mem-aref desc :double 3) (coerce beta2 'double-float)
+            (mem-aref desc :double 4) (coerce eps 'double-float)
+            (mem-aref desc :int32 10) (if codes 8 32)
+            (mem-aref desc :int32 11) 0)
+      (check (wf2hip-adamw-step desc count table (tensor-device-pointer steps))))
+    params))
