@@ -8,6 +8,8 @@
 // element (HBM-bound; the tables are small and stay in cache).  Token ids arrive as floats
 // (the example feeds :float tensors) and are rounded to nearest, ties to even, as Common Lisp's
 // ROUND does; ids outside the table are clamped to its ends (the reference reads out of bounds).
+#include <algorithm>
+
 #include "wf2_common.h"
 
 namespace wf2 {
@@ -50,18 +52,19 @@ __device__ __forceinline__ int32_t token_of(float id, int32_t vocab) {
 // every sum in an order that the rows alone decide, without atomics, so that the same call gives the same bits.
 //
 // The token table's part: the tokens are dealt out to `classes` classes by their low bits, and a workgroup of sixteen
-// wavefronts owns a class, hence every element it adds to.  It reads all ids (they stay in L2), keeps the rows of its
-// class in LDS in their order, sorts them by token (stable) and deals the sorted list out in equal runs to its
-// wavefronts, 64 vectors of the columns to each: a wavefront reads its rows eight or sixteen at a time and touches the table once per token,
-// however often that occurs; a token whose rows span several runs is put together from the wavefronts' parts in LDS.
-// (A text's most frequent word is a few per cent of it, a padded batch's padding most of it.)  The position table's part is
-// dealt out to the same workgroups.  Bound by HBM: dout once, and the rows of dwte it meets twice; short calls by
-// the length of the chain ids -> rows -> table.
+// wavefronts owns a class, or up to four share out its columns, hence every element it adds to.  It reads all ids (they stay
+// in L2), keeps the rows of its class in LDS in their order, sorts them by token (stable) and deals the sorted list out in
+// equal runs to its wavefronts, 64 vectors of the columns to each: a wavefront reads its rows eight or sixteen at a time and
+// touches the table once per token, however often that occurs; a token whose rows span several runs is put together from
+// the wavefronts' parts in LDS.  (A text's most frequent word is a few per cent of it, a padded batch's padding most of
+// it.)  The position table's part has workgroups of its own, beside those.  Bound by HBM: dout once, and the rows of dwte it
+// meets twice; short calls by the length of the chain ids -> rows -> table.  8192 rows of 768: 20.5 us with ids drawn evenly (3.8 TB/s
+// of the bytes it cannot do without), 22.3 with a text's, 104 where all are the same.
 constexpr int kGradBlock = 1024, kGradWaves = kGradBlock / kWave;
 constexpr int kGatherStep = 4 * kGradBlock;   // ids that a workgroup looks at at a time
 constexpr int kGather = 2 * kGatherStep;      // rows of a class that LDS holds at a time
 constexpr int kGatherTurns = kGather / kGradBlock;
-constexpr int kRankMost = 256;                // longer lists are sorted bit by bit
+constexpr int kRankMost = 256;                // longer lists are sorted by digits
 
 struct EmbeddingGradient {
   const float *ctx, *dout;
@@ -69,6 +72,7 @@ struct EmbeddingGradient {
   int64_t rows, seq, dim;
   int32_t vocab;
   uint32_t classes;       // a power of two
+  uint32_t parts;         // of the columns: workgroups to a class
   int token_bits;         // bits of a token above those of its class
   int shares;             // threads to a vector of the positions' part
 };
@@ -76,11 +80,13 @@ struct EmbeddingGradient {
 struct GatherLds {
   __attribute__((aligned(16))) int32_t row[kGather];
   __attribute__((aligned(16))) int32_t token[kGather];
-  int32_t votes[kGatherTurns * kGradWaves];   // of a turn's wavefronts
+  __attribute__((aligned(8))) int32_t digits[16][kGatherTurns * kGradWaves];
+  int32_t votes[kGradWaves];
 };
 
 // Stable sort of the first `count` entries by token.  Short lists: an entry's rank is the number of entries that go before
-// it.  Long ones: a pass per bit of the token above the class, zeros before ones.
+// it.  Long ones: four bits of the token above the class to a pass (a frequent token's class of 800 rows: a bit to a pass took
+// 5 us).
 __device__ __forceinline__ void gather_sort(GatherLds& s, int count, uint32_t classes, int token_bits) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   if (count <= kRankMost) {
@@ -109,43 +115,54 @@ __device__ __forceinline__ void gather_sort(GatherLds& s, int count, uint32_t cl
     return;
   }
   const int turns = (count + kGradBlock - 1) / kGradBlock;
-  for (int bit = 0; bit < token_bits; bit++) {
-    const uint32_t mask = classes << bit;
-    int32_t row[kGatherTurns], t[kGatherTurns], before[kGatherTurns];
+  for (int shift = 31 - __builtin_clz(classes), end = shift + token_bits; shift < end; shift += 4) {
+    int32_t row[kGatherTurns], t[kGatherTurns], rank[kGatherTurns];
 #pragma unroll
     for (int q = 0; q < kGatherTurns; q++) {
       if (q >= turns) break;
       const int i = q * kGradBlock + threadIdx.x;
-      t[q] = i < count ? s.token[i] : -1;   // behind the list: counted as ones, never written
+      t[q] = i < count ? s.token[i] : 0;
       row[q] = i < count ? s.row[i] : 0;
-      const uint64_t zeros = __ballot(i < count && !((uint32_t)t[q] & mask));
-      before[q] = __builtin_popcountll(zeros & ((1ull << lane) - 1));
-      if (lane == 0) s.votes[q * kGradWaves + wave] = __builtin_popcountll(zeros);
+      // the wavefront's entries of this thread's digit, and (lanes 0 to 15) those of the digit `lane`
+      uint64_t same = __ballot(i < count), of_lane = same;
+#pragma unroll
+      for (int b = 0; b < 4; b++) {
+        const bool bit = (t[q] >> (shift + b)) & 1;
+        const uint64_t votes = __ballot(bit);
+        same &= bit ? votes : ~votes;
+        of_lane &= (lane >> b) & 1 ? votes : ~votes;
+      }
+      rank[q] = __builtin_popcountll(same & ((1ull << lane) - 1));
+      if (lane < 16) s.digits[lane][q * kGradWaves + wave] = __builtin_popcountll(of_lane);
     }
     __syncthreads();
-    int sum = 0, ahead[kGatherTurns];
+    {   // a wavefront to a digit: its entries in the turns and wavefronts before, two to a lane
+      const int2 v = lane * 2 < turns * kGradWaves ? *reinterpret_cast<const int2*>(&s.digits[wave][lane * 2]) : int2{0, 0};
+      int inclusive = v.x + v.y;
 #pragma unroll
-    for (int q = 0; q < kGatherTurns; q++) {
-      if (q >= turns) break;
-      // zeros of this turn's wavefronts before this one, and of the turns before
-      const int v = lane < kGradWaves ? s.votes[q * kGradWaves + lane] : 0;
-      int inclusive = v;
-#pragma unroll
-      for (int o = 1; o < kGradWaves; o <<= 1) {
+      for (int o = 1; o < kWave; o <<= 1) {
         const int other = __shfl_up(inclusive, o);
         inclusive += lane >= o ? other : 0;
       }
-      ahead[q] = sum + __builtin_amdgcn_readlane(inclusive, wave) - __builtin_amdgcn_readlane(v, wave);
-      sum += __builtin_amdgcn_readlane(inclusive, kGradWaves - 1);
+      if (lane * 2 < turns * kGradWaves)
+        *reinterpret_cast<int2*>(&s.digits[wave][lane * 2]) = int2{inclusive - v.x - v.y, inclusive - v.y};
+      if (lane == kWave - 1) s.votes[wave] = inclusive;
     }
     __syncthreads();
+    const int all = lane < 16 ? s.votes[lane] : 0;
+    int below = all;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      const int other = __shfl_up(below, o);
+      below += lane >= o ? other : 0;
+    }
+    below -= all;   // lanes 0 to 15: entries of smaller digits
 #pragma unroll
     for (int q = 0; q < kGatherTurns; q++) {
       if (q >= turns) break;
-      const int i = q * kGradBlock + threadIdx.x;
-      if (i < count) {
-        const int zeros = ahead[q] + before[q];
-        const int at = ((uint32_t)t[q] & mask) ? sum + i - zeros : zeros;
+      const int digit = (t[q] >> shift) & 15;
+      const int at = __shfl(below, digit) + s.digits[digit][q * kGradWaves + wave] + rank[q];
+      if (q * kGradBlock + (int)threadIdx.x < count) {
         s.row[at] = row[q];
         s.token[at] = t[q];
       }
@@ -162,14 +179,45 @@ __global__ __launch_bounds__(kGradBlock) void embedding_gradient_kernel(Embeddin
   const int64_t per_row = p.dim / V;   // vectors of a row
   __shared__ GatherLds s;
   __shared__ fv part[kGradWaves][2][kWave];   // sums of tokens whose rows began before a wavefront's run, or go on behind it
-  const uint32_t mine = blockIdx.x;
+  const uint32_t mine = blockIdx.x & (p.classes - 1);
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  // the wavefronts: `across` of them side by side along the columns, `runs` runs of the list
-  const int64_t slices = (per_row + kWave - 1) / kWave;
+  // this workgroup's columns, in slices of 64 vectors; the wavefronts: `across` of them side by side along the columns,
+  // `runs` runs of the list
+  const int64_t all_slices = (per_row + kWave - 1) / kWave, per_part = (all_slices + p.parts - 1) / p.parts;
+  const int64_t slice0 = blockIdx.x / p.classes * per_part;
+  const int64_t slices = all_slices - slice0 < per_part ? all_slices - slice0 : per_part;
   const int across = slices < kGradWaves ? (int)slices : kGradWaves, runs = kGradWaves / across;
   const int me = wave / across;   // this wavefront's run; runs and more: none
   const uint64_t below = (1ull << lane) - 1;
+  // The positions' workgroups: vectors of dwpe's first seq rows, `shares` threads to a vector (many short sentences), whose
+  // sums meet in LDS.
+  const uint32_t gather_units = p.classes * p.parts;
+  if (blockIdx.x >= gather_units) {
+    fv* meet = &part[0][0][0];
+    const int vecs = kGradBlock / p.shares, mine_of = threadIdx.x / vecs;
+    const int64_t stride = (int64_t)(gridDim.x - gather_units) * vecs, step = p.seq * p.dim;
+    for (int64_t first = (int64_t)(blockIdx.x - gather_units) * vecs; first < p.seq * per_row; first += stride) {
+      const int64_t i = first + threadIdx.x % vecs;
+      fv sum = {};
+      if (i < p.seq * per_row) {
+        const float* q = p.dout + i * V;
+#pragma unroll 8
+        for (int64_t n = mine_of * step; n < p.rows * p.dim; n += p.shares * step) sum += *reinterpret_cast<const fv*>(q + n);
+      }
+      if (p.shares > 1) {
+        meet[threadIdx.x] = sum;
+        __syncthreads();
+        for (int w = 1; w < p.shares && mine_of == 0; w++) sum += meet[w * vecs + threadIdx.x];
+        __syncthreads();
+      }
+      if (mine_of == 0 && i < p.seq * per_row) {
+        fv* out = reinterpret_cast<fv*>(p.dwpe + i * V);
+        *out = *out + sum;
+      }
+    }
+    return;
+  }
   // this thread's four ids of the step that begins at row `at`; fetched a step ahead
   float ids[4];
   auto fetch = [&](int64_t at) {
@@ -179,30 +227,6 @@ __global__ __launch_bounds__(kGradBlock) void embedding_gradient_kernel(Embeddin
   };
   int64_t next = 0;   // rows looked at so far
   fetch(0);
-  // This workgroup's share of the positions: vectors of dwpe's first seq rows, `shares` threads to a vector (many short
-  // sentences), whose sums meet in LDS.
-  fv* meet = &part[0][0][0];
-  const int vecs = kGradBlock / p.shares, mine_of = threadIdx.x / vecs;
-  for (int64_t first = (int64_t)blockIdx.x * vecs; first < p.seq * per_row; first += (int64_t)p.classes * vecs) {
-    const int64_t i = first + threadIdx.x % vecs;
-    const int64_t step = p.seq * p.dim;
-    fv sum = {};
-    if (i < p.seq * per_row) {
-      const float* q = p.dout + i * V;
-#pragma unroll 8
-      for (int64_t n = mine_of * step; n < p.rows * p.dim; n += p.shares * step) sum += *reinterpret_cast<const fv*>(q + n);
-    }
-    if (p.shares > 1) {
-      meet[threadIdx.x] = sum;
-      __syncthreads();
-      for (int w = 1; w < p.shares && mine_of == 0; w++) sum += meet[w * vecs + threadIdx.x];
-      __syncthreads();
-    }
-    if (mine_of == 0 && i < p.seq * per_row) {
-      fv* out = reinterpret_cast<fv*>(p.dwpe + i * V);
-      *out = *out + sum;
-    }
-  }
   while (next < p.rows) {
     // keep rows of this class while another step's fit
     int count = 0;
@@ -246,8 +270,8 @@ __global__ __launch_bounds__(kGradBlock) void embedding_gradient_kernel(Embeddin
     const int e0 = first_of(me), e1 = me < runs ? first_of(me + 1) : e0;
     auto same = [&](int e) { return e > 0 && e < count && s.token[e] == s.token[e - 1]; };   // e belongs to the token before it
     for (int64_t turn = 0; turn < slices; turn += across) {   // the same number of turns for every wavefront
-      const int64_t vec = (turn + wave % across) * kWave + lane;
-      const bool column = vec < per_row;
+      const int64_t vec = (slice0 + turn + wave % across) * kWave + lane;
+      const bool column = turn + wave % across < slices && vec < per_row;
       const int64_t c = (column ? vec : per_row - 1) * V;   // lanes behind the row read its last vector and write nothing
       if (e0 < e1) {
         bool lead = same(e0);   // the run's first token began before it
@@ -372,14 +396,20 @@ WF2_API int wf2hip_embedding_gradient_f32(long rows, long seq, long dim, const f
       if (meet(o, i)) return fail(WF2HIP_EOVERLAP, "%s: a table's gradient overlaps an input", name);
   if (meet(out[0], out[1])) return fail(WF2HIP_EOVERLAP, "%s: the tables' gradients overlap", name);
   const bool vec = dim % 4 == 0 && ((uintptr_t)dout | (uintptr_t)dwte | (uintptr_t)dwpe) % 16 == 0;
-  EmbeddingGradient p{ctx, dout, dwte, dwpe, rows, seq, dim, (int32_t)vocab, 1, 0, 1};
-  // about sixteen rows to a class, at most a class per compute unit: every workgroup reads all the ids
-  while (p.classes < 256 && (int64_t)p.classes * 16 < rows) p.classes *= 2;
+  EmbeddingGradient p{ctx, dout, dwte, dwpe, rows, seq, dim, (int32_t)vocab, 1, 1, 0, 1};
+  // Up to four workgroups to a class, which share out the columns: a frequent token's rows are then read by as many compute
+  // units.  About sixteen rows to a workgroup, at most one per compute unit: every workgroup reads all the ids.  Eight
+  // sentences of 1024 tokens of a text, dim 768: 28.1 us with one workgroup to a class, 25.3 with three, 22.3 with the
+  // positions in workgroups of their own as well (they ran ahead of the classes in the same ones).
+  const int64_t vectors = vec ? dim / 4 : dim, slices = ceil_div(vectors, kWave);
+  p.parts = (uint32_t)ceil_div(slices, ceil_div(slices, std::min<int64_t>(slices, 4)));
+  while (p.classes * 2 * p.parts <= 256 && (int64_t)p.classes * p.parts * 16 < rows) p.classes *= 2;
   while (((int64_t)p.classes << p.token_bits) < vocab) p.token_bits++;
   while (p.shares < 16 && (int64_t)p.shares * 16 * seq < rows) p.shares *= 2;   // at most sixteen sentences to a thread
+  const uint32_t units = p.classes * p.parts + (uint32_t)std::min<int64_t>(128, ceil_div(seq * vectors, kGradBlock / p.shares));
   if (vec)
-    embedding_gradient_kernel<true><<<p.classes, kGradBlock, 0, rt().stream>>>(p);
+    embedding_gradient_kernel<true><<<units, kGradBlock, 0, rt().stream>>>(p);
   else
-    embedding_gradient_kernel<false><<<p.classes, kGradBlock, 0, rt().stream>>>(p);
+    embedding_gradient_kernel<false><<<units, kGradBlock, 0, rt().stream>>>(p);
   return after_launch("embedding_gradient_kernel");
 }
