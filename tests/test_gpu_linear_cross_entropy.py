@@ -295,6 +295,17 @@ def test_replayed_graph_equals_eager(gpu, rows, dim, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,vocab", [(2049, 5, 33), (9000, 12, 40)])
+@pytest.mark.parametrize("route", ["0", "1", "2"])
+@pytest.mark.parametrize("left_out", [0.3, 1.0])
+def test_many_rows_of_a_small_vocabulary(gpu, rows, dim, vocab, route, left_out, monkeypatch):
+    """So many rows that the number of those with a label is counted by a launch of its own."""
+    monkeypatch.setenv("WF2HIP_XENT_ROUTE", route)
+    x, w, labels = inputs(rows, dim, vocab, left_out=left_out)
+    check(gpu, x, w, labels, "mean", 0.5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,dim,vocab", [(16500, 24, 20003), (262000, 260, 3211)])
 def test_vocabulary_in_pieces(gpu, rows, dim, vocab):
     """More than 2^28 elements of ds: the backward walks the vocabulary in pieces; in the second case dx's shares of all
