@@ -256,7 +256,8 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamwArgs<BITS> a) {
   for (int t = 0; t < AdamwArgs<BITS>::kTensors; t += kWave)
     at += __builtin_popcountll(__ballot(t + lane < a.count && a.first[t + lane < a.count ? t + lane : 0] <= blockIdx.x));
   at = __builtin_amdgcn_readfirstlane(at);
-  AdamwTensor t{a.p[at], a.g[at], a.m[at], a.v[at], a.m_scale[BITS == 8 ? at : 0], a.r_scale[BITS == 8 ? at : 0], a.n[at], (blockIdx.x - a.first[at]) * (uint32_t)kAdamwChunk};
+  AdamwTensor t{a.p[at], a.g[at], a.m[at], a.v[at], a.m_scale[BITS == 8 ? at : 0], a.r_scale[BITS == 8 ? at : 0], a.n[at],
+                (blockIdx.x - a.first[at]) * (uint32_t)kAdamwChunk};
   const double lr = a.lr_at ? (double)a.lr_at[0] : a.lr;
   const float weight_decay = a.decay[at];
   // What the step's number gives, in binary64: b^t from the product that the states carry along.  The last workgroup to
@@ -338,7 +339,8 @@ WF2_API int wf2hip_adamw_step(const wf2hip_adamw_desc* d, long count, const wf2h
   const char* name = "adamw step";
   WF2_TRY(require_init());
   if (!d || count < 0 || (count && !tensors) || !steps) return fail(WF2HIP_EINVAL, "%s: null pointer or negative count", name);
-  if (d->state_bits != 8 && d->state_bits != 32) return fail(WF2HIP_EINVAL, "%s: states have 8 or 32 bits, not %d", name, d->state_bits);
+  if (d->state_bits != 8 && d->state_bits != 32)
+    return fail(WF2HIP_EINVAL, "%s: states have 8 or 32 bits, not %d", name, d->state_bits);
   if (!(d->beta1 >= 0.0 && d->beta1 < 1.0 && d->beta2 >= 0.0 && d->beta2 < 1.0))
     return fail(WF2HIP_EINVAL, "%s: decay rates must be in [0, 1)", name);
   const bool bytes8 = d->state_bits == 8;
@@ -357,8 +359,10 @@ WF2_API int wf2hip_adamw_step(const wf2hip_adamw_desc* d, long count, const wf2h
       const wf2hip_adamw_tensor& t = tensors[i];
       if (t.n < 0) return fail(WF2HIP_EINVAL, "%s: tensor %ld has a negative element count", name, i);
       if (t.n == 0) continue;
-      if (!t.param || !t.grad || !t.m || !t.v || (bytes8 && (!t.m_scale || !t.r_scale))) return fail(WF2HIP_EINVAL, "%s: null pointer in tensor %ld", name, i);
-      if (t.n >= ((int64_t)1 << 32) - kAdamwChunk) return fail(WF2HIP_EUNSUPPORTED, "%s: tensor %ld has 2^32 elements or more", name, i);
+      if (!t.param || !t.grad || !t.m || !t.v || (bytes8 && (!t.m_scale || !t.r_scale)))
+        return fail(WF2HIP_EINVAL, "%s: null pointer in tensor %ld", name, i);
+      if (t.n >= ((int64_t)1 << 32) - kAdamwChunk)
+        return fail(WF2HIP_EUNSUPPORTED, "%s: tensor %ld has 2^32 - 4096 elements or more", name, i);
       if ((((uintptr_t)t.param | (uintptr_t)t.grad) & 3) || (!bytes8 && (((uintptr_t)t.m | (uintptr_t)t.v) & 3)) ||
           (bytes8 && (((uintptr_t)t.m_scale | (uintptr_t)t.r_scale) & 3)))
         return fail(WF2HIP_EINVAL, "%s: misaligned pointer in tensor %ld", name, i);

@@ -385,7 +385,8 @@ WF2_API int wf2hip_embedding_gradient_f32(long rows, long seq, long dim, const f
   if (seq < 1 || rows % seq != 0) return fail(WF2HIP_EINVAL, "%s: rows %ld is not a multiple of the sentence length %ld", name, rows, seq);
   if (seq > n_ctx) return fail(WF2HIP_EINVAL, "%s: sentence length %ld beyond the %ld positions of dwpe", name, seq, n_ctx);
   if (vocab < 1) return fail(WF2HIP_EINVAL, "%s: empty token table", name);
-  if (rows >= INT32_MAX - 2 * kGather || vocab >= ((int64_t)1 << 30) || dim > ((int64_t)1 << 28)) return fail(WF2HIP_EUNSUPPORTED, "%s: 2^31 rows, 2^30 words, or rows of more than 2^28 elements", name);
+  if (rows >= INT32_MAX - 2 * kGather || vocab >= ((int64_t)1 << 30) || dim > ((int64_t)1 << 28))
+    return fail(WF2HIP_EUNSUPPORTED, "%s: 2^31 rows, 2^30 words, or rows of more than 2^28 elements", name);
   const struct {
     const float* at;
     int64_t n;

@@ -11,8 +11,10 @@
 //             row behind, which a second kernel folds over the tiles of the vocabulary;
 //   backward  the vocabulary is walked in pieces: a piece's logits are formed anew and leave as ds, from which the
 //             piece's rows of dw and its share of dx are formed.
-// All products run on the 16-bit matrix cores on pairs of binary16 numbers (wf2_pairs.h): they are what bounds the
-// operator beyond a few hundred rows.
+// All products run on the 16-bit matrix cores, on pairs of binary16 numbers (wf2_pairs.h) or, few rows and small products,
+// on three bfloat16 parts (wf2_direct.h): beyond a few hundred rows they are what bounds the operator.  8192 x 768 x 50257:
+// forward 1.63 ms = 388 Tflop/s (three passes: 1165), with the gradients 6.8 - 7.1 ms = 370; a library's binary16 product of 8192^3
+// reaches 1148 here.  The matrix cores are then busy 71 % of the time at 1.6 GHz: power.
 #include <stdlib.h>
 
 #include <algorithm>
@@ -551,8 +553,8 @@ __device__ __forceinline__ void tile_dw(const XentGradient& p, uint32_t share, i
 }
 
 // Both products of a piece in one launch, so that neither has a last round of its own: the tiles with the longer K first
-// (dw's K are the rows of x, dx's the words; either in shares where there are few tiles).  A tile that overhangs the columns by more than half runs as a
-// narrower one.
+// (dw's K are the rows of x, dx's the words; either in shares where there are few tiles).  A tile that overhangs the
+// columns by half or more runs as a narrower one.
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void xent_tile_gradients(XentGradient p) {
   __shared__ __attribute__((aligned(16))) char smem[kRing * kStage];
   const uint32_t dw_tiles = p.tiles_w * p.tiles_d, dx_tiles = p.tiles_x * p.tiles_d;
@@ -1019,7 +1021,8 @@ static int fold_gradients(const XentPlanes& x, const XentPlanes& w, int64_t dim,
   const bool vec = dim % 4 == 0 && ((uintptr_t)x.out | (uintptr_t)w.out) % 16 == 0;
   const int64_t per = vec ? 4 : 1, gx = ceil_div(x.n / per, kBlock), gw = ceil_div(w.n / per, kBlock);
   if (gx + gw == 0) return 0;
-  if (gx + gw >= ((int64_t)1 << 31)) return fail(WF2HIP_EUNSUPPORTED, "linear cross entropy backward: too many elements for one launch");
+  if (gx + gw >= ((int64_t)1 << 31))
+    return fail(WF2HIP_EUNSUPPORTED, "linear cross entropy backward: too many elements for one launch");
   if (vec)
     xent_fold_gradients<true><<<(uint32_t)(gx + gw), kBlock, 0, st>>>(x, w, (uint32_t)gx, dim, g);
   else
@@ -1053,21 +1056,13 @@ static XentRoute xent_route(int64_t rows, int64_t dim, int64_t vocab, bool backw
 // Width of a tile in blocks of 32: no wider than the operand, `most` where that is longer.
 static int xent_blocks(int64_t extent, int most) { return extent <= 32 ? 1 : extent <= 64 || most == 2 ? 2 : 4; }
 
-// Whether the gradients' tiles are 128 wide (a wavefront each for 32 of them) or 32 (a quarter of K each).
-static bool xent_wide_gradients(XentRoute route, int64_t rows, int64_t dim, int64_t vocab) {
-  if (const char* env = getenv("WF2HIP_XENT_ROUTE"))
-    if (env[0] == '1' || env[0] == '2') return env[0] == '1';
-  return route == kSkinny;
-}
-
 static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int64_t vocab, const float* x, const float* w,
                                 const int32_t* labels, const float* lse, int reduction, const float* dloss, float scale,
                                 float* dx, float* dw) {
   hipStream_t st = rt().stream;
   const bool small = route == kSmall;
   const int nb = xent_blocks(rows, small ? 2 : 4);
-  // the gradients have tiles of their own: 128 wide where those fill the device
-  const bool wide = xent_wide_gradients(route, rows, dim, vocab);
+  const bool wide = !small;   // the gradients' tiles: 128 wide (a wavefront each for 32), or 32 (a quarter of K each)
   const int nbw = wide ? xent_blocks(dim, 4) : 1, nbx = xent_blocks(rows, wide ? 4 : 2);
   XentDirect p{};
   p.x = x; p.w = w; p.labels = labels;
@@ -1141,7 +1136,7 @@ static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int6
 template <bool PER_ROW>
 static int split_operands(const XentSplit& p, hipStream_t st) {
   const uint32_t blocks = p.wblocks + (uint32_t)ceil_div(p.rows, 32);
-  // rows read twice without a register copy: 100 us for the (50257, 768) table where one read takes 64
+  // rows read twice without a register copy: 100 us for the (50257, 768) table where one read takes 70
   if (PER_ROW && p.dim <= 256)
     xent_split<PER_ROW, 4><<<blocks, kBlock, 0, st>>>(p);
   else if (PER_ROW && p.dim <= 512)

@@ -204,7 +204,8 @@ __device__ __forceinline__ void skinny_product(const DirectMatrix& A, const Dire
     if (BT) {
 #pragma unroll
       for (int c = 0; c < 4; c++)
-        put_parts(at + (bi >> 5) * kDirectHalf, (bi & 31) + c, bk >> 2, bv[0][c], bv[BT ? 1 : 0][c], bv[BT ? 2 : 0][c], bv[BT ? 3 : 0][c]);
+        put_parts(at + (bi >> 5) * kDirectHalf, (bi & 31) + c, bk >> 2, bv[0][c], bv[BT ? 1 : 0][c], bv[BT ? 2 : 0][c],
+                  bv[BT ? 3 : 0][c]);
     } else {
 #pragma unroll
       for (int u = 0; u < kUnits; u++)

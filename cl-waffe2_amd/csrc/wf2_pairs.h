@@ -36,9 +36,10 @@ struct PairMatrix {
   __host__ __device__ int64_t pitch() const { return (int64_t)col_blocks * kPiece; }
 };
 
-// One workgroup's 128 x 64 NB tile of C[m][n] = sum_k A(m, k) B(n, k), NB = 4 (2 and 1 at the end of a matrix that leaves most of
-// a tile empty): four wavefronts, each 64 x 32 NB as 2 x NB blocks of 32 x 32; two workgroups to a compute unit, so that one's prologue and epilogue run under the
-// other's products.  K steps of 16 arrive by DMA in a ring of three stages of 24 KB, two steps ahead.
+// One workgroup's 128 x 64 NB tile of C[m][n] = sum_k A(m, k) B(n, k), NB = 4 (2 and 1 at the end of a matrix that leaves
+// most of a tile empty): four wavefronts, each 64 x 32 NB as 2 x NB blocks of 32 x 32; two workgroups to a compute unit, so
+// that one's prologue and epilogue run under the other's products.  K steps of 16 arrive by DMA in a ring of three stages of
+// 24 KB, two steps ahead.
 // AT / BT: k runs along the rows of that operand's storage instead of its columns.
 // LOUD: the lo parts of A are stored 2^11 times too large (numbers of a wide range: dozens of octaves below the
 // largest still keep 22 bits); their partner is scaled down in registers, exactly unless it is 2^18 times below its

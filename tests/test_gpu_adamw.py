@@ -332,6 +332,30 @@ def test_extreme_sizes(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_empty_parameters_and_shared_gradients(gpu, bits):
+    """Parameters without elements change nothing for the others; a gradient may serve two parameters; no parameters at all
+    are no step."""
+    W = gpu
+    O = W.optimizers
+    a, b, _, _ = numbers(300, 5)
+    alone, shared = tensors(W, [a, b]), tensors(W, [a, a, b])
+    one = O.AdamW(alone[:1], state_bits=bits, **HYPER)
+    two = O.AdamW([W.HIPTensor([0])] + shared[:2] + [W.HIPTensor([3, 0])], state_bits=bits, **HYPER)
+    for _ in range(3):
+        one.step([alone[1]])
+        two.step([W.HIPTensor([0]), shared[2], shared[2], W.HIPTensor([3, 0])])
+    assert one.n == two.n == 3
+    for p in shared[:2]:
+        assert np.array_equal(p.numpy(), alone[0].numpy())
+    none = O.AdamW([], state_bits=bits, **HYPER)
+    none.step([])
+    assert none.n == 0
+    with pytest.raises(W.lib.HIPError):   # a parameter twice: both would write it
+        O.AdamW([shared[0], shared[0]], state_bits=bits, **HYPER).step([shared[2], shared[2]])
+
+
+@pytest.mark.gpu
 def test_argument_checks(gpu):
     W = gpu
     O, lib = W.optimizers, W.lib

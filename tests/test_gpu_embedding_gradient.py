@@ -87,6 +87,26 @@ def test_more_rows_of_a_class_than_its_lists_hold(gpu, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,t,vocab,n_ctx,dim", [(4, 300, 50, 300, 1600), (2, 500, 3000, 512, 1284), (3, 40, 9, 40, 401),
+                                                 (20, 500, 4000, 500, 260), (3, 70, 500, 70, 2052)])
+def test_columns_shared_out(gpu, n, t, vocab, n_ctx, dim):
+    """Rows of several slices of 64 vectors (64 elements where a row is no multiple of 16 bytes), which up to four
+    workgroups share: two, three and four of them, equal and unequal shares."""
+    check(gpu, *numbers(n, t, vocab, n_ctx, dim))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("distinct", [2, 17, 4096])
+def test_long_lists_of_many_tokens(gpu, distinct):
+    """9600 rows of one class whose tokens differ in up to twelve bits above those of the class."""
+    ids, dout, dwte, dwpe = numbers(16, 600, (1 << 20) + 3, 600, 4)
+    ids[:] = 1 + 256 * np.random.default_rng(distinct).integers(0, distinct, ids.shape)
+    check(gpu, ids, dout, dwte, dwpe)
+    ids[:] = np.random.default_rng(distinct).integers(0, (1 << 20) + 3, ids.shape)
+    check(gpu, ids, dout, dwte, dwpe)
+
+
+@pytest.mark.gpu
 def test_ids_are_read_as_the_forward_reads_them(gpu):
     ids, dout, dwte, dwpe = numbers(1, 11, 10, 16, 8)
     ids[0] = [0.5, 1.5, 2.5, 3.49, 8.6, 9.0, 42.0, -3.0, np.nan, np.inf, -np.inf]
