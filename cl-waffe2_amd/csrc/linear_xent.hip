@@ -810,12 +810,21 @@ __global__ __launch_bounds__(kBlock) void xent_small_loss(XentDirect p) {
   if (threadIdx.x == 0) __hip_atomic_store(&g_xent_arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   const uint32_t tiles = gridDim.x / p.tiles_n;
   double total = 0.0, held = 0.0;
-  for (int64_t r = threadIdx.x; r < p.rows; r += kBlock) {
+  int per_row = 1;   // threads to a row
+  while (per_row < kWave && per_row * 2 * p.rows <= kBlock) per_row *= 2;
+  for (int64_t r0 = 0; r0 < p.rows; r0 += kBlock / per_row) {
+    const int64_t r = r0 + threadIdx.x / per_row;
+    const uint32_t first = threadIdx.x & (per_row - 1);
     float top = -INFINITY, sum = 0.0f;
+    if (r < p.rows) {
 #pragma unroll 4
-    for (uint32_t t = 0; t < tiles; t++)
-      fold_in(top, sum, __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<unsigned long long*>(&p.part[(int64_t)t * p.rows + r]),
-                                                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)));
+      for (uint32_t t = first; t < tiles; t += per_row) {
+        unsigned long long* q = reinterpret_cast<unsigned long long*>(&p.part[(int64_t)t * p.rows + r]);
+        fold_in(top, sum, __builtin_bit_cast(float2, __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)));
+      }
+    }
+    for (int o = 1; o < per_row; o <<= 1) fold_in(top, sum, float2{__shfl_xor(top, o), __shfl_xor(sum, o)});
+    if (r >= p.rows || first != 0) continue;
     const float l = top + logf(sum);
     const int32_t label = p.labels[r];
     p.lse_out[r] = l;
@@ -955,8 +964,8 @@ __global__ __launch_bounds__(kBlock) void xent_direct_gradients(XentDirect p) {
   }
 }
 
-// Tiles times rows up to which the last workgroup finishes a small call.
-constexpr int64_t kLastMost = 4096;
+// Tiles times rows, and tiles, up to which the last workgroup finishes a small call.
+constexpr int64_t kLastMost = 4096, kLastTiles = 512;
 
 // ---- host -----------------------------------------------------------------------------------------------------
 
@@ -1044,13 +1053,15 @@ static XentRoute xent_route(int64_t rows, int64_t dim, int64_t vocab, bool backw
     if (env[0] >= '0' && env[0] <= '2') return (XentRoute)(env[0] - '0');
   // Measured (us, kPairs / kSkinny / kSmall; rows x dim x vocab):
   //   forward   256 x 768 x 1000  48 / 46 / 17    1000 x 400 x 2000 24 / 34 / 25    256 x 768 x 8192  37 / 50 / 46
-  //             16 x 1600 x 20000 98 / 56 / 37    61 x 768 x 50257  88 / 53 / 73    128 x 768 x 50257 102 / 85 / 129
-  //             256 x 768 x 50257 123 / 143 / 213
+  //             16 x 768 x 50257  91 / 53 / 48    61 x 768 x 50257  88 / 53 / 73    128 x 768 x 50257 102 / 85 / 129
+  //             1 x 768 x 50257   90 / 52 / 40    256 x 768 x 50257 123 / 143 / 213
   //   backward  256 x 768 x 1000  92 / 83 / 53    400 x 200 x 3000  78 / 94 / 75    1000 x 400 x 2000 86 / 105 / 154
-  //             16 x 1600 x 20000 198 / 149 / 263 61 x 768 x 50257  240 / 208 / 676 64 x 768 x 8192   61 / 70 / 117
-  const double work = (double)rows * (double)dim * (double)vocab;   // may pass 2^63
-  if (work <= (backward ? 0x1p28 : 0x3p28)) return kSmall;
-  return backward ? (rows <= 64 && vocab * dim >= ((int64_t)1 << 24) ? kSkinny : kPairs) : rows <= 160 ? kSkinny : kPairs;
+  //             1 x 768 x 50257   226 / 147 / 298 61 x 768 x 50257  240 / 208 / 676 64 x 768 x 8192   61 / 70 / 117
+  //             5 x 267 x 31873   76 / 55 / 92    16 x 256 x 16384  54 / 43 / 49    2 x 256 x 8192    51 / 38 / 29
+  const double work = (double)rows * (double)dim * (double)vocab, table = (double)dim * (double)vocab;   // may pass 2^63
+  if (!backward) return work <= 0x3p28 ? kSmall : rows <= 160 ? kSkinny : kPairs;
+  if (rows <= 64 && table >= (work <= 0x1p28 ? 0x1p22 : 0x1p24)) return kSkinny;
+  return work <= 0x1p28 ? kSmall : kPairs;
 }
 
 // Width of a tile in blocks of 32: no wider than the operand, `most` where that is longer.
@@ -1174,7 +1185,7 @@ WF2_API int wf2hip_linear_cross_entropy_f32(long rows, long dim, long vocab, con
   const int64_t tiles_n = ceil_div(rows, 32 * nb);
   if (tiles_v * tiles_n >= ((int64_t)1 << 31)) return fail(WF2HIP_EUNSUPPORTED, "%s: too many tiles for one launch", name);
   const uint32_t folds = (uint32_t)(rows <= kFoldRows ? rows : ceil_div(rows, kWave));
-  const bool one_launch = route == kSmall && tiles_v * rows <= kLastMost;
+  const bool one_launch = route == kSmall && tiles_v * rows <= kLastMost && tiles_v * tiles_n <= kLastTiles;
   float2* part = blocks.take<float2>(tiles_v * rows * 8);
   float* at = blocks.take<float>(rows * (int64_t)4);
   XentSum* total = one_launch ? nullptr : blocks.take<XentSum>(sizeof(XentSum));

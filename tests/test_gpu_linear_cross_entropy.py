@@ -295,6 +295,16 @@ def test_replayed_graph_equals_eager(gpu, rows, dim, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,vocab", [(1, 40, 12000), (1, 40, 20000), (2, 24, 16000), (5, 267, 8000), (100, 16, 1000),
+                                            (130, 16, 900), (1, 768, 8192)])
+@pytest.mark.parametrize("reduction", ["mean", None])
+def test_few_rows_of_a_large_vocabulary(gpu, rows, dim, vocab, reduction):
+    """Single tokens and a few: the statistics of a row come from many tiles, by one thread or up to 64."""
+    x, w, labels = inputs(rows, dim, vocab)
+    check(gpu, x, w, labels, reduction, None if reduction else np.linspace(0.5, 2.0, rows).astype(f32))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,dim,vocab", [(2049, 5, 33), (9000, 12, 40)])
 @pytest.mark.parametrize("route", ["0", "1", "2"])
 @pytest.mark.parametrize("left_out", [0.3, 1.0])
