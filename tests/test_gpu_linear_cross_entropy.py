@@ -305,6 +305,15 @@ def test_few_rows_of_a_large_vocabulary(gpu, rows, dim, vocab, reduction):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,vocab", [(520, 20, 22000), (1000, 9, 17003), (200, 33, 35001)])
+def test_a_last_round_of_narrower_tiles(gpu, rows, dim, vocab, monkeypatch):
+    """A few tiles more than the device holds at a time: the ones behind run as two or four narrower ones."""
+    monkeypatch.setenv("WF2HIP_XENT_ROUTE", "0")
+    x, w, labels = inputs(rows, dim, vocab, left_out=0.1)
+    check(gpu, x, w, labels, "mean")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,dim,vocab", [(2049, 5, 33), (9000, 12, 40)])
 @pytest.mark.parametrize("route", ["0", "1", "2"])
 @pytest.mark.parametrize("left_out", [0.3, 1.0])
