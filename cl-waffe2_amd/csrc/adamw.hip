@@ -15,7 +15,7 @@
 // block has to span (2^17 down to the smallest code, 2^35 of v) and is what the step divides by.  The parameters take
 // the step of the unrounded moments.  A wavefront holds a block, four elements per lane.
 #include <algorithm>
-#include <new>
+#include <exception>
 #include <vector>
 
 #include "wf2_common.h"
@@ -390,7 +390,7 @@ WF2_API int wf2hip_adamw_step(const wf2hip_adamw_desc* d, long count, const wf2h
     const bool streaming = total * (bytes8 ? 16 : 28) >= ((int64_t)192 << 20);   // far beyond the Infinity Cache
     return bytes8 ? (streaming ? adamw_launches<8, true>(*d, count, tensors, steps) : adamw_launches<8, false>(*d, count, tensors, steps))
                   : (streaming ? adamw_launches<32, true>(*d, count, tensors, steps) : adamw_launches<32, false>(*d, count, tensors, steps));
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {   // of the list's memory
     return fail(WF2HIP_ENOMEM, "%s: out of host memory", name);
   }
 }
