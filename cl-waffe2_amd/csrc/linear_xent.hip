@@ -1082,13 +1082,13 @@ static XentRoute xent_route(int64_t rows, int64_t dim, int64_t vocab, bool backw
     if (env[0] >= '0' && env[0] <= '2') return (XentRoute)(env[0] - '0');
   // Measured (us, kPairs / kSkinny / kSmall; rows x dim x vocab):
   //   forward   256 x 768 x 1000  48 / 46 / 17    1000 x 400 x 2000 24 / 34 / 25    256 x 768 x 8192  37 / 50 / 46
-  //             16 x 768 x 50257  91 / 53 / 48    61 x 768 x 50257  88 / 53 / 73    128 x 768 x 50257 102 / 85 / 129
-  //             1 x 768 x 50257   90 / 52 / 40    256 x 768 x 50257 123 / 143 / 213
+  //             16 x 768 x 50257  91 / 53 / 48    61 x 768 x 50257  88 / 49 / 73    128 x 768 x 50257 112 / 85 / 131
+  //             1 x 768 x 50257   90 / 44 / 40    160 x 768 x 50257 128 / 145 / 171
   //   backward  256 x 768 x 1000  92 / 83 / 53    400 x 200 x 3000  78 / 94 / 75    1000 x 400 x 2000 86 / 105 / 154
-  //             1 x 768 x 50257   226 / 147 / 298 61 x 768 x 50257  240 / 208 / 676 64 x 768 x 8192   61 / 70 / 117
+  //             1 x 768 x 50257   226 / 150 / 298 61 x 768 x 50257  242 / 203 / 684 61 x 768 x 8192   66 / 63 / 125
   //             5 x 267 x 31873   76 / 55 / 92    16 x 256 x 16384  54 / 43 / 49    2 x 256 x 8192    51 / 38 / 29
   const double work = (double)rows * (double)dim * (double)vocab, table = (double)dim * (double)vocab;   // may pass 2^63
-  if (!backward) return work <= 0x3p28 ? kSmall : rows <= 160 ? kSkinny : kPairs;
+  if (!backward) return work <= 0x3p28 ? kSmall : rows <= 128 ? kSkinny : kPairs;
   if (rows <= 64 && table >= (work <= 0x1p28 ? 0x1p22 : 0x1p24)) return kSkinny;
   return work <= 0x1p28 ? kSmall : kPairs;
 }

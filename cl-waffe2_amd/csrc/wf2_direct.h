@@ -58,6 +58,20 @@ __device__ __forceinline__ void put_parts(char* half, int i, int g, float a, flo
   *reinterpret_cast<u2*>(q + kDirectPart) = u2{pack(two[0], two[1]), pack(two[2], two[3])};
   *reinterpret_cast<u2*>(q + 2 * kDirectPart) = u2{pack(three[0], three[1]), pack(three[2], three[3])};
 }
+
+// The first `there` of four numbers, zeros behind them.
+__device__ __forceinline__ f4 first_of(const float* q, int64_t there) {
+  f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (there >= 4) {
+    v = *reinterpret_cast<const f4u*>(q);
+  } else if (there > 0) {
+    v[0] = q[0];
+    if (there > 1) v[1] = q[1];
+    if (there > 2) v[2] = q[2];
+  }
+  return v;
+}
+
 // ---- a long operand against a short one ----------------------------------------------------------------------
 //
 // A 128 x 32 NB tile of C[m][n] = sum_k A(m, k) B(n, k): a wavefront has 32 rows of A and all of the tile's columns.  No other
@@ -136,7 +150,9 @@ __device__ __forceinline__ void skinny_product(const DirectMatrix& A, const Dire
     }
   }
   const int64_t bstep = BT ? kDirectStep * B.ld : kDirectStep;
-  const int32_t* live = BT && B.live ? B.live + bk : nullptr;
+  constexpr bool LIVE = BT && !AT;                               // the one operand whose rows may be left out
+  const int32_t* live = LIVE ? B.live + bk : nullptr;
+  int32_t kept[LIVE ? kUnits : 1];
   const bool columns = !BT || n0 + 32 * NB <= B.rows;            // uniform
   f4 av[2][4], bv[kUnits];
   auto fetch_a = [&](auto set, auto whole, int64_t left) {
@@ -147,10 +163,8 @@ __device__ __forceinline__ void skinny_product(const DirectMatrix& A, const Dire
       if constexpr (decltype(whole)::value) {
         av[decltype(set)::value][u] = *reinterpret_cast<const f4u*>(q);
       } else {
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-          av[decltype(set)::value][u][c] =
-              (AT ? (lane >> 3) + u * 8 < left && c < a_inside : k + c + (lane >> 5) * 8 < left) ? q[c] : 0.0f;
+        const int64_t there = AT ? ((lane >> 3) + u * 8 < left ? a_inside : 0) : left - (k + (lane >> 5) * 8);
+        av[decltype(set)::value][u] = first_of(q, there);
       }
     }
     a += a_step;
@@ -186,21 +200,24 @@ __device__ __forceinline__ void skinny_product(const DirectMatrix& A, const Dire
       if constexpr (decltype(whole)::value) {
         bv[u] = *reinterpret_cast<const f4u*>(b[u]);
       } else {
-#pragma unroll
-        for (int c = 0; c < 4; c++) bv[u][c] = (BT ? bk + u < left && c < inside : bk + c < left) ? b[u][c] : 0.0f;
+        bv[u] = first_of(b[u], BT ? (bk + u < left ? inside : 0) : left - bk);
       }
       b[u] += bstep;
     }
-    if (BT && live) {
+    if (LIVE) {
 #pragma unroll
-      for (int u = 0; u < kUnits; u++)
-        if (bk + u < left && live[u] < 0) bv[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int u = 0; u < kUnits; u++) kept[u] = bk + u < left ? live[u] : -1;
       live += kDirectStep;
     }
   };
   auto store_b = [&](int buffer) {
     if (!busy) return;
     char* at = smem + buffer * NB * kDirectHalf;
+    if (LIVE) {
+#pragma unroll
+      for (int u = 0; u < kUnits; u++)
+        if (kept[u] < 0) bv[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     if (BT) {
 #pragma unroll
       for (int c = 0; c < 4; c++)
@@ -329,11 +346,19 @@ struct SmallStream {
           for (int c = 0; c < 4; c++) v[u * 4 + c] = x[c];
         }
       }
-    } else {
+    } else if (T) {
 #pragma unroll
       for (int n = 0; n < 16; n++) {
         const int k = (n >> 3) * 16 + (n & 7);
-        v[n] = k < mine ? q[T ? k * ld : k] : 0.0f;
+        v[n] = k < mine ? q[k * ld] : 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int k = (u >> 1) * 16 + (u & 1) * 4;
+        const f4 x = first_of(q + k, mine - k);
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[u * 4 + c] = x[c];
       }
     }
     if (T && live) {
