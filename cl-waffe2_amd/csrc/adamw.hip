@@ -3,7 +3,8 @@
 //   m <- m + (g - m) (1 - b1)        v <- v + (1 - b2) (g g - v)             (the reference's Adam,
 //   p <- p - lr wd p - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)     source/optimizers/impls/adam.lisp:45-117,
 //                                                                             with the decay of the weights apart)
-// Bound by HBM: 28 bytes per parameter with 32-bit states, 16 with 8-bit ones.  A model has hundreds of tensors, most of
+// Bound by HBM: 28 bytes per parameter with 32-bit states, 16 with 8-bit ones; 148 tensors of 124 M parameters: 607 us and
+// 350 us, both 5.7 TB/s.  A model has hundreds of tensors, most of
 // them vectors: one launch per tensor costs more than their work, so the tensors' addresses travel as kernel arguments
 // and a workgroup finds the tensor its 4096 elements belong to by comparing its index with every tensor's first workgroup,
 // a tensor per lane.
