@@ -1084,13 +1084,16 @@ static XentRoute xent_route(int64_t rows, int64_t dim, int64_t vocab, bool backw
   //   forward   256 x 768 x 1000  48 / 46 / 17    1000 x 400 x 2000 24 / 34 / 25    256 x 768 x 8192  37 / 50 / 46
   //             16 x 768 x 50257  91 / 53 / 48    61 x 768 x 50257  88 / 49 / 73    128 x 768 x 50257 112 / 85 / 131
   //             1 x 768 x 50257   90 / 44 / 40    160 x 768 x 50257 128 / 145 / 171
+  //             1079 x 45 x 5205  34 / 36 / 44    300 x 64 x 5000   18 / 20 / 19    20000 x 16 x 512  23 / 26 / 46
   //   backward  256 x 768 x 1000  92 / 83 / 53    400 x 200 x 3000  78 / 94 / 75    1000 x 400 x 2000 86 / 105 / 154
   //             1 x 768 x 50257   226 / 150 / 298 61 x 768 x 50257  242 / 203 / 684 61 x 768 x 8192   66 / 63 / 125
   //             5 x 267 x 31873   76 / 55 / 92    16 x 256 x 16384  54 / 43 / 49    2 x 256 x 8192    51 / 38 / 29
+  //             1079 x 45 x 5205  40 / 66 / 97    400 x 30 x 3000   31 / 45 / 27    20000 x 16 x 512  61 / 74 / 103
   const double work = (double)rows * (double)dim * (double)vocab, table = (double)dim * (double)vocab;   // may pass 2^63
-  if (!backward) return work <= 0x3p28 ? kSmall : rows <= 128 ? kSkinny : kPairs;
+  const double logits = (double)rows * (double)vocab;
+  if (!backward) return work <= 0x3p28 && logits <= 0x3p19 ? kSmall : rows <= 128 ? kSkinny : kPairs;
   if (rows <= 64 && table >= (work <= 0x1p28 ? 0x1p22 : 0x1p24)) return kSkinny;
-  return work <= 0x1p28 ? kSmall : kPairs;
+  return work <= 0x1p28 && logits <= 0x5p18 ? kSmall : kPairs;
 }
 
 // Width of a tile in blocks of 32: no wider than the operand, `most` where that is longer.
