@@ -1086,13 +1086,13 @@ static XentRoute xent_route(int64_t rows, int64_t dim, int64_t vocab, bool backw
   //             1 x 768 x 50257   90 / 44 / 40    160 x 768 x 50257 128 / 145 / 171
   //             1079 x 45 x 5205  34 / 36 / 44    300 x 64 x 5000   18 / 20 / 19    20000 x 16 x 512  23 / 26 / 46
   //   backward  256 x 768 x 1000  92 / 83 / 53    400 x 200 x 3000  78 / 94 / 75    1000 x 400 x 2000 86 / 105 / 154
-  //             1 x 768 x 50257   226 / 150 / 298 61 x 768 x 50257  242 / 203 / 684 61 x 768 x 8192   66 / 63 / 125
-  //             5 x 267 x 31873   76 / 55 / 92    16 x 256 x 16384  54 / 43 / 49    2 x 256 x 8192    51 / 38 / 29
+  //             1 x 768 x 50257   226 / 150 / 298 61 x 768 x 50257  242 / 203 / 684 64 x 768 x 8192   66 / 44 / 119
+  //             5 x 267 x 31873   76 / 60 / 92    16 x 256 x 16384  54 / 33 / 48    2 x 256 x 8192    51 / 38 / 29
   //             1079 x 45 x 5205  40 / 66 / 97    400 x 30 x 3000   31 / 45 / 27    20000 x 16 x 512  61 / 74 / 103
   const double work = (double)rows * (double)dim * (double)vocab, table = (double)dim * (double)vocab;   // may pass 2^63
   const double logits = (double)rows * (double)vocab;
   if (!backward) return work <= 0x3p28 && logits <= 0x3p19 ? kSmall : rows <= 128 ? kSkinny : kPairs;
-  if (rows <= 64 && table >= (work <= 0x1p28 ? 0x1p22 : 0x1p24)) return kSkinny;
+  if (rows <= 64 && table >= 0x1p22) return kSkinny;
   return work <= 0x1p28 && logits <= 0x5p18 ? kSmall : kPairs;
 }
 
@@ -1103,10 +1103,12 @@ static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int6
                                 const int32_t* labels, const float* lse, int reduction, const float* dloss, float scale,
                                 float* dx, float* dw) {
   hipStream_t st = rt().stream;
-  const bool small = route == kSmall;
-  const int nb = xent_blocks(rows, small ? 2 : 4);
-  const bool wide = !small;   // the gradients' tiles: 128 wide (a wavefront each for 32), or 32 (a quarter of K each)
-  const int nbw = wide ? xent_blocks(dim, 4) : 1, nbx = xent_blocks(rows, wide ? 4 : 2);
+  const int nb = xent_blocks(rows, 2), nbx = nb;
+  // ds in tiles of 32 words also where tiles of 128 would leave a quarter of the compute units idle (gradients of 8 x 768 x 8192: 53 -> 32 us)
+  const bool wide = route == kSkinny;
+  const bool small = !wide || ceil_div(vocab, kSkinnyRows) * ceil_div(rows, 32 * nb) * 4 < rt().num_cus * 3;
+  // the gradients' tiles: 128 wide (a wavefront each for 32), or 32 (a quarter of K each)
+  const int nbw = wide ? xent_blocks(dim, 4) : 1;
   XentDirect p{};
   p.x = x; p.w = w; p.labels = labels;
   p.rows = rows; p.dim = dim; p.vocab = vocab;
@@ -1151,8 +1153,6 @@ static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int6
   const uint32_t tiles = p.tiles_v * p.tiles_n, units = p.dw_units + p.dx_units;
   if (small)
     nb == 1 ? xent_small_ds<1><<<tiles, kBlock, 0, st>>>(p) : xent_small_ds<2><<<tiles, kBlock, 0, st>>>(p);
-  else if (nb == 4)
-    xent_direct_ds<4><<<tiles, kBlock, 0, st>>>(p);
   else
     nb == 1 ? xent_direct_ds<1><<<tiles, kBlock, 0, st>>>(p) : xent_direct_ds<2><<<tiles, kBlock, 0, st>>>(p);
   WF2_TRY(after_launch("xent ds"));
@@ -1161,10 +1161,7 @@ static int xent_backward_direct(XentRoute route, int64_t rows, int64_t dim, int6
   } else {
     auto with = [&](auto w_blocks) {
       constexpr int NBW = decltype(w_blocks)::value;
-      if (nbx == 4)
-        xent_direct_gradients<NBW, 4><<<units, kBlock, 0, st>>>(p);
-      else
-        nbx == 1 ? xent_direct_gradients<NBW, 1><<<units, kBlock, 0, st>>>(p) : xent_direct_gradients<NBW, 2><<<units, kBlock, 0, st>>>(p);
+      nbx == 1 ? xent_direct_gradients<NBW, 1><<<units, kBlock, 0, st>>>(p) : xent_direct_gradients<NBW, 2><<<units, kBlock, 0, st>>>(p);
     };
     if (nbw == 4)
       with(std::integral_constant<int, 4>());

@@ -314,6 +314,15 @@ def test_a_last_round_of_narrower_tiles(gpu, rows, dim, vocab, monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,vocab", [(1, 12, 33001), (40, 70, 33000), (100, 12, 33000), (64, 129, 17000)])
+def test_tiles_of_128_words(gpu, rows, dim, vocab, monkeypatch):
+    """Vocabularies long enough for every kernel of the direct products to take 128 words at a time."""
+    monkeypatch.setenv("WF2HIP_XENT_ROUTE", "1")
+    x, w, labels = inputs(rows, dim, vocab, left_out=0.1 if rows > 1 else 0.0)
+    check(gpu, x, w, labels, "mean")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,dim,vocab", [(2049, 5, 33), (9000, 12, 40)])
 @pytest.mark.parametrize("route", ["0", "1", "2"])
 @pytest.mark.parametrize("left_out", [0.3, 1.0])
